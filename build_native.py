@@ -38,6 +38,9 @@ CORE_CC = [
     "gpuexp/optional_sources.cc", "gpuexp/client.cc", "gpuexp/pmc_rounds.cc", "gpuexp/pmc_harness.cc",
     "gpuexp/pmc_agents.cc", "bindings.cc",
 ]
+# No packed fp32 arithmetic: hipcc makes v_pk_{add,mul,fma}_f32 from ordinary float code, and some of
+# their forms have given wrong results on MI355X now and then.
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SENTINEL_HIP = ["gpuexp/sentinel.hip"]
 SENTINEL_HSACO = "gpuexp/sentinel_hsaco.hip"  # device-only code object for raw AQL dispatch
 CALIB_HSACO = "kernels/calib_hsaco.hip"       # PMC calibration workloads, dispatched on the PMC queue
@@ -86,7 +89,7 @@ def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | Non
         return obj
     obj.parent.mkdir(parents=True, exist_ok=True)
     if src.suffix == ".hip":
-        cmd = [str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "-x", "hip"] + _common_flags(None)
+        cmd = [str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "-x", "hip"] + HIP_FLAGS + _common_flags(None)
         if sanitize:
             # Host-side sanitizer only: GPU ASan is not available on this pool.
             cmd += ["-Xarch_host", f"-fsanitize={sanitize}", "-fno-gpu-sanitize"]
@@ -129,7 +132,7 @@ def build_hsaco(src: str, out: Path, hdr_mtime: float, force: bool) -> Path:
         return out
     tmp = out.with_suffix(".tmp.hsaco")
     _run([str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "--cuda-device-only", "--no-gpu-bundle-output",
-          "-O3", "-std=c++17", f"-I{CSRC}", "-o", str(tmp), str(s)])
+          *HIP_FLAGS, "-O3", "-std=c++17", f"-I{CSRC}", "-o", str(tmp), str(s)])
     os.replace(tmp, out)
     return out
 
