@@ -1,0 +1,50 @@
+// Launchers of the 8-bit operators (fp8_quant.hip, gemm_fp8.hip) and their host-side rules.
+// A tensor in 8 bits is [rows][cols] bytes with a row stride `ld` (bytes); its scales are E8M0
+// bytes (2^(byte - 127)) [rows / block_rows][ceil(cols / 128)] with a row stride `lds`.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace gpuexp {
+
+enum Fp8Type { kE4M3 = 0, kE5M2 = 1 };               // also the matrix instruction's type codes
+enum WideType { kBF16 = 0, kF16 = 1, kF32 = 2 };     // types of 16 and 32 bits
+constexpr int kFp8Block = 128;
+
+struct Fp8Out {  // a tensor in 8 bits to write; q == nullptr: not wanted
+  uint8_t* q;
+  uint8_t* scale;
+  int64_t ld;
+  int64_t lds;
+};
+
+struct Fp8In {
+  const uint8_t* q;
+  const uint8_t* scale;
+  int64_t ld;
+  int64_t lds;
+  int block_rows;  // 1 or 128 rows share a scale
+  int type;        // Fp8Type
+};
+
+// out = x[rows][cols] in 8 bits; outT = its transpose [cols][rows].  block_rows 1: blocks of
+// 1 x 128 along each output's own rows; 128: blocks of 128 x 128, the transpose the same values.
+hipError_t launch_quantize_fp8(const void* x, int xtype, int64_t ldx, int64_t rows, int64_t cols, int type,
+                               int block_rows, Fp8Out out, Fp8Out outT, hipStream_t stream);
+hipError_t launch_dequantize_fp8(Fp8In in, int64_t rows, int64_t cols, void* x, int xtype, int64_t ldx,
+                                 hipStream_t stream);
+// outT = in's transpose; block_rows 1: requantised in blocks of 1 x 128 along in's rows
+hipError_t launch_transpose_fp8(Fp8In in, int64_t rows, int64_t cols, Fp8Out outT, hipStream_t stream);
+
+struct GemmFp8Args {
+  Fp8In a, b;  // [M][K], [N][K]
+  void* c;     // [M][ldc] of ctype (kBF16 or kF16)
+  int64_t ldc;
+  int64_t M, N, K;
+  int ctype;
+};
+hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream);
+
+}  // namespace gpuexp

@@ -1,0 +1,136 @@
+"""The 8-bit operators' refusals (CPU: every check comes before anything is launched)."""
+import pytest
+import torch
+
+from kubernetes_gpu_exporter_amd.ops.fp8 import dequantize_fp8, gemm_fp8, linear_fp8, quantize_fp8, transpose_fp8
+from kubernetes_gpu_exporter_amd.ops.gemm import kernels
+from tests.fp8_oracle import E4M3, E5M2, E8M0, pair, quantized, values
+
+
+def q(m, k, block_rows=1, dtype=E4M3):
+    return pair(m, k, torch.Generator().manual_seed(m * k), dtype, block_rows)
+
+
+def test_types_are_refused():
+    x = torch.zeros(4, 128)
+    with pytest.raises(TypeError, match="bfloat16, float16 or float32"):
+        quantize_fp8(x.double())
+    with pytest.raises(TypeError, match="e4m3fn or float8_e5m2"):
+        quantize_fp8(x, torch.float16)
+    a, s = q(4, 128)
+    with pytest.raises(TypeError, match="must be float8"):
+        gemm_fp8(x, s, a, s)
+    with pytest.raises(TypeError, match="e8m0"):
+        gemm_fp8(a, s.view(torch.uint8), a, s)
+    with pytest.raises(TypeError, match="writes bfloat16 or float16"):
+        gemm_fp8(a, s, a, s, out_dtype=torch.float32)
+    with pytest.raises(TypeError, match="gives bfloat16"):
+        dequantize_fp8(a, s, torch.float64)
+    with pytest.raises(TypeError, match="activations"):
+        linear_fp8(x, x)
+    with pytest.raises(TypeError, match="weights"):
+        linear_fp8(x.bfloat16(), x)
+
+
+@pytest.mark.parametrize("block_rows", [0, 2, 64, 256])
+def test_block_rows_are_refused(block_rows):
+    with pytest.raises(ValueError, match="block_rows"):
+        quantize_fp8(torch.zeros(4, 128), block_rows=block_rows)
+
+
+def test_shapes_are_refused():
+    a, s = q(4, 256)
+    b, t = q(8, 128)
+    with pytest.raises(ValueError, match="shape mismatch"):
+        gemm_fp8(a, s, b, t)
+    with pytest.raises(ValueError, match="the scales of a"):
+        gemm_fp8(a, s[:, :1], a, s)
+    with pytest.raises(ValueError, match="the scales of b"):
+        gemm_fp8(a, s, a, s[:3])
+    with pytest.raises(ValueError, match="2-dimensional"):
+        transpose_fp8(a[0], s)
+    with pytest.raises(ValueError, match="2-dimensional"):
+        quantize_fp8(torch.zeros(128))
+    with pytest.raises(ValueError, match="out must be"):
+        gemm_fp8(a, s, a, s, out=torch.zeros(4, 5, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="shape mismatch"):
+        linear_fp8(torch.zeros(2, 3, dtype=torch.bfloat16), torch.zeros(4, 5, dtype=torch.bfloat16))
+
+
+def test_layouts_are_refused():
+    a, s = q(4, 256)
+    with pytest.raises(ValueError, match="columns next to each other"):
+        quantize_fp8(torch.zeros(128, 4).T)
+    with pytest.raises(ValueError, match="columns next to each other"):
+        quantize_fp8(torch.zeros(1, 128).expand(4, 128))  # rows that overlap
+    with pytest.raises(ValueError, match="columns next to each other"):
+        transpose_fp8(a.T, q(256, 4)[1])
+    packed = torch.zeros(4 * 250, dtype=torch.uint8).view(E4M3).view(4, 250)
+    with pytest.raises(ValueError, match="multiples of 16"):
+        gemm_fp8(packed, s, packed, s)
+    shifted = torch.zeros(4 * 256 + 16, dtype=torch.uint8)[8:8 + 4 * 256].view(E4M3).view(4, 256)
+    with pytest.raises(ValueError, match="multiples of 16"):
+        gemm_fp8(shifted, s, shifted, s)
+    tight = torch.zeros(4, 2, dtype=torch.uint8).view(E8M0)
+    with pytest.raises(ValueError, match="multiples of 4"):
+        gemm_fp8(a, tight, a, tight)
+    with pytest.raises(ValueError, match="multiples of 16"):
+        gemm_fp8(a[:1].expand(4, 256), s, a, s)
+
+
+def test_weights_in_8_bits_take_no_gradient():
+    w, s = q(256, 128, 128)
+    with pytest.raises(ValueError, match="no gradient"):
+        linear_fp8(torch.zeros(2, 128, dtype=torch.bfloat16), w.clone().requires_grad_(), s)
+
+
+def test_cpu_tensors_are_refused():
+    a, s = q(4, 256)
+    for call in (lambda: quantize_fp8(torch.zeros(4, 256)), lambda: dequantize_fp8(a, s),
+                 lambda: transpose_fp8(a, s), lambda: gemm_fp8(a, s, a, s),
+                 lambda: linear_fp8(torch.zeros(4, 256).bfloat16(), torch.zeros(8, 256).bfloat16())):
+        with pytest.raises(ValueError, match="same GPU"):
+            call()
+
+
+def test_native_calls_check_addresses_and_strides(native):
+    """The native entry points turn what their vector accesses cannot take into errors, before any launch."""
+    k = kernels()
+    good = (1 << 20, 1 << 20, 128, 4, 1, 0)
+    for bad in ((1 << 20 | 8, 1 << 20, 128, 4, 1, 0), (1 << 20, 1 << 20 | 2, 128, 4, 1, 0),
+                (1 << 20, 1 << 20, 120, 4, 1, 0), (1 << 20, 1 << 20, 112, 4, 1, 0), (1 << 20, 1 << 20, 128, 0, 1, 0),
+                (1 << 20, 1 << 20, 128, 4, 2, 0), (1 << 20, 1 << 20, 128, 4, 1, 2), (0, 0, 128, 4, 1, 0)):
+        with pytest.raises(ValueError):
+            k.gemm_fp8(*bad, *good, 1 << 20, 128, 4, 4, 128, 0, 0)
+        with pytest.raises(ValueError):
+            k.gemm_fp8(*good, *bad, 1 << 20, 128, 4, 4, 128, 0, 0)
+        with pytest.raises(ValueError):
+            k.transpose_fp8(*bad, 4, 128, 1 << 20, 1 << 20, 16, 4, 0)
+        with pytest.raises(ValueError):
+            k.dequantize_fp8(*bad, 4, 128, 1 << 20, 0, 128, 0)
+    for c, ldc, ctype in ((0, 4, 0), (1 << 20, 3, 0), (1 << 20 | 1, 4, 0), (1 << 20, 4, 2)):
+        with pytest.raises(ValueError):
+            k.gemm_fp8(*good, *good, c, ldc, 4, 4, 128, ctype, 0)
+    with pytest.raises(ValueError):
+        k.quantize_fp8(1 << 20, 0, 127, 4, 128, 0, 1, 1 << 20, 1 << 20, 128, 4, 0, 0, 0, 0, 0)
+    with pytest.raises(ValueError):
+        k.quantize_fp8(1 << 20, 0, 128, 4, 128, 0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    with pytest.raises(RuntimeError):  # a launch of 2^32 threads and more
+        k.quantize_fp8(1 << 20, 0, 1 << 20, 1 << 20, 1 << 20, 0, 1, 1 << 20, 1 << 20, 1 << 20, 1 << 13, 0, 0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+def test_oracle_matches_torch_rounding(dtype):
+    """The oracle's rounding is torch's own cast where no scale applies (largest value = the type's)."""
+    x = torch.randn(64, 128, generator=torch.Generator().manual_seed(1)) * torch.logspace(-4, 2, 128)
+    x[:, 0] = 448.0 if dtype == E4M3 else 57344.0
+    got, e = quantized(x.clamp(-57344 if dtype == E5M2 else -448, 57344 if dtype == E5M2 else 448), dtype)
+    assert bool((e == 0).all())
+    assert torch.equal(got.float(), x.clamp(-57344 if dtype == E5M2 else -448, 57344 if dtype == E5M2 else 448)
+                       .to(dtype).float())
+
+
+def test_oracle_values_of_a_hand_made_pair():
+    a = torch.tensor([[1.0, -2.0, 448.0]]).to(E4M3)
+    s = torch.tensor([[128]], dtype=torch.uint8).view(E8M0)
+    assert values(a, s).tolist() == [[2.0, -4.0, 896.0]]
