@@ -14,8 +14,8 @@
 //
 // Operands are read with raw buffer loads straight into LDS: a lane whose row or 16-byte chunk is
 // past the end gets an offset past the buffer's end and reads zeros, so ragged sizes need no other
-// path; where K ends inside a 16-byte chunk the fragments of the last block are masked, so what
-// follows the last value in a row has no effect.
+// path; where K ends inside a 16-byte chunk, that chunk is a step of its own with its rest zeroed, so
+// what follows the last value in a row has no effect.
 #include "fp8_launch.h"
 
 #include <type_traits>
@@ -27,6 +27,7 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr int kBK = 128;  // bytes of K per tile: one scale block
@@ -52,26 +53,37 @@ __device__ __forceinline__ rsrc_t tile_rsrc(const Operand& o, int row0, int tile
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(o.q) + int64_t(row0) * o.ld, 0, int(bytes), 0x00020000);
 }
 
-// zeroes the bytes of a fragment whose k (within the block) is at or past `left`; the fragment is
-// two 16-byte chunks c0, c1
-__device__ __forceinline__ void mask_frag(i32x8& f, int c0, int c1, int left) {
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const int k = (w < 4 ? c0 * 16 : c1 * 16) + (w & 3) * 4;
-    const int n = left - k;  // bytes of this word that are in range
-    if (n < 4) f[w] = n <= 0 ? 0 : f[w] & int((1u << (8 * n)) - 1u);
-  }
-}
-
-template <int kA, int kB>
+// kByte: the byte of sa and sb that holds the scale
+template <int kA, int kB, int kByte = 0>
 __device__ __forceinline__ f32x4 mfma(const i32x8& a, const i32x8& b, f32x4 c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, kA, kB, 0, sa, 0, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, kA, kB, kByte, sa, kByte, sb);
 }
 
 template <typename T>
 __device__ __forceinline__ uint16_t to16(float v) {
   const T h = (T)v;
   return __builtin_bit_cast(uint16_t, h);
+}
+
+// Where K ends inside a 16-byte chunk, the tiles stop before that chunk and this fragment makes one
+// more step of it: the lanes that hold chunk 0 of `row` (others: on = false) read it with what
+// follows K zeroed, the rest is zero.
+__device__ __forceinline__ i32x8 tail_frag(rsrc_t rsrc, int64_t ld, int row, bool on, int K) {
+  const int k = K & ~15;
+  const uint32_t off = on ? uint32_t(row) * uint32_t(ld) + k : kOob;
+  i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int n = K - k - 4 * w;  // bytes of this word that count
+    if (n < 4) v[w] = n <= 0 ? 0 : v[w] & int((1u << (8 * n)) - 1u);
+  }
+  const i32x4 zero{0, 0, 0, 0};
+  return __builtin_shufflevector(v, zero, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// the scale of `row` in K's last block
+__device__ __forceinline__ int tail_scale(const Operand& o, int row, int K) {
+  row = (row < o.rows ? row : o.rows - 1) >> o.shift;
+  return o.scale[int64_t(row) * o.lds + (K - 1) / kBK];
 }
 
 // ---- 128 x 128 tile, 4 waves of 64 x 64, two tiles of K in LDS ----
@@ -85,18 +97,19 @@ gemm_fp8_128_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
   const int nbn = (B.rows + 127) / 128;
   const int row_a = int(blockIdx.x / nbn) * 128, row_b = int(blockIdx.x % nbn) * 128;
   const rsrc_t ra = tile_rsrc(A, row_a, 128, K), rb = tile_rsrc(B, row_b, 128, K);
-  const int nk = (K + kBK - 1) / kBK;
+  const int K16 = K & ~15;
+  const int nk = (K16 + kBK - 1) / kBK;
 
   auto stage = [&](int t) {
     uint8_t* buf = smem + (t & 1) * 2 * 128 * kBK;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int rblk = (wave * 4 + i) * 8, row = rblk + (lane >> 3);
-      const int k = t * kBK + swz(row, lane & 7) * 16;
-      const uint32_t oa = k < K ? uint32_t(row) * uint32_t(A.ld) + k : kOob;
-      const uint32_t ob = k < K ? uint32_t(row) * uint32_t(B.ld) + k : kOob;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(buf + rblk * kBK), 16, oa, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(buf + (128 + rblk) * kBK), 16, ob, 0, 0, 0);
+      const int rblk = (wave * 4 + i) * 8, row = rblk + (lane >> 3), chunk = swz(row, lane & 7) * 16;
+      const uint32_t oa = uint32_t(row) * uint32_t(A.ld) + chunk, ob = uint32_t(row) * uint32_t(B.ld) + chunk;
+      const bool in = t * kBK + chunk < K16;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(buf + rblk * kBK), 16, in ? oa : kOob, t * kBK, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(buf + (128 + rblk) * kBK), 16, in ? ob : kOob, t * kBK,
+                                               0, 0);
     }
   };
 
@@ -147,13 +160,21 @@ gemm_fp8_128_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
       af[i] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
       bf[i] = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    const int left = K - t * kBK;
-    if (left < kBK && (left & 15)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mask_frag(af[i], c0, c1, left);
-        mask_frag(bf[i], c0, c1, left);
-      }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma<kA, kB>(af[i], bf[j], acc[i][j], int(sa[i]), int(sb[j]));
+  }
+
+  if (K != K16) {
+    i32x8 af[4], bf[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = wm * 64 + i * 16 + (lane & 15), y = wn * 64 + i * 16 + (lane & 15);
+      af[i] = tail_frag(ra, A.ld, x, lane < 16, K);
+      bf[i] = tail_frag(rb, B.ld, y, lane < 16, K);
+      sa[i] = tail_scale(A, row_a + x, K);
+      sb[i] = tail_scale(B, row_b + y, K);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -172,6 +193,299 @@ gemm_fp8_128_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
         const int col = row_b + wn * 64 + j * 16 + (lane & 15);
         if (row < A.rows && col < B.rows) C[int64_t(row) * ldc + col] = to16<TC>(acc[i][j][r]);
       }
+}
+
+// ---- 256 x 256 tile, 8 waves, two barriers per phase ----
+// Waves are 2 along M x 4 along N, each a 128 x 64 block of C as 2 x 2 quadrants of 64 x 32; a
+// K tile (128 bytes of K) is four phases, one quadrant of 8 MFMA (256 cycles) each.  A "group" is
+// the 128 rows of a tile that one phase reads: A-M0 / A-M1 = the first / second 64 rows of each
+// wave row, B-N0 / B-N1 = the first / second 32 rows of each wave column; 16 KiB, two 16-byte loads
+// into LDS per thread.  Wave row 1 runs one barrier behind wave row 0, so that on every SIMD one
+// wave's MFMA run while the other reads LDS and issues loads.  With Bf / Bs = B-N0 / B-N1 for even
+// K tiles and the reverse for odd ones, phase p of K tile t
+//   P1  loads A-M1(t+1), reads A-M0(t),   multiplies (M0, Bf)
+//   P2  loads Bf(t+2),   reads Bs(t),     multiplies (M0, Bs)
+//   P3  loads A-M0(t+2), reads A-M1(t),   multiplies (M1, Bs)
+//   P4  loads Bs(t+2),   reads Bf(t+1),   multiplies (M1, Bf)
+// so a group's rows are loaded 2 phases after their last read in that buffer and 6 before their
+// next, and the wait in each phase (loads complete in order) retires the group issued 5 phases
+// earlier, one phase before it is read.  Past the end of K the same loads go on with every lane out
+// of range (zeros, no memory traffic), so the counts hold to the last tile.
+//
+// The rows' scales go the same way: 4 bytes hold a row's next 4 blocks, so each wave loads those of
+// 64 rows with one instruction every 4 K tiles, 4 K tiles ahead, into 2 x 2 KiB of LDS; a lane keeps
+// its 8 + 4 rows' words, and the instruction picks the byte: the K loop is unrolled by 4.
+// LDS is [A|B][buffer][256][128]: every read of an operand is then within an immediate offset (16
+// bits) of one address per chunk.
+constexpr int kTile256 = 256 * kBK;
+constexpr int kScales256 = 4 * kTile256;
+
+// gfx9 encoding: vmcnt [3:0] and [15:14], expcnt [6:4], lgkmcnt [11:8]
+constexpr int waitcnt_vm(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | (((n >> 4) & 3) << 14); }
+constexpr int kWaitLgkm0 = 0xF | (0x7 << 4) | (0x3 << 14);
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(N));
+}
+
+// every wave's counted wait is behind this barrier; this wave's LDS reads have landed
+__device__ __forceinline__ void barrier_before_mfma() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ void barrier_after_mfma() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A fragment of 32 rows x 64 k: lane l holds row l % 32 and, with g = l / 32, the chunks 2 h + g and
+// 2 h + g + 4 of the row's 8, h = 0, 1 for the two halves of a K tile.  Any assignment does that A
+// and B share, and in this one the four places are xors of each other, alike for rows 32 apart.
+struct FragAt {
+  const uint8_t *p0, *p1;  // h = 0: chunks g, g + 4
+  const uint8_t *p2, *p3;  // h = 1
+};
+__device__ __forceinline__ FragAt frag_at(const uint8_t* rows, int lane) {
+  const int at = (lane & 31) * kBK, c = swz(lane & 31, lane >> 5) * 16;
+  return {rows + at + c, rows + at + (c ^ 64), rows + at + (c ^ 32), rows + at + (c ^ 96)};
+}
+__device__ __forceinline__ void read_frag(const FragAt& f, int offset, i32x8 (&out)[2]) {
+  const i32x4 a = *reinterpret_cast<const i32x4*>(f.p0 + offset);
+  const i32x4 b = *reinterpret_cast<const i32x4*>(f.p1 + offset);
+  const i32x4 c = *reinterpret_cast<const i32x4*>(f.p2 + offset);
+  const i32x4 d = *reinterpret_cast<const i32x4*>(f.p3 + offset);
+  out[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  out[1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int kA, int kB, int kByte>
+__device__ __forceinline__ f32x16 mfma32(const i32x8& a, const i32x8& b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, kA, kB, kByte, sa, kByte, sb);
+}
+
+template <int kA, int kB, typename TC>
+__global__ void __launch_bounds__(512, 1)
+gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int vec_c) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kScales256 + 2 * 2048];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave >> 2, wc = wave & 3;
+
+  // Blocks are dealt to the 8 XCDs in turn: each XCD gets a contiguous range of tiles, ordered in
+  // groups of 4 row panels x all column panels, so the tiles that run at once share panels in its L2.
+  constexpr int kGroupM = 4;
+  const int nbn = (B.rows + 255) / 256, nbm = (A.rows + 255) / 256;
+  const int nwg = nbm * nbn;
+  const int orig = blockIdx.x;
+  const int xcd = orig & 7, q = nwg >> 3, r = nwg & 7;
+  const int wgid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (orig >> 3);
+  const int in_group = kGroupM * nbn;
+  const int first_m = (wgid / in_group) * kGroupM;
+  const int gsize = nbm - first_m < kGroupM ? nbm - first_m : kGroupM;
+  const int row_a = (first_m + (wgid % in_group) % gsize) * 256, row_b = ((wgid % in_group) / gsize) * 256;
+
+  const int K16 = K & ~15;
+  const int nk = (K16 + kBK - 1) / kBK;  // >= 2
+  const rsrc_t ra = tile_rsrc(A, row_a, 256, K), rb = tile_rsrc(B, row_b, 256, K);
+
+  // A load instruction covers 8 rows x 128 bytes; its first row is a multiple of 8 whose parity (in
+  // eights) is that of `i` below, on which the swizzle depends.  The row and K tile go into the
+  // scalar offset, which the range check counts: rows past the end read as zeros.  Chunks past K16
+  // are sent past the buffer's end.
+  const int lrow = lane >> 3;
+  const int chunk[2] = {swz(lrow, lane & 7) * 16, swz(8 + lrow, lane & 7) * 16};
+  const uint32_t va[2] = {uint32_t(lrow) * uint32_t(A.ld) + chunk[0], uint32_t(lrow) * uint32_t(A.ld) + chunk[1]};
+  const uint32_t vb[2] = {uint32_t(lrow) * uint32_t(B.ld) + chunk[0], uint32_t(lrow) * uint32_t(B.ld) + chunk[1]};
+  auto stage_a = [&](int half, int t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rb8 = wave * 2 + i;
+      const int row = (rb8 / 8) * 128 + half * 64 + (rb8 % 8) * 8;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(smem + (t & 1) * kTile256 + row * kBK), 16,
+                                               chunk[i] < K16 - t * kBK ? va[i] : kOob,
+                                               uint32_t(row) * uint32_t(A.ld) + t * kBK, 0, 0);
+    }
+  };
+  auto stage_b = [&](int half, int t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rb8 = wave * 2 + i;
+      const int row = (rb8 / 4) * 64 + half * 32 + (rb8 % 4) * 8;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(smem + (2 + (t & 1)) * kTile256 + row * kBK), 16,
+                                               chunk[i] < K16 - t * kBK ? vb[i] : kOob,
+                                               uint32_t(row) * uint32_t(B.ld) + t * kBK, 0, 0);
+    }
+  };
+  // scales: wave w < 4 loads A's rows w * 64 + lane, the others B's
+  const Operand& S = wave < 4 ? A : B;
+  int srow = (wave < 4 ? row_a : row_b) + (wave & 3) * 64 + lane;
+  srow = (srow < S.rows ? srow : S.rows - 1) >> S.shift;
+  const uint8_t* sptr = S.scale + int64_t(srow) * S.lds;
+  const int quads = (nk + 3) / 4;
+  auto stage_scales = [&](int quad) {  // the words of K tiles quad * 4 .. + 4; past the end the last again
+    typedef __attribute__((address_space(1))) void* gptr_t;
+    __builtin_amdgcn_global_load_lds((gptr_t)(sptr + (quad < quads ? quad : quads - 1) * 4),
+                                     (lds_ptr_t)(smem + kScales256 + (quad & 1) * 2048 + wave * 256), 4, 0, 0);
+  };
+
+  f32x16 acc[2][2][2];  // [m half][n half][32 rows of A], each 32 columns of C x 32 rows
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[a][b][i][e] = 0.f;
+  i32x8 af[2][2], b0[2], b1[2];  // [32 rows][k half]
+  uint32_t sa[4], sb[2];
+  const FragAt a_at = frag_at(smem + wr * 128 * kBK, lane), b_at = frag_at(smem + 2 * kTile256 + wc * 64 * kBK, lane);
+
+  stage_scales(0);
+  stage_b(0, 0); stage_a(0, 0); stage_b(1, 0); stage_a(1, 0);
+  stage_b(1, 1); stage_a(0, 1); stage_b(0, 1);
+  wait_vm<6>();
+  __builtin_amdgcn_s_barrier();
+  if (wr == 1) __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  read_frag(b_at, 0, b0);
+
+  // B is the first operand, so that a lane's results lie along a row of C: 4 columns next to each
+  // other.  (The two halves of K chain through an accumulator, so they are two MFMA apart.)
+  auto quadrant = [&](f32x16 (&c)[2], const i32x8 (&bf)[2], int m, int n, auto byte_tag) {
+    constexpr int byte = decltype(byte_tag)::value;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        c[i] = mfma32<kB, kA, byte>(bf[h], af[i][h], c[i], int(sb[n]), int(sa[m * 2 + i]));
+  };
+  auto read_a = [&](int buf, int half) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) read_frag(a_at, buf * kTile256 + (half * 64 + i * 32) * kBK, af[i]);
+  };
+  auto read_b = [&](int buf, int half, i32x8 (&bf)[2]) { read_frag(b_at, buf * kTile256 + half * 32 * kBK, bf); };
+
+  auto tile = [&](int t, auto byte_tag) {  // byte: t % 4
+    constexpr int byte = decltype(byte_tag)::value;
+    constexpr bool odd = byte & 1;
+    constexpr int cur = byte & 1;
+    // P1
+    if constexpr (byte == 0) {
+      const uint8_t* sc = smem + kScales256 + ((t >> 2) & 1) * 2048 + (lane & 31) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(sc + (wr * 128 + i * 32) * 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sb[i] = *reinterpret_cast<const uint32_t*>(sc + 1024 + (wc * 64 + i * 32) * 4);
+      stage_scales((t >> 2) + 1);
+    }
+    stage_a(1, t + 1);
+    read_a(cur, 0);
+    wait_vm<10>();
+    barrier_before_mfma();
+    if constexpr (odd) quadrant(acc[0][1], b1, 0, 1, byte_tag); else quadrant(acc[0][0], b0, 0, 0, byte_tag);
+    barrier_after_mfma();
+    // P2
+    stage_b(odd ? 1 : 0, t + 2);
+    if constexpr (odd) read_b(cur, 0, b0); else read_b(cur, 1, b1);
+    wait_vm<10>();
+    barrier_before_mfma();
+    if constexpr (odd) quadrant(acc[0][0], b0, 0, 0, byte_tag); else quadrant(acc[0][1], b1, 0, 1, byte_tag);
+    barrier_after_mfma();
+    // P3
+    stage_a(0, t + 2);
+    read_a(cur, 1);
+    wait_vm<10>();
+    barrier_before_mfma();
+    if constexpr (odd) quadrant(acc[1][0], b0, 1, 0, byte_tag); else quadrant(acc[1][1], b1, 1, 1, byte_tag);
+    barrier_after_mfma();
+    // P4 (after the last tile the read finds what an earlier tile left; nothing uses it)
+    stage_b(odd ? 0 : 1, t + 2);
+    if constexpr (odd) read_b(1 - cur, 0, b0); else read_b(1 - cur, 1, b1);
+    wait_vm<10>();
+    barrier_before_mfma();
+    if constexpr (odd) quadrant(acc[1][1], b1, 1, 1, byte_tag); else quadrant(acc[1][0], b0, 1, 0, byte_tag);
+    barrier_after_mfma();
+  };
+  for (int t = 0;; t += 4) {
+    tile(t, std::integral_constant<int, 0>{});
+    if (t + 1 >= nk) break;
+    tile(t + 1, std::integral_constant<int, 1>{});
+    if (t + 2 >= nk) break;
+    tile(t + 2, std::integral_constant<int, 2>{});
+    if (t + 3 >= nk) break;
+    tile(t + 3, std::integral_constant<int, 3>{});
+    if (t + 4 >= nk) break;
+  }
+  if (wr == 0) __builtin_amdgcn_s_barrier();  // wave row 1 is one barrier behind
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();  // no load in flight, every wave's reads done: LDS is free
+
+  if (K != K16) {
+    i32x8 at[4], bt[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = wr * 128 + i * 32 + (lane & 31);
+      at[i] = tail_frag(ra, A.ld, row, lane < 32, K);
+      sa[i] = tail_scale(A, row_a + row, K);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int row = wc * 64 + n * 32 + (lane & 31);
+      bt[n] = tail_frag(rb, B.ld, row, lane < 32, K);
+      sb[n] = tail_scale(B, row_b + row, K);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[i >> 1][n][i & 1] = mfma32<kB, kA, 0>(bt[n], at[i], acc[i >> 1][n][i & 1], int(sb[n]), int(sa[i]));
+  }
+
+  // C through LDS (128 KiB), so that every global store is 16 bytes of a row.  D of 32x32x64: column
+  // (here a row of C) = lane % 32, row (a column of C) = (e / 4) * 8 + (lane / 32) * 4 + e % 4: a lane
+  // writes 8 bytes, the two halves of a wave the two halves of 16-byte chunks, which are xored with the
+  // row so that 32 rows fall into different banks.
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = wr * 128 + m * 64 + i * 32 + (lane & 31);
+          const int c = wc * 8 + n * 4 + e;
+          const f32x16& v = acc[m][n][i];
+          typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+          const u32x2 w{uint32_t(to16<TC>(v[4 * e])) | (uint32_t(to16<TC>(v[4 * e + 1])) << 16),
+                        uint32_t(to16<TC>(v[4 * e + 2])) | (uint32_t(to16<TC>(v[4 * e + 3])) << 16)};
+          *reinterpret_cast<u32x2*>(smem + row * 512 + ((c ^ (lane & 31)) << 4) + (lane >> 5) * 8) = w;
+        }
+  __syncthreads();
+#pragma unroll 4
+  for (int p = 0; p < 16; ++p) {
+    const int idx = p * 512 + threadIdx.x;
+    const int row = idx >> 5, c = idx & 31;
+    if (row_a + row >= A.rows) break;
+    const i32x4 v = *reinterpret_cast<const i32x4*>(smem + row * 512 + ((c ^ (row & 31)) << 4));
+    const int col = row_b + c * 8;
+    uint16_t* dst = C + int64_t(row_a + row) * ldc + col;
+    if (vec_c && col + 8 <= B.rows) {
+      __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(dst));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < B.rows) dst[e] = uint16_t(uint32_t(v[e >> 1]) >> (16 * (e & 1)));
+    }
+  }
 }
 
 Operand operand(const Fp8In& in, int64_t rows) {
@@ -201,15 +515,33 @@ bool side_ok(const Fp8In& in, int64_t rows, int64_t K) {
 
 }  // namespace
 
+int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
+  if (variant < 0 || variant > 2) return -1;
+  const int64_t tiles256 = ((M + 255) / 256) * ((N + 255) / 256);
+  if (variant == 2) return K >= kBK + 16 ? 2 : -1;  // two K tiles
+  if (variant == 0) return K >= kBK + 16 && tiles256 >= 64 ? 2 : 1;
+  return variant;
+}
+
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   if (g.M < 0 || g.N < 0 || g.K < 0 || !side_ok(g.a, g.M, g.K) || !side_ok(g.b, g.N, g.K)) return hipErrorInvalidValue;
   if (g.M == 0 || g.N == 0) return hipSuccess;
-  const int64_t tiles = ((g.M + 127) / 128) * ((g.N + 127) / 128);
-  if (tiles >= (int64_t(1) << 24)) return hipErrorInvalidValue;  // 2^32 threads
+  const int variant = resolve_gemm_fp8_variant(g.M, g.N, g.K, g.variant);
+  if (variant < 0) return hipErrorInvalidValue;
+  const int64_t edge = variant == 2 ? 256 : 128;
+  const int64_t tiles = ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
+  if (tiles >= (int64_t(1) << 23)) return hipErrorInvalidValue;  // 2^32 threads
+  const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc % 8 == 0;
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
-    hipLaunchKernelGGL((gemm_fp8_128_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(256), 0, stream,
-                       operand(g.a, g.M), operand(g.b, g.N), static_cast<uint16_t*>(g.c), g.ldc, int(g.K));
+    const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
+    uint16_t* c = static_cast<uint16_t*>(g.c);
+    if (variant == 2)
+      hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
+                         c, g.ldc, int(g.K), vec_c);
+    else
+      hipLaunchKernelGGL((gemm_fp8_128_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob,
+                         c, g.ldc, int(g.K));
   });
   return hipGetLastError();
 }

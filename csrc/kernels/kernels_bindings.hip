@@ -158,8 +158,10 @@ PYBIND11_MODULE(_gpuexp_kernels, m) {
   }, "The transpose of an 8-bit tensor; blocks of 1 x 128 are quantised anew along its own rows");
   m.def("gemm_fp8", [](uintptr_t a, uintptr_t sa, int64_t lda, int64_t ldsa, int block_a, int type_a, uintptr_t b,
                        uintptr_t sb, int64_t ldb, int64_t ldsb, int block_b, int type_b, uintptr_t c, int64_t ldc,
-                       int64_t M, int64_t N, int64_t K, int ctype, uintptr_t stream) {
+                       int64_t M, int64_t N, int64_t K, int ctype, uintptr_t stream, int variant) {
     gpuexp::GemmFp8Args g{};
+    if (gpuexp::resolve_gemm_fp8_variant(M, N, K, variant) < 0)
+      throw std::invalid_argument("gemm_fp8: variant is 0 (auto), 1 (128x128) or 2 (256x256, K >= 144)");
     g.a = fp8_in(a, sa, lda, ldsa, block_a, type_a, M, K);
     g.b = fp8_in(b, sb, ldb, ldsb, block_b, type_b, N, K);
     if (!c || ldc < N || c % 2 || (ctype != 0 && ctype != 1))
@@ -170,8 +172,14 @@ PYBIND11_MODULE(_gpuexp_kernels, m) {
     g.N = N;
     g.K = K;
     g.ctype = ctype;
+    g.variant = variant;
     check(gpuexp::launch_gemm_fp8(g, reinterpret_cast<hipStream_t>(stream)), "gemm_fp8 launch");
-  }, "C[M,N] = A[M,K] @ B[N,K]^T; 8-bit operands with block scales, fp32 accumulate (scaled MFMA 16x16x128)");
+  }, "C[M,N] = A[M,K] @ B[N,K]^T; 8-bit operands with block scales, fp32 accumulate (scaled MFMA). The last argument, "
+     "variant: 0 auto, 1 = 128x128 tile, 2 = 256x256 tile");
+  m.def("gemm_fp8_variant", &gpuexp::resolve_gemm_fp8_variant, py::arg("M"), py::arg("N"), py::arg("K"),
+        py::arg("variant") = 0,
+        "The kernel variant a gemm_fp8 call with these sizes runs (0 = auto resolved), -1 if they do not fit it. "
+        "Host-only: no GPU needed.");
   m.def("gemm_burn", [](int device, int M, int N, int K, double seconds, int iters_per_sync, int variant) {
     // Torch-free synthetic GEMM pod: keeps one GPU busy for `seconds` and reports the
     // achieved bf16 TFLOP/s (random operands).

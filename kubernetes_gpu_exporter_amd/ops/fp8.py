@@ -196,12 +196,13 @@ def transpose_fp8(q, scale, stream=None):
     return qt, st
 
 
-def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=None):
+def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=None, variant: int = 0):
     """out[M, N] = a[M, K] @ b[N, K]^T for operands in 8 bits with their block scales; each may be
     e4m3 or e5m2 and have blocks of 1 x 128 or 128 x 128.  Any M, N, K >= 0 (K = 0 gives zeros).
     Sums are held in 32 bits and rounded once into bf16 or f16 (`out_dtype`, or `out`'s type; `out`
     needs its columns next to each other, its rows may be further apart).  The matrix instruction
-    drops a product 2^-14 and more below the largest of the 32 it adds at once."""
+    drops a product 2^-14 and more below the largest of the 32 it adds at once.  variant 0 picks the
+    kernel by the sizes; 1 / 2 force the 128x128 / 256x256 tile (the latter for K >= 144)."""
     oa, ob = _operand("a", a, a_scale), _operand("b", b, b_scale)
     (M, K), N = a.shape, b.shape[0]
     if b.shape[1] != K:
@@ -215,13 +216,13 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=
     device = _gpu("gemm_fp8", a, a_scale, b, b_scale, *([] if out is None else [out]))
     if stream is not None:
         with _elsewhere(stream, a, a_scale, b, b_scale, *([] if out is None else [out])):
-            return gemm_fp8(a, a_scale, b, b_scale, out, out_dtype)
+            return gemm_fp8(a, a_scale, b, b_scale, out, out_dtype, variant=variant)
     if out is None:
         out = torch.empty((M, N), dtype=dtype, device=device)
     if M and N:
         raw, guard = _on(device)
         with guard:
-            kernels().gemm_fp8(*oa, *ob, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K, _WIDE[dtype], raw)
+            kernels().gemm_fp8(*oa, *ob, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K, _WIDE[dtype], raw, variant)
     return out
 
 

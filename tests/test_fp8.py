@@ -101,16 +101,19 @@ def test_native_calls_check_addresses_and_strides(native):
                 (1 << 20, 1 << 20, 120, 4, 1, 0), (1 << 20, 1 << 20, 112, 4, 1, 0), (1 << 20, 1 << 20, 128, 0, 1, 0),
                 (1 << 20, 1 << 20, 128, 4, 2, 0), (1 << 20, 1 << 20, 128, 4, 1, 2), (0, 0, 128, 4, 1, 0)):
         with pytest.raises(ValueError):
-            k.gemm_fp8(*bad, *good, 1 << 20, 128, 4, 4, 128, 0, 0)
+            k.gemm_fp8(*bad, *good, 1 << 20, 128, 4, 4, 128, 0, 0, 0)
         with pytest.raises(ValueError):
-            k.gemm_fp8(*good, *bad, 1 << 20, 128, 4, 4, 128, 0, 0)
+            k.gemm_fp8(*good, *bad, 1 << 20, 128, 4, 4, 128, 0, 0, 0)
         with pytest.raises(ValueError):
             k.transpose_fp8(*bad, 4, 128, 1 << 20, 1 << 20, 16, 4, 0)
         with pytest.raises(ValueError):
             k.dequantize_fp8(*bad, 4, 128, 1 << 20, 0, 128, 0)
     for c, ldc, ctype in ((0, 4, 0), (1 << 20, 3, 0), (1 << 20 | 1, 4, 0), (1 << 20, 4, 2)):
         with pytest.raises(ValueError):
-            k.gemm_fp8(*good, *good, c, ldc, 4, 4, 128, ctype, 0)
+            k.gemm_fp8(*good, *good, c, ldc, 4, 4, 128, ctype, 0, 0)
+    for variant in (-1, 2, 99):  # 2, the 256x256 tile, takes K >= 144
+        with pytest.raises(ValueError, match="variant"):
+            k.gemm_fp8(*good, *good, 1 << 20, 4, 4, 4, 128, 0, 0, variant)
     with pytest.raises(ValueError):
         k.quantize_fp8(1 << 20, 0, 127, 4, 128, 0, 1, 1 << 20, 1 << 20, 128, 4, 0, 0, 0, 0, 0)
     with pytest.raises(ValueError):
