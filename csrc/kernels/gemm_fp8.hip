@@ -488,6 +488,131 @@ gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
   }
 }
 
+// ---- few rows of A (one token to 64): B is read once, from memory straight into registers ----
+// Bound by B's bytes.  A block takes 16 * kR rows of B and all of A's (kMT tiles of 16); its waves
+// divide K in units of 512 bytes (four scale blocks: a row's four scales are one word, and 8 KiB of B
+// per 16 rows are in flight per wave and the next 8 KiB behind them).  A comes from the caches.  The
+// waves' sums are joined in LDS in the waves' order, so results do not depend on timing.
+// B is the matrix instruction's first operand: a lane then holds 4 columns of C next to each other.
+constexpr int kQuad = 4 * kBK;
+
+template <int kA, int kB, int kMT, int kR>
+__global__ void __launch_bounds__(1024)
+gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int c_is_f16, int vec_c) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t dyn_smem[];
+  f32x4* part = reinterpret_cast<f32x4*>(dyn_smem);  // [wave][kMT * kR][lane]
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int row_b = blockIdx.x * (16 * kR);
+  const int K16 = K & ~15;
+  const int nk = (K16 + kBK - 1) / kBK, quads = (nk + 3) / 4;
+  const int q0 = quads * wave / waves, q1 = quads * (wave + 1) / waves;
+  const rsrc_t ra = tile_rsrc(A, 0, kMT * 16, K), rb = tile_rsrc(B, row_b, 16 * kR, K);
+  const int l15 = lane & 15, chunk = (lane >> 4) * 16;  // this lane's chunks of a block: chunk, chunk + 64
+
+  const uint32_t* psb[kR];
+  const uint32_t* psa[kMT];
+#pragma unroll
+  for (int r = 0; r < kR; ++r) {
+    int n = row_b + r * 16 + l15;
+    n = (n < B.rows ? n : B.rows - 1) >> B.shift;
+    psb[r] = reinterpret_cast<const uint32_t*>(B.scale + int64_t(n) * B.lds);
+  }
+#pragma unroll
+  for (int m = 0; m < kMT; ++m) {
+    int n = m * 16 + l15;
+    n = (n < A.rows ? n : A.rows - 1) >> A.shift;
+    psa[m] = reinterpret_cast<const uint32_t*>(A.scale + int64_t(n) * A.lds);
+  }
+  // one scale block (128 bytes of K) of 16 rows; past K16 zeros
+  auto load = [&](rsrc_t rsrc, int64_t ld, int row, int k) {
+    const uint32_t at = uint32_t(row) * uint32_t(ld) + chunk;
+    const i32x4 lo = __builtin_bit_cast(
+        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk < K16 - k ? at : kOob, k, 0));
+    const i32x4 hi = __builtin_bit_cast(
+        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk + 64 < K16 - k ? at + 64 : kOob, k, 0));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto load_quad = [&](int q, i32x8 (&b)[kR][4], uint32_t (&sb)[kR], uint32_t (&sa)[kMT]) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[r][i] = load(rb, B.ld, r * 16 + l15, q * kQuad + i * kBK);
+#pragma unroll
+    for (int r = 0; r < kR; ++r) sb[r] = psb[r][q];
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) sa[m] = psa[m][q];
+  };
+
+  f32x4 acc[kMT][kR];
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int r = 0; r < kR; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  i32x8 b[kR][4], b_next[kR][4];
+  uint32_t sb[kR], sa[kMT], sb_next[kR], sa_next[kMT];
+  if (q0 < q1) load_quad(q0, b, sb, sa);
+  for (int q = q0; q < q1; ++q) {
+    if (q + 1 < q1) load_quad(q + 1, b_next, sb_next, sa_next);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = q * kQuad + i * kBK;
+      if (k < K16) {  // (behind K the scales are whatever pads their rows)
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) {
+          const i32x8 a = load(ra, A.ld, m * 16 + l15, k);
+#pragma unroll
+          for (int r = 0; r < kR; ++r)
+            acc[m][r] = mfma<kB, kA>(b[r][i], a, acc[m][r], int(sb[r] >> (8 * i)), int(sa[m] >> (8 * i)));
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[r][i] = b_next[r][i];
+      sb[r] = sb_next[r];
+    }
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) sa[m] = sa_next[m];
+  }
+  if (K != K16 && wave == waves - 1) {
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) {
+      const i32x8 a = tail_frag(ra, A.ld, m * 16 + l15, lane < 16, K);
+      const int s = tail_scale(A, m * 16 + l15, K);
+#pragma unroll
+      for (int r = 0; r < kR; ++r)
+        acc[m][r] = mfma<kB, kA>(tail_frag(rb, B.ld, r * 16 + l15, lane < 16, K), a, acc[m][r],
+                                 tail_scale(B, row_b + r * 16 + l15, K), s);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int r = 0; r < kR; ++r) part[(wave * kMT * kR + m * kR + r) * 64 + lane] = acc[m][r];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kMT * kR * 64; i += blockDim.x) {
+    f32x4 v = part[i];
+    for (int w = 1; w < waves; ++w) v += part[w * kMT * kR * 64 + i];
+    const int l = i & 63, m = i / 64 / kR, r = i / 64 % kR;
+    const int row = m * 16 + (l & 15), col = row_b + r * 16 + (l >> 4) * 4;
+    if (row >= A.rows) continue;
+    uint16_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = c_is_f16 ? to16<_Float16>(v[e]) : to16<__bf16>(v[e]);
+    uint16_t* dst = C + int64_t(row) * ldc + col;
+    if (vec_c && col + 4 <= B.rows) {
+      typedef __attribute__((ext_vector_type(4))) uint16_t u16x4;
+      *reinterpret_cast<u16x4*>(dst) = u16x4{h[0], h[1], h[2], h[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < B.rows) dst[e] = h[e];
+    }
+  }
+}
+
 Operand operand(const Fp8In& in, int64_t rows) {
   return {in.q, in.scale, in.ld, in.lds, int(rows), in.block_rows == 1 ? 0 : 7};
 }
@@ -515,13 +640,30 @@ bool side_ok(const Fp8In& in, int64_t rows, int64_t K) {
 
 }  // namespace
 
+// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows; -1: not these sizes.
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
-  if (variant < 0 || variant > 2) return -1;
+  if (variant < 0 || variant > 3) return -1;
   const int64_t tiles256 = ((M + 255) / 256) * ((N + 255) / 256);
   if (variant == 2) return K >= kBK + 16 ? 2 : -1;  // two K tiles
-  if (variant == 0) return K >= kBK + 16 && tiles256 >= 64 ? 2 : 1;
+  if (variant == 3) return M <= 64 ? 3 : -1;
+  if (variant == 0) return M <= 64 ? 3 : K >= kBK + 16 && tiles256 >= 64 ? 2 : 1;
   return variant;
 }
+
+namespace {
+
+template <int a, int b, int kMT, int kR>
+void launch_rows(const GemmFp8Args& g, Operand oa, Operand ob, hipStream_t stream) {
+  const int64_t quads = ((g.K & ~int64_t(15)) + kQuad - 1) / kQuad;
+  int waves = 1;
+  while (waves < 8 && waves * 2 <= quads) waves *= 2;
+  const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 8 == 0 && g.ldc % 4 == 0;
+  hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kMT, kR>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
+                     dim3(waves * 64), waves * kMT * kR * 64 * sizeof(f32x4), stream, oa, ob,
+                     static_cast<uint16_t*>(g.c), g.ldc, int(g.K), g.ctype == kF16, vec_c);
+}
+
+}  // namespace
 
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   if (g.M < 0 || g.N < 0 || g.K < 0 || !side_ok(g.a, g.M, g.K) || !side_ok(g.b, g.N, g.K)) return hipErrorInvalidValue;
@@ -529,19 +671,24 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   const int variant = resolve_gemm_fp8_variant(g.M, g.N, g.K, g.variant);
   if (variant < 0) return hipErrorInvalidValue;
   const int64_t edge = variant == 2 ? 256 : 128;
-  const int64_t tiles = ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
-  if (tiles >= (int64_t(1) << 23)) return hipErrorInvalidValue;  // 2^32 threads
+  const int64_t tiles = variant == 3 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
+  if (tiles >= (int64_t(1) << 22)) return hipErrorInvalidValue;  // 2^32 threads
   const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc % 8 == 0;
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
     const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
     uint16_t* c = static_cast<uint16_t*>(g.c);
-    if (variant == 2)
+    if (variant == 3) {
+      if (g.M <= 16) launch_rows<a, b, 1, 1>(g, oa, ob, stream);
+      else if (g.M <= 32) launch_rows<a, b, 2, 1>(g, oa, ob, stream);
+      else launch_rows<a, b, 4, 1>(g, oa, ob, stream);
+    } else if (variant == 2) {
       hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
                          c, g.ldc, int(g.K), vec_c);
-    else
+    } else {
       hipLaunchKernelGGL((gemm_fp8_128_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob,
                          c, g.ldc, int(g.K));
+    }
   });
   return hipGetLastError();
 }
