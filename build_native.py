@@ -44,8 +44,8 @@ HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SENTINEL_HIP = ["gpuexp/sentinel.hip"]
 SENTINEL_HSACO = "gpuexp/sentinel_hsaco.hip"  # device-only code object for raw AQL dispatch
 CALIB_HSACO = "kernels/calib_hsaco.hip"       # PMC calibration workloads, dispatched on the PMC queue
-KERNELS_HIP = ["kernels/gemm_bf16.hip", "kernels/fp8_quant.hip", "kernels/gemm_fp8.hip", "kernels/probe_kernels.hip",
-               "kernels/kernels_bindings.hip"]
+KERNELS_HIP = ["kernels/gemm_bf16.hip", "kernels/fp8_quant.hip", "kernels/gemm_fp8.hip", "kernels/linear_fp8.hip",
+               "kernels/probe_kernels.hip", "kernels/kernels_bindings.hip"]
 ROCPROF_CC = ["gpuexp/rocprof_plugin.cc"]
 AQLPMC_CC = ["gpuexp/aql_pmc.cc"]
 TRACER_CC = ["gpuexp/rccl_tracer.cc"]

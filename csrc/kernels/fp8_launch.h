@@ -50,4 +50,30 @@ struct GemmFp8Args {
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant);
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream);
 
+// y[M][N] = x[M][K] . w[N][K]^T in 8 bits and its backward pass, several launches behind one call.
+// Two workspaces in device memory: `kept` holds between the passes what the backward pass reads (x in
+// 8 bits if dw is wanted, the transposed weight in 8 bits if dx is), `temp` only during a pass.
+struct LinearFp8Args {
+  int64_t M, N, K;
+  bool want_dx, want_dw;
+  const void* x;  // [M][ldx], type
+  int64_t ldx;
+  const void* w;  // [N][ldw], wtype; not read by the backward pass
+  int64_t ldw;
+  int type, wtype;  // of x, y and their gradients, and of w and dw: kBF16 or kF16
+  uint8_t* kept;
+  uint8_t* temp;
+};
+struct LinearFp8Bytes {
+  int64_t kept, forward_temp, backward_temp;
+};
+LinearFp8Bytes linear_fp8_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);
+hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream);
+hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
+                                      hipStream_t stream);
+// the same with a weight that is in 8 bits already; temp: x in 8 bits (serve_fp8_bytes)
+int64_t serve_fp8_bytes(int64_t M, int64_t N, int64_t K);
+hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
+                            uint8_t* temp, hipStream_t stream);
+
 }  // namespace gpuexp

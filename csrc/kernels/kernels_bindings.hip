@@ -50,6 +50,24 @@ gpuexp::Fp8Out fp8_out(uintptr_t q, uintptr_t scale, int64_t ld, int64_t lds, in
   return {reinterpret_cast<uint8_t*>(q), reinterpret_cast<uint8_t*>(scale), ld, lds};
 }
 
+gpuexp::LinearFp8Args linear_args(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw, int type, int wtype,
+                                  uintptr_t kept, uintptr_t temp) {
+  if (M < 0 || N < 0 || K < 0 || type < 0 || type > 1 || wtype < 0 || wtype > 1)
+    throw std::invalid_argument("linear_fp8: sizes >= 0, types 0 (bf16) or 1 (f16)");
+  if (kept % 256 || temp % 256) throw std::invalid_argument("linear_fp8: workspaces start at multiples of 256 bytes");
+  gpuexp::LinearFp8Args a{};
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.want_dx = want_dx;
+  a.want_dw = want_dw;
+  a.type = type;
+  a.wtype = wtype;
+  a.kept = reinterpret_cast<uint8_t*>(kept);
+  a.temp = reinterpret_cast<uint8_t*>(temp);
+  return a;
+}
+
 }  // namespace
 
 // Separate module from the telemetry core: it links a HIP runtime, so it is imported
@@ -158,7 +176,7 @@ PYBIND11_MODULE(_gpuexp_kernels, m) {
   }, "The transpose of an 8-bit tensor; blocks of 1 x 128 are quantised anew along its own rows");
   m.def("gemm_fp8", [](uintptr_t a, uintptr_t sa, int64_t lda, int64_t ldsa, int block_a, int type_a, uintptr_t b,
                        uintptr_t sb, int64_t ldb, int64_t ldsb, int block_b, int type_b, uintptr_t c, int64_t ldc,
-                       int64_t M, int64_t N, int64_t K, int ctype, uintptr_t stream, int variant) {
+                       int64_t M, int64_t N, int64_t K, int ctype, int variant, uintptr_t stream) {
     gpuexp::GemmFp8Args g{};
     if (gpuexp::resolve_gemm_fp8_variant(M, N, K, variant) < 0)
       throw std::invalid_argument("gemm_fp8: variant is 0 (auto), 1 (128x128), 2 (256x256, K >= 144) or 3 (few rows, M <= 64)");
@@ -174,12 +192,51 @@ PYBIND11_MODULE(_gpuexp_kernels, m) {
     g.ctype = ctype;
     g.variant = variant;
     check(gpuexp::launch_gemm_fp8(g, reinterpret_cast<hipStream_t>(stream)), "gemm_fp8 launch");
-  }, "C[M,N] = A[M,K] @ B[N,K]^T; 8-bit operands with block scales, fp32 accumulate (scaled MFMA). The last argument, "
-     "variant: 0 auto, 1 = 128x128 tile, 2 = 256x256 tile, 3 = few rows");
+  }, "C[M,N] = A[M,K] @ B[N,K]^T; 8-bit operands with block scales, fp32 accumulate (scaled MFMA). The last argument but "
+     "the stream, variant: 0 auto, 1 = 128x128 tile, 2 = 256x256 tile, 3 = few rows");
   m.def("gemm_fp8_variant", &gpuexp::resolve_gemm_fp8_variant, py::arg("M"), py::arg("N"), py::arg("K"),
         py::arg("variant") = 0,
         "The kernel variant a gemm_fp8 call with these sizes runs (0 = auto resolved), -1 if they do not fit it. "
         "Host-only: no GPU needed.");
+  m.def("linear_fp8_bytes", [](int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
+    if (M < 0 || N < 0 || K < 0) throw std::invalid_argument("linear_fp8: sizes >= 0");
+    const gpuexp::LinearFp8Bytes b = gpuexp::linear_fp8_bytes(M, N, K, want_dx, want_dw);
+    return py::make_tuple(b.kept, b.forward_temp, b.backward_temp);
+  }, "Bytes of the workspaces of a linear layer in 8 bits: (kept between the passes, forward, backward)");
+  m.def("linear_fp8_forward", [](int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw, uintptr_t x, int64_t ldx,
+                                 int type, uintptr_t w, int64_t ldw, int wtype, uintptr_t kept, uintptr_t temp,
+                                 uintptr_t y, uintptr_t stream) {
+    gpuexp::LinearFp8Args a = linear_args(M, N, K, want_dx, want_dw, type, wtype, kept, temp);
+    if ((M && K && (!x || ldx < K)) || (N && K && (!w || ldw < K)) || (M && N && !y))
+      throw std::invalid_argument("linear_fp8_forward: null pointer, or rows that overlap");
+    a.x = reinterpret_cast<const void*>(x);
+    a.ldx = ldx;
+    a.w = reinterpret_cast<const void*>(w);
+    a.ldw = ldw;
+    check(gpuexp::launch_linear_fp8_forward(a, reinterpret_cast<void*>(y), reinterpret_cast<hipStream_t>(stream)),
+          "linear_fp8 forward launch");
+  }, "y[M,N] = x[M,K] @ w[N,K]^T in 8 bits (types 0 bf16, 1 f16); `kept` holds what the backward pass needs");
+  m.def("linear_fp8_backward", [](int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw, uintptr_t dy,
+                                  int64_t lddy, int type, int wtype, uintptr_t kept, uintptr_t temp, uintptr_t dx,
+                                  uintptr_t dw, uintptr_t stream) {
+    const gpuexp::LinearFp8Args a = linear_args(M, N, K, want_dx, want_dw, type, wtype, kept, temp);
+    if ((M && N && (!dy || lddy < N)) || (want_dx && M && K && !dx) || (want_dw && N && K && !dw))
+      throw std::invalid_argument("linear_fp8_backward: null pointer, or rows that overlap");
+    check(gpuexp::launch_linear_fp8_backward(a, reinterpret_cast<const void*>(dy), lddy, reinterpret_cast<void*>(dx),
+                                             reinterpret_cast<void*>(dw), reinterpret_cast<hipStream_t>(stream)),
+          "linear_fp8 backward launch");
+  }, "dx[M,K] and / or dw[N,K] of linear_fp8_forward");
+  m.def("serve_fp8_bytes", &gpuexp::serve_fp8_bytes, "Bytes of serve_fp8's workspace");
+  m.def("serve_fp8", [](uintptr_t x, int type, int64_t ldx, uintptr_t w, uintptr_t scale, int64_t ld, int64_t lds,
+                        int block_rows, int wtype, int64_t M, int64_t N, int64_t K, uintptr_t y, uintptr_t temp,
+                        uintptr_t stream) {
+    const gpuexp::Fp8In in = fp8_in(w, scale, ld, lds, block_rows, wtype, N, K);
+    if (M < 0 || type < 0 || type > 1 || (M && K && (!x || ldx < K)) || (M && N && !y) || temp % 256)
+      throw std::invalid_argument("serve_fp8: types 0-1, rows that do not overlap, a workspace at a multiple of 256");
+    check(gpuexp::launch_serve_fp8(reinterpret_cast<const void*>(x), type, ldx, in, M, N, K, reinterpret_cast<void*>(y),
+                                   reinterpret_cast<uint8_t*>(temp), reinterpret_cast<hipStream_t>(stream)),
+          "serve_fp8 launch");
+  }, "y[M,N] = x[M,K] @ w[N,K]^T; x bf16 / f16 is quantised on the way, w is in 8 bits");
   m.def("gemm_burn", [](int device, int M, int N, int K, double seconds, int iters_per_sync, int variant) {
     // Torch-free synthetic GEMM pod: keeps one GPU busy for `seconds` and reports the
     // achieved bf16 TFLOP/s (random operands).

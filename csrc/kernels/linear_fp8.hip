@@ -1,0 +1,96 @@
+// A linear layer in 8 bits: what its passes launch, and where in two workspaces they keep it.
+//   forward    x -> Q(x) (kept if the weight takes a gradient), w -> Q(w) and its transpose (kept if x
+//              takes one), y = Q(x) Q(w)^T
+//   backward   dy -> Q(dy) and Q(dy^T) in one pass over dy, dx = Q(dy) Q(w), dw = Q(dy^T) T(Q(x))^T
+//              with T the kept x transposed and requantised along the tokens
+// Host code only; one call from Python per pass, since a small step is bound by the host.
+#include "fp8_launch.h"
+
+namespace gpuexp {
+
+namespace {
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// a tensor in 8 bits inside a workspace: values, then scales
+struct Piece {
+  int64_t rows, cols, at;
+  int block_rows;
+  int64_t ld() const { return up(cols, 16); }
+  int64_t lds() const { return up(up(cols, kFp8Block) / kFp8Block, 4); }
+  int64_t scales_at() const { return at + up(rows * ld(), 256); }
+  int64_t end() const { return scales_at() + up(up(rows, block_rows) / block_rows * lds(), 256); }
+  Fp8Out out(uint8_t* base) const { return {base + at, base + scales_at(), ld(), lds()}; }
+  Fp8In in(const uint8_t* base) const { return {base + at, base + scales_at(), ld(), lds(), block_rows, kE4M3}; }
+};
+
+struct Plan {
+  Piece xq, wq, wt;      // forward: x, w; w transposed
+  Piece gq, gt, xt;      // backward: dy, dy transposed, x transposed
+  LinearFp8Bytes bytes;
+  Plan(int64_t M, int64_t N, int64_t K, bool dx, bool dw) : bytes{0, 0, 0} {
+    auto take = [](Piece& p, int64_t& at, int64_t rows, int64_t cols, int block_rows) {
+      p = {rows, cols, at, block_rows};
+      at = p.end();
+    };
+    take(xq, dw ? bytes.kept : bytes.forward_temp, M, K, 1);
+    take(wq, bytes.forward_temp, N, K, kFp8Block);
+    if (dx) {
+      take(wt, bytes.kept, K, N, kFp8Block);
+      take(gq, bytes.backward_temp, M, N, 1);
+    }
+    if (dw) {
+      take(gt, bytes.backward_temp, N, M, 1);
+      take(xt, bytes.backward_temp, K, M, 1);
+    }
+  }
+};
+
+hipError_t gemm(Fp8In a, Fp8In b, int64_t M, int64_t N, int64_t K, void* c, int ctype, hipStream_t stream) {
+  return launch_gemm_fp8({a, b, c, N, M, N, K, ctype, 0}, stream);
+}
+
+#define GPUEXP_RETURN_IF(call)                   \
+  if (hipError_t e_ = (call); e_ != hipSuccess) \
+  return e_
+
+}  // namespace
+
+LinearFp8Bytes linear_fp8_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
+  return Plan(M, N, K, want_dx, want_dw).bytes;
+}
+
+hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream) {
+  const Plan p(a.M, a.N, a.K, a.want_dx, a.want_dw);
+  uint8_t* x_at = a.want_dw ? a.kept : a.temp;
+  GPUEXP_RETURN_IF(launch_quantize_fp8(a.x, a.type, a.ldx, a.M, a.K, kE4M3, 1, p.xq.out(x_at), {}, stream));
+  GPUEXP_RETURN_IF(launch_quantize_fp8(a.w, a.wtype, a.ldw, a.N, a.K, kE4M3, kFp8Block, p.wq.out(a.temp),
+                                       a.want_dx ? p.wt.out(a.kept) : Fp8Out{}, stream));
+  return gemm(p.xq.in(x_at), p.wq.in(a.temp), a.M, a.N, a.K, y, a.type, stream);
+}
+
+hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
+                                      hipStream_t stream) {
+  const Plan p(a.M, a.N, a.K, a.want_dx, a.want_dw);
+  GPUEXP_RETURN_IF(launch_quantize_fp8(dy, a.type, lddy, a.M, a.N, kE4M3, 1,
+                                       a.want_dx ? p.gq.out(a.temp) : Fp8Out{},
+                                       a.want_dw ? p.gt.out(a.temp) : Fp8Out{}, stream));
+  if (a.want_dx)
+    GPUEXP_RETURN_IF(gemm(p.gq.in(a.temp), p.wt.in(a.kept), a.M, a.K, a.N, dx, a.type, stream));
+  if (a.want_dw) {
+    GPUEXP_RETURN_IF(launch_transpose_fp8(p.xq.in(a.kept), a.M, a.K, p.xt.out(a.temp), stream));
+    GPUEXP_RETURN_IF(gemm(p.gt.in(a.temp), p.xt.in(a.temp), a.N, a.K, a.M, dw, a.wtype, stream));
+  }
+  return hipSuccess;
+}
+
+int64_t serve_fp8_bytes(int64_t M, int64_t N, int64_t K) { return Piece{M, K, 0, 1}.end(); }
+
+hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
+                            uint8_t* temp, hipStream_t stream) {
+  const Piece xq{M, K, 0, 1};
+  GPUEXP_RETURN_IF(launch_quantize_fp8(x, type, ldx, M, K, kE4M3, 1, xq.out(temp), {}, stream));
+  return gemm(xq.in(temp), w, M, N, K, y, type, stream);
+}
+
+}  // namespace gpuexp

@@ -44,16 +44,25 @@ def _elsewhere(stream, *tensors):
     return torch.cuda.stream(s)
 
 
-def _on(device):
-    """(raw current stream of `device`, a context that makes it the current device)."""
-    return torch.cuda.current_stream(device).cuda_stream, torch.cuda.device(device)
+def _launch(device, native, *args):
+    """A native call on torch's current stream of `device`, which it makes the current device."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # (torch.cuda.current_stream makes an object: 2 us)
+    if torch.cuda.current_device() == device.index:
+        native(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            native(*args, stream)
 
 
 def _gpu(name, *tensors):
     device = tensors[0].device
-    if device.type != "cuda" or any(t.device != device for t in tensors):
-        raise ValueError(f"{name}: tensors must be on the same GPU, got {[str(t.device) for t in tensors]}")
-    return device
+    if device.type == "cuda":
+        for t in tensors:
+            if t.device != device:
+                break
+        else:
+            return device
+    raise ValueError(f"{name}: tensors must be on the same GPU, got {[str(t.device) for t in tensors]}")
 
 
 def _empty(rows, cols, dtype, pad, device):
@@ -68,19 +77,18 @@ def _held(rows, cols, dtype, block_rows, device):
             _empty(-(-rows // block_rows), -(-cols // BLOCK), _E8M0, 4, device))
 
 
-def _row_stride(name, t, pad):
+def _row_stride(name, t, rows, cols, pad):
     """Bytes between rows of a 1-byte tensor [rows, cols] whose rows start at multiples of `pad`."""
-    rows, cols = t.shape
-    ld = -(-cols // pad) * pad
-    if not t.numel():
-        return ld
-    if cols > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} must have its columns next to each other, got strides {tuple(t.stride())}")
-    if rows > 1:
-        ld = t.stride(0)
+    if not (rows and cols):
+        return -(-cols // pad) * pad
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        raise ValueError(f"{name} must have its columns next to each other, got strides {(ld, step)}")
+    if rows == 1:
+        ld = -(-cols // pad) * pad
     if ld % pad or ld < cols or t.data_ptr() % pad:
-        raise ValueError(f"{name}'s rows must start at multiples of {pad} bytes and not overlap (row stride {ld}, "
-                         f"address % {pad} = {t.data_ptr() % pad}); quantize_fp8 makes such tensors")
+        raise ValueError(f"{name}'s rows must start at multiples of {pad} bytes and not overlap (row stride "
+                         f"{ld}, address % {pad} = {t.data_ptr() % pad}); quantize_fp8 makes such tensors")
     return ld
 
 
@@ -93,18 +101,19 @@ def _operand(name, q, scale):
     if q.dim() != 2 or scale.dim() != 2:
         raise ValueError(f"{name} and its scales must be 2-dimensional, got {tuple(q.shape)} and {tuple(scale.shape)}")
     rows, cols = q.shape
-    nb = -(-cols // BLOCK)
-    if tuple(scale.shape) == (rows, nb):
+    nb, scale_shape = -(-cols // BLOCK), scale.shape
+    if scale_shape == (rows, nb):
         block_rows = 1
-    elif tuple(scale.shape) == (-(-rows // BLOCK), nb):
+    elif scale_shape == (-(-rows // BLOCK), nb):
         block_rows = BLOCK
     else:
         raise ValueError(f"the scales of {name} {tuple(q.shape)} must be {(rows, nb)} (blocks of 1 x 128) or "
                          f"{(-(-rows // BLOCK), nb)} (128 x 128), got {tuple(scale.shape)}")
-    # (no address where there is nothing: an empty view may have any)
-    q_at, scale_at = (q.data_ptr(), scale.data_ptr()) if q.numel() else (0, 0)
-    return (q_at, scale_at, _row_stride(name, q, 16), _row_stride(f"the scales of {name}", scale, 4),
-            block_rows, _TYPES[q.dtype])
+    ld = _row_stride(name, q, rows, cols, 16)
+    lds = _row_stride(name + "'s scale", scale, scale_shape[0], nb, 4)
+    if not (rows and cols):  # (no address where there is nothing: an empty view may have any)
+        return 0, 0, ld, lds, block_rows, _TYPES[q.dtype]
+    return q.data_ptr(), scale.data_ptr(), ld, lds, block_rows, _TYPES[q.dtype]
 
 
 def _wide(name, x):
@@ -136,12 +145,11 @@ def _quantize(x, dtype, block_rows, rows=True, columns=False):
     out = _held(m, k, dtype, block_rows, device) if rows else None
     out_t = _held(k, m, dtype, block_rows, device) if columns else None
     if m and k:
-        stream, guard = _on(device)
         args = []
         for o in (out, out_t):
             args += [0, 0, 0, 0] if o is None else [o[0].data_ptr(), o[1].data_ptr(), o[0].stride(0), o[1].stride(0)]
-        with guard:
-            kernels().quantize_fp8(x.data_ptr(), _WIDE[x.dtype], ld, m, k, _TYPES[dtype], block_rows, *args, stream)
+        _launch(device, kernels().quantize_fp8, x.data_ptr(), _WIDE[x.dtype], ld, m, k, _TYPES[dtype], block_rows,
+                *args)
     return out, out_t
 
 
@@ -170,9 +178,7 @@ def dequantize_fp8(q, scale, dtype=torch.bfloat16, stream=None):
     rows, cols = q.shape
     x = torch.empty((rows, cols), dtype=dtype, device=device)
     if rows and cols:
-        raw, guard = _on(device)
-        with guard:
-            kernels().dequantize_fp8(*op, rows, cols, x.data_ptr(), _WIDE[dtype], cols, raw)
+        _launch(device, kernels().dequantize_fp8, *op, rows, cols, x.data_ptr(), _WIDE[dtype], cols)
     return x
 
 
@@ -190,9 +196,8 @@ def transpose_fp8(q, scale, stream=None):
     rows, cols = q.shape
     qt, st = _held(cols, rows, q.dtype, op[4], device)
     if rows and cols:
-        raw, guard = _on(device)
-        with guard:
-            kernels().transpose_fp8(*op, rows, cols, qt.data_ptr(), st.data_ptr(), qt.stride(0), st.stride(0), raw)
+        _launch(device, kernels().transpose_fp8, *op, rows, cols, qt.data_ptr(), st.data_ptr(), qt.stride(0),
+                st.stride(0))
     return qt, st
 
 
@@ -221,44 +226,74 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=
     if out is None:
         out = torch.empty((M, N), dtype=dtype, device=device)
     if M and N:
-        raw, guard = _on(device)
-        with guard:
-            kernels().gemm_fp8(*oa, *ob, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K, _WIDE[dtype], raw, variant)
+        _launch(device, kernels().gemm_fp8, *oa, *ob, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K,
+                _WIDE[dtype], variant)
     return out
+
+
+def _forward(x, weight, want_dx, want_dw):
+    """(y, what the backward pass needs) of x [M, K] and weight [N, K], one native call."""
+    (M, K), N = x.shape, weight.shape[0]
+    kept_bytes, temp_bytes, _ = kernels().linear_fp8_bytes(M, N, K, want_dx, want_dw)
+    y = x.new_empty((M, N))
+    kept = torch.empty(kept_bytes, dtype=torch.uint8, device=x.device)
+    temp = torch.empty(temp_bytes, dtype=torch.uint8, device=x.device)
+    _launch(x.device, kernels().linear_fp8_forward, M, N, K, want_dx, want_dw, x.data_ptr(), _wide("x", x),
+            _WIDE[x.dtype], weight.data_ptr(), _wide("weight", weight), _WIDE[weight.dtype], kept.data_ptr(),
+            temp.data_ptr(), y.data_ptr())
+    return y, kept
 
 
 class _LinearFp8(torch.autograd.Function):
     """y = x W^T with both operands in 8 bits; what it keeps for the backward pass is in 8 bits."""
 
     @staticmethod
-    def forward(ctx, x, weight, weight_scale):
-        ctx.frozen = weight_scale is not None
-        ctx.x_grad, ctx.w_grad = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        ctx.dtypes = x.dtype, weight.dtype
-        xq = _quantize(x, torch.float8_e4m3fn, 1)[0]
-        if ctx.frozen:
-            wq = wt = (weight, weight_scale)
-        else:
-            wq, wt = _quantize(weight, torch.float8_e4m3fn, BLOCK, columns=ctx.x_grad)
-        kept = (*(xq if ctx.w_grad else ()), *(wt if ctx.x_grad else ()))
-        ctx.save_for_backward(*kept)
-        return gemm_fp8(*xq, *wq, out_dtype=x.dtype)
+    def forward(ctx, x, weight):
+        ctx.want = ctx.needs_input_grad
+        ctx.sizes = x.shape[0], weight.shape[0], x.shape[1]
+        ctx.weight_dtype = weight.dtype
+        y, kept = _forward(x, weight, *ctx.want)
+        ctx.save_for_backward(kept)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        kept = list(ctx.saved_tensors)
-        xq = (kept.pop(0), kept.pop(0)) if ctx.w_grad else None
-        wt = (kept.pop(0), kept.pop(0)) if ctx.x_grad else None
-        gq, gt = _quantize(_rows(grad), torch.float8_e4m3fn, 1, rows=ctx.x_grad, columns=ctx.w_grad)
-        dx = dw = None
-        if ctx.x_grad:
-            if ctx.frozen:
-                wt = transpose_fp8(*wt)
-            dx = gemm_fp8(*gq, *wt, out_dtype=ctx.dtypes[0])
-        if ctx.w_grad:
-            dw = gemm_fp8(*gt, *transpose_fp8(*xq), out_dtype=ctx.dtypes[1])
-        return dx, dw, None
+        (kept,), (M, N, K), (want_dx, want_dw) = ctx.saved_tensors, ctx.sizes, ctx.want
+        grad = _rows(grad)
+        dx = grad.new_empty((M, K)) if want_dx else None
+        dw = torch.empty((N, K), dtype=ctx.weight_dtype, device=grad.device) if want_dw else None
+        temp = torch.empty(kernels().linear_fp8_bytes(M, N, K, want_dx, want_dw)[2], dtype=torch.uint8,
+                           device=grad.device)
+        _launch(grad.device, kernels().linear_fp8_backward, M, N, K, want_dx, want_dw, grad.data_ptr(),
+                _wide("grad", grad), _WIDE[grad.dtype], _WIDE[ctx.weight_dtype], kept.data_ptr(), temp.data_ptr(),
+                dx.data_ptr() if want_dx else 0, dw.data_ptr() if want_dw else 0)
+        return dx, dw
+
+
+def _serve(x, N, op):
+    """y of x [M, K] and a weight [N, K] in 8 bits (`op`: its checked operand), one native call."""
+    M, K = x.shape
+    y = x.new_empty((M, N))
+    temp = torch.empty(kernels().serve_fp8_bytes(M, N, K), dtype=torch.uint8, device=x.device)
+    _launch(x.device, kernels().serve_fp8, x.data_ptr(), _WIDE[x.dtype], _wide("x", x), *op, M, N, K, y.data_ptr(),
+            temp.data_ptr())
+    return y
+
+
+class _ServeFp8(torch.autograd.Function):
+    """The same with a weight that is in 8 bits already and takes no gradient."""
+
+    @staticmethod
+    def forward(ctx, x, weight, weight_scale, op):
+        ctx.save_for_backward(weight, weight_scale)
+        return _serve(x, weight.shape[0], op)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        gq = quantize_fp8(_rows(grad))
+        return gemm_fp8(*gq, *transpose_fp8(*ctx.saved_tensors), out_dtype=grad.dtype), None, None, None
 
 
 def _rows(x):
@@ -272,7 +307,7 @@ def linear_fp8(x, weight, weight_scale=None):
     Training: `weight` in bf16 or f16.  Both operands are quantised to e4m3 (x in blocks of 1 x 128,
     the weight 128 x 128).  For the backward pass x is kept as its 8-bit checkpoint, half the memory
     of the activation; dx = Q(dy) W with the kept 8-bit weight, dW = Q(dy^T) x with the checkpoint
-    transposed (transpose_fp8).  A double backward is refused.
+    transposed (as transpose_fp8 does).  A double backward is refused.
 
     Serving: `weight` in 8 bits with its `weight_scale`, as quantize_fp8(w, block_rows=128) gives
     them; x may take a gradient, the weight takes none."""
@@ -280,17 +315,21 @@ def linear_fp8(x, weight, weight_scale=None):
         raise ValueError(f"shape mismatch {tuple(x.shape)} x {tuple(weight.shape)}^T")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"linear_fp8 takes bfloat16 or float16 activations, got {x.dtype}")
+    x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    grad = torch.is_grad_enabled()
     if weight_scale is None:
         if weight.dtype not in (torch.bfloat16, torch.float16):
             raise TypeError("linear_fp8 takes bfloat16 or float16 weights, or 8-bit ones with weight_scale, got "
                             f"{weight.dtype}")
         _gpu("linear_fp8", x, weight)
+        x2, weight = _rows(x2), _rows(weight)
+        y = _LinearFp8.apply(x2, weight) if grad and (x2.requires_grad or weight.requires_grad) else \
+            _forward(x2, weight, False, False)[0]
     else:
         if weight.requires_grad:
             raise ValueError("weights in 8 bits take no gradient")
-        _operand("weight", weight, weight_scale)
+        op = _operand("weight", weight, weight_scale)
         _gpu("linear_fp8", x, weight, weight_scale)
-    x2 = _rows(x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1]))
-    w2 = weight if weight_scale is not None else _rows(weight)
-    y = _LinearFp8.apply(x2, w2, weight_scale)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
+        x2 = _rows(x2)
+        y = _ServeFp8.apply(x2, weight, weight_scale, op) if grad and x2.requires_grad else _serve(x2, weight.shape[0], op)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[1])

@@ -113,7 +113,7 @@ def test_native_calls_check_addresses_and_strides(native):
             k.gemm_fp8(*good, *good, c, ldc, 4, 4, 128, ctype, 0, 0)
     for variant in (-1, 2, 99):  # 2, the 256x256 tile, takes K >= 144
         with pytest.raises(ValueError, match="variant"):
-            k.gemm_fp8(*good, *good, 1 << 20, 4, 4, 4, 128, 0, 0, variant)
+            k.gemm_fp8(*good, *good, 1 << 20, 4, 4, 4, 128, 0, variant, 0)
     with pytest.raises(ValueError):
         k.quantize_fp8(1 << 20, 0, 127, 4, 128, 0, 1, 1 << 20, 1 << 20, 128, 4, 0, 0, 0, 0, 0)
     with pytest.raises(ValueError):
