@@ -86,113 +86,249 @@ __device__ __forceinline__ int tail_scale(const Operand& o, int row, int K) {
   return o.scale[int64_t(row) * o.lds + (K - 1) / kBK];
 }
 
-// ---- 128 x 128 tile, 4 waves of 64 x 64, two tiles of K in LDS ----
-template <int kA, int kB, typename TC>
-__global__ void __launch_bounds__(256, 2)
-gemm_fp8_128_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K) {
-  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * 2 * 128 * kBK];  // [buf][A|B][128][128]
+// The first rows of this block's tile.  Blocks are dealt to the 8 XCDs in turn: each XCD gets a
+// contiguous range of tiles, ordered in groups of kGroupM row panels x all column panels, so the tiles
+// that run at once share panels in its L2.
+template <int kBM, int kBN, int kGroupM>
+__device__ __forceinline__ void tile_of_block(int M, int N, int& row_a, int& row_b) {
+  const int nbn = (N + kBN - 1) / kBN, nbm = (M + kBM - 1) / kBM;
+  const int nwg = nbm * nbn;
+  const int orig = blockIdx.x;
+  const int xcd = orig & 7, q = nwg >> 3, r = nwg & 7;
+  const int wgid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (orig >> 3);
+  const int in_group = kGroupM * nbn;
+  const int first_m = (wgid / in_group) * kGroupM;
+  const int gsize = nbm - first_m < kGroupM ? nbm - first_m : kGroupM;
+  row_a = (first_m + (wgid % in_group) % gsize) * kBM;
+  row_b = ((wgid % in_group) / gsize) * kBN;
+}
+
+// gfx9 encoding: vmcnt [3:0] and [15:14], expcnt [6:4], lgkmcnt [11:8]
+constexpr int waitcnt_vm(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | (((n >> 4) & 3) << 14); }
+constexpr int kWaitLgkm0 = 0xF | (0x7 << 4) | (0x3 << 14);
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(N));
+}
+
+// A fragment of 32 rows x 64 k: lane l holds row l % 32 and, with g = l / 32, the chunks 2 h + g and
+// 2 h + g + 4 of the row's 8, h = 0, 1 for the two halves of a K tile.  Any assignment does that A
+// and B share, and in this one the four places are xors of each other, alike for rows 32 apart.
+struct FragAt {
+  const uint8_t *p0, *p1;  // h = 0: chunks g, g + 4
+  const uint8_t *p2, *p3;  // h = 1
+};
+__device__ __forceinline__ FragAt frag_at(const uint8_t* rows, int lane) {
+  const int at = (lane & 31) * kBK, c = swz(lane & 31, lane >> 5) * 16;
+  return {rows + at + c, rows + at + (c ^ 64), rows + at + (c ^ 32), rows + at + (c ^ 96)};
+}
+__device__ __forceinline__ void read_frag(const FragAt& f, int offset, i32x8 (&out)[2]) {
+  const i32x4 a = *reinterpret_cast<const i32x4*>(f.p0 + offset);
+  const i32x4 b = *reinterpret_cast<const i32x4*>(f.p1 + offset);
+  const i32x4 c = *reinterpret_cast<const i32x4*>(f.p2 + offset);
+  const i32x4 d = *reinterpret_cast<const i32x4*>(f.p3 + offset);
+  out[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  out[1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int kA, int kB, int kByte>
+__device__ __forceinline__ f32x16 mfma32(const i32x8& a, const i32x8& b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, kA, kB, kByte, sa, kByte, sb);
+}
+
+// C leaves through LDS, so that every global store is 16 bytes of a row.  D of 32x32x64: column (here
+// a row of C, B being the first operand) = lane % 32, row (a column of C) = (e / 4) * 8 + (lane / 32) * 4
+// + e % 4: a lane writes 8 bytes, the two halves of a wave the two halves of 16-byte chunks, which are
+// xored with the row so that the 32 rows fall into different banks.
+template <int kBN, typename TC>
+__device__ __forceinline__ void tile_to_lds(uint8_t* smem, int row0, int col0, int lane, const f32x16& v) {
+  typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+  const int row = row0 + (lane & 31);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = col0 / 8 + e;
+    const u32x2 w{uint32_t(to16<TC>(v[4 * e])) | (uint32_t(to16<TC>(v[4 * e + 1])) << 16),
+                  uint32_t(to16<TC>(v[4 * e + 2])) | (uint32_t(to16<TC>(v[4 * e + 3])) << 16)};
+    *reinterpret_cast<u32x2*>(smem + row * kBN * 2 + ((c ^ (row & (kBN / 8 - 1) & 31)) << 4) + (lane >> 5) * 8) = w;
+  }
+}
+template <int kBM, int kBN, int kThreads>
+__device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64_t ldc, int M, int N, int row_a,
+                                         int row_b, int vec_c) {
+  constexpr int kChunks = kBN / 8;
+#pragma unroll 4
+  for (int p = 0; p < kBM * kChunks / kThreads; ++p) {
+    const int idx = p * kThreads + threadIdx.x;
+    const int row = idx / kChunks, c = idx % kChunks;
+    if (row_a + row >= M) break;
+    const i32x4 v = *reinterpret_cast<const i32x4*>(smem + row * kBN * 2 + ((c ^ (row & (kChunks - 1) & 31)) << 4));
+    const int col = row_b + c * 8;
+    uint16_t* dst = C + int64_t(row_a + row) * ldc + col;
+    if (vec_c && col + 8 <= N) {
+      __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(dst));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < N) dst[e] = uint16_t(uint32_t(v[e >> 1]) >> (16 * (e & 1)));
+    }
+  }
+}
+
+// ---- 128 x 128 and 64 x 64 tiles, 4 waves, kStages tiles of K in LDS ----
+// For sizes with too few 256 x 256 tiles to fill the card.  Waves are 2 x 2, each with a quarter of the
+// tile.  While K tile t is multiplied from registers, t + 1 is read from LDS and t + kStages is loaded
+// into the buffer that t left; one barrier per K tile.  Behind it every wave has its part of tile t + 1
+// (a counted wait: loads complete in order) and has tile t in registers.  Past the end of K the loads go
+// on out of range, so the count holds.  A block has kStages - 1 tiles in flight, 96 KiB (128) or 80 KiB
+// (64): one block per CU covers the memory's latency.  The scales come as in the 256 x 256 kernel; a
+// quad's words are read with its first K tile, and the next quad's loaded then, which the count covers
+// as long as kStages <= 6.
+template <int kA, int kB, typename TC, int kBM, int kBN, int kStages>
+__global__ void __launch_bounds__(256, 1)
+gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int vec_c) {
+  constexpr int kStage = (kBM + kBN) * kBK, kScales = kStages * kStage, kRows = kBM + kBN;
+  constexpr int kMI = kBM / 64, kNI = kBN / 64, kLoads = kRows / 32;  // 32-row fragments and loads per wave
+  static_assert(kStages <= 6 && kBM * kBN * 2 <= kScales, "scales land too late, or C does not fit");
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kScales + 2 * kRows * 4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const int nbn = (B.rows + 127) / 128;
-  const int row_a = int(blockIdx.x / nbn) * 128, row_b = int(blockIdx.x % nbn) * 128;
-  const rsrc_t ra = tile_rsrc(A, row_a, 128, K), rb = tile_rsrc(B, row_b, 128, K);
-  const int K16 = K & ~15;
-  const int nk = (K16 + kBK - 1) / kBK;
+  int row_a, row_b;
+  tile_of_block<kBM, kBN, 8>(A.rows, B.rows, row_a, row_b);
+  const int K16 = K & ~15, nk = (K16 + kBK - 1) / kBK;
+  const rsrc_t ra = tile_rsrc(A, row_a, kBM, K), rb = tile_rsrc(B, row_b, kBN, K);
 
+  // load i of a wave covers rows (wave + 4 i) * 8 .. + 8 of [A rows, B rows]
+  const int lrow = lane >> 3;
+  const int chunk = swz((wave & 1) * 8 + lrow, lane & 7) * 16;  // (the swizzle sees the parity of row / 8)
+  const uint32_t va = uint32_t(lrow) * uint32_t(A.ld) + chunk, vb = uint32_t(lrow) * uint32_t(B.ld) + chunk;
   auto stage = [&](int t) {
-    uint8_t* buf = smem + (t & 1) * 2 * 128 * kBK;
+    uint8_t* buf = smem + (t % kStages) * kStage;
+    const bool in = chunk < K16 - t * kBK;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int rblk = (wave * 4 + i) * 8, row = rblk + (lane >> 3), chunk = swz(row, lane & 7) * 16;
-      const uint32_t oa = uint32_t(row) * uint32_t(A.ld) + chunk, ob = uint32_t(row) * uint32_t(B.ld) + chunk;
-      const bool in = t * kBK + chunk < K16;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(buf + rblk * kBK), 16, in ? oa : kOob, t * kBK, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(buf + (128 + rblk) * kBK), 16, in ? ob : kOob, t * kBK,
-                                               0, 0);
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = (wave + 4 * i) * 8;
+      if (i < kBM / 32)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(buf + row * kBK), 16, in ? va : kOob,
+                                                 uint32_t(row) * uint32_t(A.ld) + t * kBK, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(buf + row * kBK), 16, in ? vb : kOob,
+                                                 uint32_t(row - kBM) * uint32_t(B.ld) + t * kBK, 0, 0);
     }
   };
+  // scales: wave w loads those of rows w * 64 + lane of [A rows, B rows]
+  const bool loads_scales = wave * 64 < kRows;
+  const bool of_a = wave * 64 < kBM;
+  const Operand& S = of_a ? A : B;
+  int srow = (of_a ? row_a + wave * 64 : row_b + wave * 64 - kBM) + lane;
+  srow = (srow < S.rows ? srow : S.rows - 1) >> S.shift;
+  const uint8_t* sptr = S.scale + int64_t(srow) * S.lds;
+  const int quads = (nk + 3) / 4;
+  auto stage_scales = [&](int quad) {
+    typedef __attribute__((address_space(1))) void* gptr_t;
+    if (loads_scales)
+      __builtin_amdgcn_global_load_lds((gptr_t)(sptr + (quad < quads ? quad : quads - 1) * 4),
+                                       (lds_ptr_t)(smem + kScales + (quad & 1) * kRows * 4 + wave * 256), 4, 0, 0);
+  };
 
-  // scales: one dword holds a row's next four blocks
-  const uint32_t *pa[4], *pb[4];
+  f32x16 acc[kMI][kNI];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    int r = row_a + wm * 64 + i * 16 + (lane & 15);
-    r = (r < A.rows ? r : A.rows - 1) >> A.shift;
-    pa[i] = reinterpret_cast<const uint32_t*>(A.scale + int64_t(r) * A.lds);
-    r = row_b + wn * 64 + i * 16 + (lane & 15);
-    r = (r < B.rows ? r : B.rows - 1) >> B.shift;
-    pb[i] = reinterpret_cast<const uint32_t*>(B.scale + int64_t(r) * B.lds);
-  }
-  uint32_t sa[4], sb[4];
-  f32x4 acc[4][4];
+  for (int i = 0; i < kMI; ++i)
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < kNI; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  i32x8 af[2][kMI][2], bf[2][kNI][2];  // K tiles t and t + 1
+  uint32_t sa[kMI], sb[kNI], sa_next[kMI], sb_next[kNI];
+  const FragAt a_at = frag_at(smem + wm * (kBM / 2) * kBK, lane);
+  const FragAt b_at = frag_at(smem + (kBM + wn * (kBN / 2)) * kBK, lane);
+  auto read = [&](int t, i32x8 (&fa)[kMI][2], i32x8 (&fb)[kNI][2]) {
+    const int buf = (t % kStages) * kStage;
+#pragma unroll
+    for (int i = 0; i < kMI; ++i) read_frag(a_at, buf + i * 32 * kBK, fa[i]);
+#pragma unroll
+    for (int j = 0; j < kNI; ++j) read_frag(b_at, buf + j * 32 * kBK, fb[j]);
+  };
+  auto read_scales = [&](int quad, uint32_t (&a)[kMI], uint32_t (&b)[kNI]) {
+    const uint8_t* sc = smem + kScales + (quad & 1) * kRows * 4 + (lane & 31) * 4;
+#pragma unroll
+    for (int i = 0; i < kMI; ++i) a[i] = *reinterpret_cast<const uint32_t*>(sc + (wm * (kBM / 2) + i * 32) * 4);
+#pragma unroll
+    for (int j = 0; j < kNI; ++j)
+      b[j] = *reinterpret_cast<const uint32_t*>(sc + (kBM + wn * (kBN / 2) + j * 32) * 4);
+  };
 
-  if (nk > 0) stage(0);
-  for (int t = 0; t < nk; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // tile t landed for every wave; the other buffer is free
-    if (t + 1 < nk) stage(t + 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if ((t & 3) == 0) {
-        sa[i] = pa[i][t >> 2];
-        sb[i] = pb[i][t >> 2];
-      } else {
-        sa[i] >>= 8;
-        sb[i] >>= 8;
-      }
+  auto tile = [&](int t, auto byte_tag) {
+    constexpr int byte = decltype(byte_tag)::value, cur = byte & 1;
+    // tile t + 1 is here, and the reads of tile t have landed
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm((kStages - 2) * kLoads) & ~0xF00);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if constexpr (byte == 3) {
+      read_scales((t + 1) >> 2, sa_next, sb_next);
+      stage_scales(((t + 1) >> 2) + 1);
     }
-    const uint8_t* As = smem + (t & 1) * 2 * 128 * kBK;
-    const uint8_t* Bs = As + 128 * kBK;
-    const int c0 = lane >> 4, c1 = 4 + (lane >> 4);
-    i32x8 af[4], bf[4];
+    stage(t + kStages);
+    read(t + 1, af[1 - cur], bf[1 - cur]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int x = wm * 64 + i * 16 + (lane & 15), y = wn * 64 + i * 16 + (lane & 15);
-      const i32x4 a0 = *reinterpret_cast<const i32x4*>(As + x * kBK + swz(x, c0) * 16);
-      const i32x4 a1 = *reinterpret_cast<const i32x4*>(As + x * kBK + swz(x, c1) * 16);
-      const i32x4 b0 = *reinterpret_cast<const i32x4*>(Bs + y * kBK + swz(y, c0) * 16);
-      const i32x4 b1 = *reinterpret_cast<const i32x4*>(Bs + y * kBK + swz(y, c1) * 16);
-      af[i] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-      bf[i] = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < kMI; ++i)
+#pragma unroll
+        for (int j = 0; j < kNI; ++j)
+          acc[i][j] = mfma32<kB, kA, byte>(bf[cur][j][h], af[cur][i][h], acc[i][j], int(sb[j]), int(sa[i]));
+    if constexpr (byte == 3) {
+#pragma unroll
+      for (int i = 0; i < kMI; ++i) sa[i] = sa_next[i];
+#pragma unroll
+      for (int j = 0; j < kNI; ++j) sb[j] = sb_next[j];
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (nk > 0) {
+    stage_scales(0);
+    stage_scales(1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma<kA, kB>(af[i], bf[j], acc[i][j], int(sa[i]), int(sb[j]));
+    for (int t = 0; t < kStages; ++t) stage(t);
+    wait_vm<(kStages - 1) * kLoads>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read_scales(0, sa, sb);
+    read(0, af[0], bf[0]);
+    for (int t = 0;; t += 4) {
+      tile(t, std::integral_constant<int, 0>{});
+      if (t + 1 >= nk) break;
+      tile(t + 1, std::integral_constant<int, 1>{});
+      if (t + 2 >= nk) break;
+      tile(t + 2, std::integral_constant<int, 2>{});
+      if (t + 3 >= nk) break;
+      tile(t + 3, std::integral_constant<int, 3>{});
+      if (t + 4 >= nk) break;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();  // no load in flight, every wave's reads done: LDS is free
   }
-
   if (K != K16) {
-    i32x8 af[4], bf[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int x = wm * 64 + i * 16 + (lane & 15), y = wn * 64 + i * 16 + (lane & 15);
-      af[i] = tail_frag(ra, A.ld, x, lane < 16, K);
-      bf[i] = tail_frag(rb, B.ld, y, lane < 16, K);
-      sa[i] = tail_scale(A, row_a + x, K);
-      sb[i] = tail_scale(B, row_b + y, K);
-    }
+    for (int i = 0; i < kMI; ++i) {
+      const int x = wm * (kBM / 2) + i * 32 + (lane & 31);
+      const i32x8 a = tail_frag(ra, A.ld, x, lane < 32, K);
+      const int s = tail_scale(A, row_a + x, K);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma<kA, kB>(af[i], bf[j], acc[i][j], int(sa[i]), int(sb[j]));
-  }
-
-  // C/D map of 16x16x128: col = lane % 16, row = (lane / 16) * 4 + r
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = row_a + wm * 64 + i * 16 + (lane >> 4) * 4 + r;
-        const int col = row_b + wn * 64 + j * 16 + (lane & 15);
-        if (row < A.rows && col < B.rows) C[int64_t(row) * ldc + col] = to16<TC>(acc[i][j][r]);
+      for (int j = 0; j < kNI; ++j) {
+        const int y = wn * (kBN / 2) + j * 32 + (lane & 31);
+        acc[i][j] = mfma32<kB, kA, 0>(tail_frag(rb, B.ld, y, lane < 32, K), a, acc[i][j], tail_scale(B, row_b + y, K),
+                                      s);
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMI; ++i)
+#pragma unroll
+    for (int j = 0; j < kNI; ++j)
+      tile_to_lds<kBN, TC>(smem, wm * (kBM / 2) + i * 32, wn * (kBN / 2) + j * 32, lane, acc[i][j]);
+  __syncthreads();
+  lds_to_c<kBM, kBN, 256>(smem, C, ldc, A.rows, B.rows, row_a, row_b, vec_c);
 }
 
 // ---- 256 x 256 tile, 8 waves, two barriers per phase ----
@@ -220,15 +356,6 @@ gemm_fp8_128_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
 constexpr int kTile256 = 256 * kBK;
 constexpr int kScales256 = 4 * kTile256;
 
-// gfx9 encoding: vmcnt [3:0] and [15:14], expcnt [6:4], lgkmcnt [11:8]
-constexpr int waitcnt_vm(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | (((n >> 4) & 3) << 14); }
-constexpr int kWaitLgkm0 = 0xF | (0x7 << 4) | (0x3 << 14);
-
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(N));
-}
-
 // every wave's counted wait is behind this barrier; this wave's LDS reads have landed
 __device__ __forceinline__ void barrier_before_mfma() {
   __builtin_amdgcn_sched_barrier(0);
@@ -245,30 +372,6 @@ __device__ __forceinline__ void barrier_after_mfma() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// A fragment of 32 rows x 64 k: lane l holds row l % 32 and, with g = l / 32, the chunks 2 h + g and
-// 2 h + g + 4 of the row's 8, h = 0, 1 for the two halves of a K tile.  Any assignment does that A
-// and B share, and in this one the four places are xors of each other, alike for rows 32 apart.
-struct FragAt {
-  const uint8_t *p0, *p1;  // h = 0: chunks g, g + 4
-  const uint8_t *p2, *p3;  // h = 1
-};
-__device__ __forceinline__ FragAt frag_at(const uint8_t* rows, int lane) {
-  const int at = (lane & 31) * kBK, c = swz(lane & 31, lane >> 5) * 16;
-  return {rows + at + c, rows + at + (c ^ 64), rows + at + (c ^ 32), rows + at + (c ^ 96)};
-}
-__device__ __forceinline__ void read_frag(const FragAt& f, int offset, i32x8 (&out)[2]) {
-  const i32x4 a = *reinterpret_cast<const i32x4*>(f.p0 + offset);
-  const i32x4 b = *reinterpret_cast<const i32x4*>(f.p1 + offset);
-  const i32x4 c = *reinterpret_cast<const i32x4*>(f.p2 + offset);
-  const i32x4 d = *reinterpret_cast<const i32x4*>(f.p3 + offset);
-  out[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  out[1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-template <int kA, int kB, int kByte>
-__device__ __forceinline__ f32x16 mfma32(const i32x8& a, const i32x8& b, f32x16 c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, kA, kB, kByte, sa, kByte, sb);
-}
-
 template <int kA, int kB, typename TC>
 __global__ void __launch_bounds__(512, 1)
 gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int vec_c) {
@@ -277,18 +380,8 @@ gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave >> 2, wc = wave & 3;
 
-  // Blocks are dealt to the 8 XCDs in turn: each XCD gets a contiguous range of tiles, ordered in
-  // groups of 4 row panels x all column panels, so the tiles that run at once share panels in its L2.
-  constexpr int kGroupM = 4;
-  const int nbn = (B.rows + 255) / 256, nbm = (A.rows + 255) / 256;
-  const int nwg = nbm * nbn;
-  const int orig = blockIdx.x;
-  const int xcd = orig & 7, q = nwg >> 3, r = nwg & 7;
-  const int wgid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (orig >> 3);
-  const int in_group = kGroupM * nbn;
-  const int first_m = (wgid / in_group) * kGroupM;
-  const int gsize = nbm - first_m < kGroupM ? nbm - first_m : kGroupM;
-  const int row_a = (first_m + (wgid % in_group) % gsize) * 256, row_b = ((wgid % in_group) / gsize) * 256;
+  int row_a, row_b;
+  tile_of_block<256, 256, 4>(A.rows, B.rows, row_a, row_b);
 
   const int K16 = K & ~15;
   const int nk = (K16 + kBK - 1) / kBK;  // >= 2
@@ -449,43 +542,15 @@ gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
         acc[i >> 1][n][i & 1] = mfma32<kB, kA, 0>(bt[n], at[i], acc[i >> 1][n][i & 1], int(sb[n]), int(sa[i]));
   }
 
-  // C through LDS (128 KiB), so that every global store is 16 bytes of a row.  D of 32x32x64: column
-  // (here a row of C) = lane % 32, row (a column of C) = (e / 4) * 8 + (lane / 32) * 4 + e % 4: a lane
-  // writes 8 bytes, the two halves of a wave the two halves of 16-byte chunks, which are xored with the
-  // row so that 32 rows fall into different banks.
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = wr * 128 + m * 64 + i * 32 + (lane & 31);
-          const int c = wc * 8 + n * 4 + e;
-          const f32x16& v = acc[m][n][i];
-          typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-          const u32x2 w{uint32_t(to16<TC>(v[4 * e])) | (uint32_t(to16<TC>(v[4 * e + 1])) << 16),
-                        uint32_t(to16<TC>(v[4 * e + 2])) | (uint32_t(to16<TC>(v[4 * e + 3])) << 16)};
-          *reinterpret_cast<u32x2*>(smem + row * 512 + ((c ^ (lane & 31)) << 4) + (lane >> 5) * 8) = w;
-        }
+        tile_to_lds<256, TC>(smem, wr * 128 + m * 64 + i * 32, wc * 64 + n * 32, lane, acc[m][n][i]);
   __syncthreads();
-#pragma unroll 4
-  for (int p = 0; p < 16; ++p) {
-    const int idx = p * 512 + threadIdx.x;
-    const int row = idx >> 5, c = idx & 31;
-    if (row_a + row >= A.rows) break;
-    const i32x4 v = *reinterpret_cast<const i32x4*>(smem + row * 512 + ((c ^ (row & 31)) << 4));
-    const int col = row_b + c * 8;
-    uint16_t* dst = C + int64_t(row_a + row) * ldc + col;
-    if (vec_c && col + 8 <= B.rows) {
-      __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(dst));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col + e < B.rows) dst[e] = uint16_t(uint32_t(v[e >> 1]) >> (16 * (e & 1)));
-    }
-  }
+  lds_to_c<256, 256, 512>(smem, C, ldc, A.rows, B.rows, row_a, row_b, vec_c);
 }
 
 // ---- few rows of A (one token to 64): B is read once, from memory straight into registers ----
@@ -640,9 +705,9 @@ bool side_ok(const Fp8In& in, int64_t rows, int64_t K) {
 
 }  // namespace
 
-// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows; -1: not these sizes.
+// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows, 4 = 64 x 64 tile; -1: not these sizes.
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
-  if (variant < 0 || variant > 3) return -1;
+  if (variant < 0 || variant > 4) return -1;
   const int64_t tiles256 = ((M + 255) / 256) * ((N + 255) / 256);
   if (variant == 2) return K >= kBK + 16 ? 2 : -1;  // two K tiles
   if (variant == 3) return M <= 64 ? 3 : -1;
@@ -670,7 +735,7 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   if (g.M == 0 || g.N == 0) return hipSuccess;
   const int variant = resolve_gemm_fp8_variant(g.M, g.N, g.K, g.variant);
   if (variant < 0) return hipErrorInvalidValue;
-  const int64_t edge = variant == 2 ? 256 : 128;
+  const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
   const int64_t tiles = variant == 3 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
   if (tiles >= (int64_t(1) << 22)) return hipErrorInvalidValue;  // 2^32 threads
   const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc % 8 == 0;
@@ -686,8 +751,9 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
       hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
                          c, g.ldc, int(g.K), vec_c);
     } else {
-      hipLaunchKernelGGL((gemm_fp8_128_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob,
-                         c, g.ldc, int(g.K));
+      auto k = variant == 1 ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 4>
+                            : gemm_fp8_tile_kernel<a, b, decltype(tc), 64, 64, 6>;
+      hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K), vec_c);
     }
   });
   return hipGetLastError();
