@@ -277,6 +277,13 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
 #pragma unroll
         for (int j = 0; j < kNI; ++j)
           acc[i][j] = mfma32<kB, kA, byte>(bf[cur][j][h], af[cur][i][h], acc[i][j], int(sb[j]), int(sa[i]));
+    // the reads and loads go out between the MFMA: in a burst they would hold up the wave at issue
+#pragma unroll
+    for (int i = 0; i < 2 * kMI * kNI; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * (kMI + kNI) / (kMI * kNI), 0);
+      __builtin_amdgcn_sched_group_barrier(0x010, kLoads / (2 * kMI * kNI), 0);
+    }
     if constexpr (byte == 3) {
 #pragma unroll
       for (int i = 0; i < kMI; ++i) sa[i] = sa_next[i];
