@@ -18,6 +18,7 @@
 // what follows the last value in a row has no effect.
 #include "fp8_launch.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace gpuexp {
@@ -174,21 +175,21 @@ __device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64
   }
 }
 
-// ---- 128 x 128 and 64 x 64 tiles, 4 waves, kStages tiles of K in LDS ----
+// ---- 128 x 128 and 64 x 64 tiles, 4 waves, 2 or 4 tiles of K in LDS ----
 // For sizes with too few 256 x 256 tiles to fill the card.  Waves are 2 x 2, each with a quarter of the
 // tile.  While K tile t is multiplied from registers, t + 1 is read from LDS and t + kStages is loaded
 // into the buffer that t left; one barrier per K tile.  Behind it every wave has its part of tile t + 1
 // (a counted wait: loads complete in order) and has tile t in registers.  Past the end of K the loads go
-// on out of range, so the count holds.  A block has kStages - 1 tiles in flight, 96 KiB (128) or 80 KiB
-// (64): one block per CU covers the memory's latency.  The scales come as in the 256 x 256 kernel; a
-// quad's words are read with its first K tile, and the next quad's loaded then, which the count covers
-// as long as kStages <= 6.
+// on out of range, so the count holds.  The K loop is unrolled by 4, so with 2 or 4 stages every LDS
+// address is a constant (6 stages of 64 x 64, with more in flight, took 19 us where 4 take 15, at
+// 64 x 8192 x 8192).  The scales come as in the 256 x 256 kernel; a quad's words are read with its first
+// K tile, and the next quad's loaded then, which the count covers.
 template <int kA, int kB, typename TC, int kBM, int kBN, int kStages>
 __global__ void __launch_bounds__(256, 1)
 gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int vec_c) {
   constexpr int kStage = (kBM + kBN) * kBK, kScales = kStages * kStage, kRows = kBM + kBN;
   constexpr int kMI = kBM / 64, kNI = kBN / 64, kLoads = kRows / 32;  // 32-row fragments and loads per wave
-  static_assert(kStages <= 6 && kBM * kBN * 2 <= kScales, "scales land too late, or C does not fit");
+  static_assert((kStages == 2 || kStages == 4) && kBM * kBN * 2 <= kScales, "slots are t % 4's, and C fits");
   __shared__ __attribute__((aligned(16))) uint8_t smem[kScales + 2 * kRows * 4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -202,8 +203,8 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   const int lrow = lane >> 3;
   const int chunk = swz((wave & 1) * 8 + lrow, lane & 7) * 16;  // (the swizzle sees the parity of row / 8)
   const uint32_t va = uint32_t(lrow) * uint32_t(A.ld) + chunk, vb = uint32_t(lrow) * uint32_t(B.ld) + chunk;
-  auto stage = [&](int t) {
-    uint8_t* buf = smem + (t % kStages) * kStage;
+  auto stage = [&](int t, int slot) {  // slot: t % kStages
+    uint8_t* buf = smem + slot * kStage;
     const bool in = chunk < K16 - t * kBK;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -242,8 +243,8 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   uint32_t sa[kMI], sb[kNI], sa_next[kMI], sb_next[kNI];
   const FragAt a_at = frag_at(smem + wm * (kBM / 2) * kBK, lane);
   const FragAt b_at = frag_at(smem + (kBM + wn * (kBN / 2)) * kBK, lane);
-  auto read = [&](int t, i32x8 (&fa)[kMI][2], i32x8 (&fb)[kNI][2]) {
-    const int buf = (t % kStages) * kStage;
+  auto read = [&](int slot, i32x8 (&fa)[kMI][2], i32x8 (&fb)[kNI][2]) {
+    const int buf = slot * kStage;
 #pragma unroll
     for (int i = 0; i < kMI; ++i) read_frag(a_at, buf + i * 32 * kBK, fa[i]);
 #pragma unroll
@@ -268,8 +269,8 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
       read_scales((t + 1) >> 2, sa_next, sb_next);
       stage_scales(((t + 1) >> 2) + 1);
     }
-    stage(t + kStages);
-    read(t + 1, af[1 - cur], bf[1 - cur]);
+    stage(t + kStages, byte % kStages);
+    read((byte + 1) % kStages, af[1 - cur], bf[1 - cur]);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -296,7 +297,7 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
     stage_scales(0);
     stage_scales(1);
 #pragma unroll
-    for (int t = 0; t < kStages; ++t) stage(t);
+    for (int t = 0; t < kStages; ++t) stage(t, t);
     wait_vm<(kStages - 1) * kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -712,14 +713,35 @@ bool side_ok(const Fp8In& in, int64_t rows, int64_t K) {
 
 }  // namespace
 
-// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows, 4 = 64 x 64 tile; -1: not these sizes.
+// What a call takes on this card, in microseconds, by the tile: measured over 23 sizes from 33 x 4096 x
+// 4096 to 8192^3, which these lines fit within 20 % and order rightly but for near ties.  `r` is rounds
+// of 256 blocks, `nk` tiles of K.  Up to one round a block has a CU to itself and a K tile costs what its
+// loads take, the more the more blocks load at once; beyond it rounds add up, whole ones where one block
+// fills a CU.  Examples (128 x 128, 128 x 128 two per CU, 256 x 256, 64 x 64; us):
+//   256 x 4096 x 4096   16.2  15.9  36.4   8.6        2048 x 4096 x 4096  38.9  33.1  38.9   51.9
+//   1024 x 4096 x 4096  20.4  24.7  37.5  26.7        4096 x 4096 x 4096  76.4  64.0  55.9  101.3
+double tile_us(int variant, int64_t M, int64_t N, double nk) {
+  const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
+  const double r = double((M + edge - 1) / edge) * double((N + edge - 1) / edge) / 256, whole = std::ceil(r);
+  switch (variant) {
+    case 1: return r <= 1 ? 4 + (0.36 + 0.14 * r) * nk : whole * (3 + 0.5 * nk);
+    case 2: return r <= 1 ? 6 + 6 * r + (0.85 + 0.4 * r * r) * nk : 6 + whole * (10 + 1.28 * nk);
+    case 4: return r <= 1 ? 3 + 0.16 * nk : 2 + r * (1.2 + 0.19 * nk);
+    default: return r <= 1 ? 3 + (0.35 + 0.3 * r) * nk : 2 + r * (1.9 + 0.43 * nk);
+  }
+}
+
+// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows, 4 = 64 x 64 tile,
+// 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU); -1: not these sizes.
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
-  if (variant < 0 || variant > 4) return -1;
-  const int64_t tiles256 = ((M + 255) / 256) * ((N + 255) / 256);
-  if (variant == 2) return K >= kBK + 16 ? 2 : -1;  // two K tiles
-  if (variant == 3) return M <= 64 ? 3 : -1;
-  if (variant == 0) return M <= 64 ? 3 : K >= kBK + 16 && tiles256 >= 64 ? 2 : 1;
-  return variant;
+  const bool two_k_tiles = K >= kBK + 16;
+  if (variant < 0 || variant > 5 || (variant == 2 && !two_k_tiles) || (variant == 3 && M > 64)) return -1;
+  if (variant != 0) return variant;
+  if (M <= 16) return 3;
+  int best = 4;
+  for (int v : {1, 5, 2})
+    if ((v != 2 || two_k_tiles) && tile_us(v, M, N, double(K) / kBK) < tile_us(best, M, N, double(K) / kBK)) best = v;
+  return best;
 }
 
 namespace {
@@ -758,8 +780,9 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
       hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
                          c, g.ldc, int(g.K), vec_c);
     } else {
-      auto k = variant == 1 ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 4>
-                            : gemm_fp8_tile_kernel<a, b, decltype(tc), 64, 64, 6>;
+      auto k = variant == 1   ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 4>
+               : variant == 5 ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 2>
+                              : gemm_fp8_tile_kernel<a, b, decltype(tc), 64, 64, 4>;
       hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K), vec_c);
     }
   });
