@@ -44,8 +44,8 @@ struct GemmFp8Args {
   int64_t ldc;
   int64_t M, N, K;
   int ctype;
-  int variant;  // 0: by the sizes; 1: 128 x 128 tile, 2: 256 x 256 (K >= 144), 3: few rows (M <= 64), 4: 64 x 64,
-                // 5: 128 x 128 with two K tiles in LDS, so two blocks per CU
+  int variant;  // 0: by the sizes; 1: 128 x 128 tile, 2: 256 x 256 (K >= 144), 3: few rows (M <= 16), 4: 64 x 64,
+                // 5: 128 x 128 with two K tiles in LDS, so two blocks per CU, 6: few rows, 32 of B per wave
 };
 // the kernel that a call runs (0 resolved), or -1 if the sizes do not fit it
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant);

@@ -561,115 +561,92 @@ gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
   lds_to_c<256, 256, 512>(smem, C, ldc, A.rows, B.rows, row_a, row_b, vec_c);
 }
 
-// ---- few rows of A (one token to 64): B is read once, from memory straight into registers ----
-// Bound by B's bytes.  A block takes 16 * kR rows of B and all of A's (kMT tiles of 16); its waves
-// divide K in units of 512 bytes (four scale blocks: a row's four scales are one word, and 8 KiB of B
-// per 16 rows are in flight per wave and the next 8 KiB behind them).  A comes from the caches.  The
-// waves' sums are joined in LDS in the waves' order, so results do not depend on timing.
+// ---- up to 16 rows of A (tokens of a decoding step): B goes from memory straight to registers ----
+// Bound by B's bytes, read once.  A block takes 16 * kR rows of B; its waves divide K in units of 512
+// bytes (four scale blocks, so that a row's four scales are one word), whose loads are in flight
+// together, and many waves run on a CU.  Nothing is staged, since no two waves read the same of B (a ring
+// in LDS for each wave, which reads whole lines, took the same time).  A comes from the caches; 32 rows
+// of B per wave halve what is read of it.  The waves' sums are joined in LDS in the waves' order, so
+// results do not depend on timing.
 // B is the matrix instruction's first operand: a lane then holds 4 columns of C next to each other.
 constexpr int kQuad = 4 * kBK;
 
-template <int kA, int kB, int kMT, int kR>
+template <int kA, int kB, int kR>
 __global__ void __launch_bounds__(1024)
 gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int c_is_f16, int vec_c) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t dyn_smem[];
-  f32x4* part = reinterpret_cast<f32x4*>(dyn_smem);  // [wave][kMT * kR][lane]
+  __shared__ f32x4 part[16 * kR * 64];  // [wave][kR][lane]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int row_b = blockIdx.x * (16 * kR);
   const int K16 = K & ~15;
   const int nk = (K16 + kBK - 1) / kBK, quads = (nk + 3) / 4;
   const int q0 = quads * wave / waves, q1 = quads * (wave + 1) / waves;
-  const rsrc_t ra = tile_rsrc(A, 0, kMT * 16, K), rb = tile_rsrc(B, row_b, 16 * kR, K);
+  const rsrc_t ra = tile_rsrc(A, 0, 16, K), rb = tile_rsrc(B, row_b, 16 * kR, K);
   const int l15 = lane & 15, chunk = (lane >> 4) * 16;  // this lane's chunks of a block: chunk, chunk + 64
 
   const uint32_t* psb[kR];
-  const uint32_t* psa[kMT];
 #pragma unroll
   for (int r = 0; r < kR; ++r) {
     int n = row_b + r * 16 + l15;
     n = (n < B.rows ? n : B.rows - 1) >> B.shift;
     psb[r] = reinterpret_cast<const uint32_t*>(B.scale + int64_t(n) * B.lds);
   }
-#pragma unroll
-  for (int m = 0; m < kMT; ++m) {
-    int n = m * 16 + l15;
-    n = (n < A.rows ? n : A.rows - 1) >> A.shift;
-    psa[m] = reinterpret_cast<const uint32_t*>(A.scale + int64_t(n) * A.lds);
-  }
+  const int ma = (l15 < A.rows ? l15 : A.rows - 1) >> A.shift;
+  const uint32_t* psa = reinterpret_cast<const uint32_t*>(A.scale + int64_t(ma) * A.lds);
   // one scale block (128 bytes of K) of 16 rows; past K16 zeros
-  auto load = [&](rsrc_t rsrc, int64_t ld, int row, int k) {
-    const uint32_t at = uint32_t(row) * uint32_t(ld) + chunk;
+  auto load = [&](rsrc_t rsrc, uint32_t at, int k) {
     const i32x4 lo = __builtin_bit_cast(
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk < K16 - k ? at : kOob, k, 0));
     const i32x4 hi = __builtin_bit_cast(
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk + 64 < K16 - k ? at + 64 : kOob, k, 0));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto load_quad = [&](int q, i32x8 (&b)[kR][4], uint32_t (&sb)[kR], uint32_t (&sa)[kMT]) {
-#pragma unroll
-    for (int r = 0; r < kR; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[r][i] = load(rb, B.ld, r * 16 + l15, q * kQuad + i * kBK);
-#pragma unroll
-    for (int r = 0; r < kR; ++r) sb[r] = psb[r][q];
-#pragma unroll
-    for (int m = 0; m < kMT; ++m) sa[m] = psa[m][q];
-  };
+  const uint32_t at_a = uint32_t(l15) * uint32_t(A.ld) + chunk, at_b = uint32_t(l15) * uint32_t(B.ld) + chunk;
 
-  f32x4 acc[kMT][kR];
+  f32x4 acc[kR];
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
-#pragma unroll
-    for (int r = 0; r < kR; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-  i32x8 b[kR][4], b_next[kR][4];
-  uint32_t sb[kR], sa[kMT], sb_next[kR], sa_next[kMT];
-  if (q0 < q1) load_quad(q0, b, sb, sa);
+  for (int r = 0; r < kR; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int q = q0; q < q1; ++q) {
-    if (q + 1 < q1) load_quad(q + 1, b_next, sb_next, sa_next);
+    i32x8 a[4], b[kR][4];
+    uint32_t sb[kR];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int k = q * kQuad + i * kBK;
-      if (k < K16) {  // (behind K the scales are whatever pads their rows)
 #pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          const i32x8 a = load(ra, A.ld, m * 16 + l15, k);
-#pragma unroll
-          for (int r = 0; r < kR; ++r)
-            acc[m][r] = mfma<kB, kA>(b[r][i], a, acc[m][r], int(sb[r] >> (8 * i)), int(sa[m] >> (8 * i)));
-        }
-      }
+      for (int r = 0; r < kR; ++r) b[r][i] = load(rb, at_b + r * 16 * uint32_t(B.ld), q * kQuad + i * kBK);
+      a[i] = load(ra, at_a, q * kQuad + i * kBK);
     }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) sb[r] = psb[r][q];
+    uint32_t sa = psa[q];
+    // behind K the scales are whatever pads their rows, and the values are zeros: 2^0 will do
+    const int blocks = nk - q * 4;
+    const uint32_t pad = blocks >= 4 ? 0u : 0xffffffffu << (8 * blocks);
+    sa = (sa & ~pad) | (0x7f7f7f7fu & pad);
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[r][i] = b_next[r][i];
-      sb[r] = sb_next[r];
+      sb[r] = (sb[r] & ~pad) | (0x7f7f7f7fu & pad);
+      acc[r] = mfma<kB, kA, 0>(b[r][0], a[0], acc[r], int(sb[r]), int(sa));
+      acc[r] = mfma<kB, kA, 1>(b[r][1], a[1], acc[r], int(sb[r]), int(sa));
+      acc[r] = mfma<kB, kA, 2>(b[r][2], a[2], acc[r], int(sb[r]), int(sa));
+      acc[r] = mfma<kB, kA, 3>(b[r][3], a[3], acc[r], int(sb[r]), int(sa));
     }
-#pragma unroll
-    for (int m = 0; m < kMT; ++m) sa[m] = sa_next[m];
   }
   if (K != K16 && wave == waves - 1) {
+    const i32x8 a = tail_frag(ra, A.ld, l15, lane < 16, K);
+    const int s = tail_scale(A, l15, K);
 #pragma unroll
-    for (int m = 0; m < kMT; ++m) {
-      const i32x8 a = tail_frag(ra, A.ld, m * 16 + l15, lane < 16, K);
-      const int s = tail_scale(A, m * 16 + l15, K);
-#pragma unroll
-      for (int r = 0; r < kR; ++r)
-        acc[m][r] = mfma<kB, kA>(tail_frag(rb, B.ld, r * 16 + l15, lane < 16, K), a, acc[m][r],
-                                 tail_scale(B, row_b + r * 16 + l15, K), s);
-    }
+    for (int r = 0; r < kR; ++r)
+      acc[r] = mfma<kB, kA>(tail_frag(rb, B.ld, r * 16 + l15, lane < 16, K), a, acc[r],
+                            tail_scale(B, row_b + r * 16 + l15, K), s);
   }
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
-#pragma unroll
-    for (int r = 0; r < kR; ++r) part[(wave * kMT * kR + m * kR + r) * 64 + lane] = acc[m][r];
+  for (int r = 0; r < kR; ++r) part[(wave * kR + r) * 64 + lane] = acc[r];
   __syncthreads();
-  for (int i = threadIdx.x; i < kMT * kR * 64; i += blockDim.x) {
+  for (int i = threadIdx.x; i < kR * 64; i += blockDim.x) {
     f32x4 v = part[i];
-    for (int w = 1; w < waves; ++w) v += part[w * kMT * kR * 64 + i];
-    const int l = i & 63, m = i / 64 / kR, r = i / 64 % kR;
-    const int row = m * 16 + (l & 15), col = row_b + r * 16 + (l >> 4) * 4;
+    for (int w = 1; w < waves; ++w) v += part[w * kR * 64 + i];
+    const int l = i & 63, r = i >> 6;
+    const int row = l & 15, col = row_b + r * 16 + (l >> 4) * 4;
     if (row >= A.rows) continue;
     uint16_t h[4];
 #pragma unroll
@@ -731,13 +708,18 @@ double tile_us(int variant, int64_t M, int64_t N, double nk) {
   }
 }
 
-// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows, 4 = 64 x 64 tile,
-// 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU); -1: not these sizes.
+// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows (M <= 16), 4 = 64 x 64 tile,
+// 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU), 6 = few rows, 32 of B per wave;
+// -1: not these sizes.
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
   const bool two_k_tiles = K >= kBK + 16;
-  if (variant < 0 || variant > 5 || (variant == 2 && !two_k_tiles) || (variant == 3 && M > 64)) return -1;
+  if (variant < 0 || variant > 6 || (variant == 2 && !two_k_tiles) || ((variant == 3 || variant == 6) && M > 16)) return -1;
   if (variant != 0) return variant;
-  if (M <= 16) return 3;
+  // Up to 16 tokens: 16 rows of B per wave, or 32, which reads A half as often, where that still fills
+  // the card, or 64 x 64 tiles, which read A once, where B is very wide.  One and 16 tokens, weights
+  // from memory, us:  4096 x 8192  10.1 / 11.7 / 18.7 and 12.9 / 15.1 / 19.2
+  //   8192 x 8192  16.4 / 15.0 / 21.4 and 21.6 / 17.0 / 22.4     16384 x 2048  9.2 / 8.9 / 8.3 and 11.9 / 9.6 / 8.4
+  if (M <= 16) return N >= 16384 && (K <= 2048 || M > 8) ? 4 : N >= 8192 && K >= 2048 && (M > 4 || K >= 8192) ? 6 : 3;
   int best = 4;
   for (int v : {1, 5, 2})
     if ((v != 2 || two_k_tiles) && tile_us(v, M, N, double(K) / kBK) < tile_us(best, M, N, double(K) / kBK)) best = v;
@@ -746,15 +728,15 @@ int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
 
 namespace {
 
-template <int a, int b, int kMT, int kR>
+template <int a, int b, int kR>
 void launch_rows(const GemmFp8Args& g, Operand oa, Operand ob, hipStream_t stream) {
   const int64_t quads = ((g.K & ~int64_t(15)) + kQuad - 1) / kQuad;
   int waves = 1;
-  while (waves < 8 && waves * 2 <= quads) waves *= 2;
+  while (waves < 16 && waves < quads) waves *= 2;
   const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 8 == 0 && g.ldc % 4 == 0;
-  hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kMT, kR>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
-                     dim3(waves * 64), waves * kMT * kR * 64 * sizeof(f32x4), stream, oa, ob,
-                     static_cast<uint16_t*>(g.c), g.ldc, int(g.K), g.ctype == kF16, vec_c);
+  hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kR>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
+                     dim3(waves * 64), 0, stream, oa, ob, static_cast<uint16_t*>(g.c), g.ldc, int(g.K),
+                     g.ctype == kF16, vec_c);
 }
 
 }  // namespace
@@ -765,17 +747,16 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   const int variant = resolve_gemm_fp8_variant(g.M, g.N, g.K, g.variant);
   if (variant < 0) return hipErrorInvalidValue;
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
-  const int64_t tiles = variant == 3 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
+  const int64_t tiles = variant == 3 || variant == 6 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
   if (tiles >= (int64_t(1) << 22)) return hipErrorInvalidValue;  // 2^32 threads
   const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc % 8 == 0;
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
     const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
     uint16_t* c = static_cast<uint16_t*>(g.c);
-    if (variant == 3) {
-      if (g.M <= 16) launch_rows<a, b, 1, 1>(g, oa, ob, stream);
-      else if (g.M <= 32) launch_rows<a, b, 2, 1>(g, oa, ob, stream);
-      else launch_rows<a, b, 4, 1>(g, oa, ob, stream);
+    if (variant == 3 || variant == 6) {
+      if (variant == 3) launch_rows<a, b, 1>(g, oa, ob, stream);
+      else launch_rows<a, b, 2>(g, oa, ob, stream);
     } else if (variant == 2) {
       hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
                          c, g.ldc, int(g.K), vec_c);

@@ -179,7 +179,8 @@ PYBIND11_MODULE(_gpuexp_kernels, m) {
                        int64_t M, int64_t N, int64_t K, int ctype, int variant, uintptr_t stream) {
     gpuexp::GemmFp8Args g{};
     if (gpuexp::resolve_gemm_fp8_variant(M, N, K, variant) < 0)
-      throw std::invalid_argument("gemm_fp8: variant is 0 (auto), 1 (128x128), 2 (256x256, K >= 144), 3 (few rows, M <= 64), 4 (64x64) or 5 (128x128, two blocks per CU)");
+      throw std::invalid_argument("gemm_fp8: variant is 0 (auto), 1 (128x128), 2 (256x256, K >= 144), 3 (few rows, M <= 16), 4 (64x64), 5 (128x128, "
+                                  "two blocks per CU) or 6 (few rows, 32 of B per wave)");
     g.a = fp8_in(a, sa, lda, ldsa, block_a, type_a, M, K);
     g.b = fp8_in(b, sb, ldb, ldsb, block_b, type_b, N, K);
     if (!c || ldc < N || c % 2 || (ctype != 0 && ctype != 1))
@@ -193,7 +194,8 @@ PYBIND11_MODULE(_gpuexp_kernels, m) {
     g.variant = variant;
     check(gpuexp::launch_gemm_fp8(g, reinterpret_cast<hipStream_t>(stream)), "gemm_fp8 launch");
   }, "C[M,N] = A[M,K] @ B[N,K]^T; 8-bit operands with block scales, fp32 accumulate (scaled MFMA). The last argument but "
-     "the stream, variant: 0 auto, 1 = 128x128 tile, 2 = 256x256 tile, 3 = few rows, 4 = 64x64, 5 = 128x128 with two blocks per CU");
+     "the stream, variant: 0 auto, 1 = 128x128 tile, 2 = 256x256 tile, 3 = few rows, 4 = 64x64, 5 = 128x128 with two "
+     "blocks per CU, 6 = few rows, 32 of B per wave");
   m.def("gemm_fp8_variant", &gpuexp::resolve_gemm_fp8_variant, py::arg("M"), py::arg("N"), py::arg("K"),
         py::arg("variant") = 0,
         "The kernel variant a gemm_fp8 call with these sizes runs (0 = auto resolved), -1 if they do not fit it. "

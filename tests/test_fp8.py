@@ -137,3 +137,15 @@ def test_oracle_values_of_a_hand_made_pair():
     a = torch.tensor([[1.0, -2.0, 448.0]]).to(E4M3)
     s = torch.tensor([[128]], dtype=torch.uint8).view(E8M0)
     assert values(a, s).tolist() == [[2.0, -4.0, 896.0]]
+
+
+@pytest.mark.parametrize("M,N,K,variant,want", [
+    (8192, 8192, 8192, 0, 2), (4096, 4096, 4096, 0, 2),  # many tiles: 256 x 256
+    (2048, 4096, 4096, 0, 5), (1024, 4096, 4096, 0, 1), (333, 1001, 2050, 0, 4),
+    (1, 4096, 4096, 0, 3), (16, 8192, 8192, 0, 6), (16, 32768, 4096, 0, 4),
+    (8192, 8192, 128, 0, 5), (8192, 8192, 128, 2, -1),  # one K tile: not the 256 x 256 tile's
+    (17, 64, 64, 3, -1), (17, 64, 64, 6, -1), (16, 64, 64, 6, 6), (1, 1, 0, 0, 3), (100, 100, 0, 0, 4),
+    (64, 64, 64, 7, -1), (64, 64, 64, -1, -1),
+])
+def test_gemm_variant_resolution(native, M, N, K, variant, want):
+    assert kernels().gemm_fp8_variant(M, N, K, variant) == want

@@ -187,7 +187,7 @@ GEMMS = [(1, 1, 1), (1, 16, 128), (1, 1000, 640), (2, 129, 127), (5, 64, 16), (1
 
 
 @pytest.mark.parametrize("m,n,k", GEMMS)
-@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_is_exact_on_whole_numbers(m, n, k, variant):
     if kernels().gemm_fp8_variant(m, n, k, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
@@ -219,7 +219,7 @@ def test_gemm_on_random_operands(m, n, k, out):
 
 
 @pytest.mark.parametrize("m", [1, 16, 40, 200, 700])
-@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_repeats_bit_for_bit(m, variant):
     """Sums are joined in a fixed order: the same call gives the same bits (a tile read
     before it landed, or loaded over while read, would show here)."""
@@ -234,7 +234,7 @@ def test_gemm_repeats_bit_for_bit(m, variant):
 
 
 @pytest.mark.parametrize("m,n", [(3, 5), (16, 257), (130, 70), (300, 300), (512, 256)])
-@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_into_a_view_leaves_the_rest(m, n, variant):
     if kernels().gemm_fp8_variant(m, n, 384, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
@@ -259,7 +259,7 @@ def test_gemm_of_empty_sizes(m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 40, 300), (20, 40, 300), (200, 300, 300), (512, 512, 500)])
-@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_nan_and_inf_stay_in_their_row(m, n, k, variant):
     if kernels().gemm_fp8_variant(m, n, k, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
