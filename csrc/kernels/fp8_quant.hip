@@ -4,10 +4,10 @@
 //   e = min { e >= -127 : amax <= L 2^e },   amax = the block's largest finite magnitude,
 // L = 448 (e4m3) or 57344 (e5m2); a block of zeros has e = 0.  Both L are 1.75 * 2^p (p = 8,
 // 15), so for amax = m * 2^E, 1 <= m < 2, e = E - p + (m > 1.75): exact from the float's bits.
-// A power of two is what the scaled matrix instruction takes (a byte, e + 127), its product
-// with the values is exact, so a value is rounded ONCE, to nearest even, by the conversion;
-// an infinity becomes the type's infinity (e5m2) or NaN (e4m3), a NaN stays NaN.
-// A 16- or 32-bit input is read as it is: nothing is rounded before the conversion.
+// A power of two is what the scaled matrix instruction takes (a byte, e + 127) and what the scaled
+// conversions of this chip take (a float with that byte as its exponent; they divide or multiply by it
+// exactly, all 256 bytes checked), so a value is rounded ONCE, to nearest even, by the conversion; an
+// infinity becomes the type's infinity (e5m2) or NaN (e4m3), a NaN stays NaN.
 //
 // All kernels here are bound by memory: 3 bytes move for each bfloat16 value that is quantised.
 #include "fp8_launch.h"
@@ -20,163 +20,158 @@ namespace {
 
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+typedef __attribute__((ext_vector_type(2))) short s16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 constexpr int kQThreads = 256;
 
-__device__ __forceinline__ uint32_t bits(float v) { return __float_as_uint(v); }
-
-// finite magnitudes order as their bits; infinities and NaN count as zero
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t b = bits(v) & 0x7fffffffu;
-  return b >= 0x7f800000u ? 0u : b;
-}
-
+// The byte e + 127 of a block whose largest finite magnitude has these bits (of a 32-bit float).
 template <int kType>
-__device__ __forceinline__ int block_exponent(uint32_t amax) {
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
   constexpr int p = kType == kE4M3 ? 8 : 15;
-  if (amax == 0) return 0;
-  const int e = int(amax >> 23) - 127 - p + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < -127 ? -127 : e;  // (subnormal amax included: its exponent field is 0)
+  const int byte = int(amax >> 23) - p + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return amax == 0 ? 127 : byte < 0 ? 0 : byte;  // (a subnormal amax too: its exponent field is 0)
 }
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float(uint32_t(byte) << 23); }
 
-// 2^-e as a float: e in [-127, 120], so always a normal number
-__device__ __forceinline__ float inv_scale(int e) { return __uint_as_float(uint32_t(127 - e) << 23); }
+// ---- 8 values next to each other: 4 words of 16-bit values, or 8 of 32 ----
+template <int kX>
+struct Eight {
+  static constexpr int kWords = kX == kF32 ? 8 : 4;
+  uint32_t w[kWords];
+};
 
-template <int kType>
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  int r = 0;
-  if constexpr (kType == kE4M3) {
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
-  } else {
-    r = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, r, false);
-    r = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, r, true);
+// From element i of x; those behind the first n read as 0 and are not touched in memory.
+// kVec: i is a multiple of 8 elements on a 16-byte boundary.
+template <int kX, bool kVec>
+__device__ __forceinline__ Eight<kX> load8(const void* x, int64_t i, int n) {
+  Eight<kX> v;
+  if (kVec && n >= 8) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const char*>(x) + i * (kX == kF32 ? 4 : 2));
+#pragma unroll
+    for (int j = 0; j < Eight<kX>::kWords; ++j) v.w[j] = p[j >> 2][j & 3];
+    return v;
   }
-  return uint32_t(r);
+#pragma unroll
+  for (int j = 0; j < Eight<kX>::kWords; ++j) {
+    if constexpr (kX == kF32) {
+      v.w[j] = j < n ? static_cast<const uint32_t*>(x)[i + j] : 0;
+    } else {
+      const uint16_t* p = static_cast<const uint16_t*>(x) + i;
+      v.w[j] = 2 * j < n ? p[2 * j] : 0;
+      if (2 * j + 1 < n) v.w[j] |= uint32_t(p[2 * j + 1]) << 16;
+    }
+  }
+  return v;
 }
 
-template <int kType>
-__device__ __forceinline__ void unpack4(uint32_t w, float* v) {
-  typedef __attribute__((ext_vector_type(2))) float f32x2;
-  f32x2 lo, hi;
-  if constexpr (kType == kE4M3) {
-    lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false);
-    hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), true);
-  } else {
-    lo = __builtin_amdgcn_cvt_pk_f32_bf8(int(w), false);
-    hi = __builtin_amdgcn_cvt_pk_f32_bf8(int(w), true);
-  }
-  v[0] = lo[0];
-  v[1] = lo[1];
-  v[2] = hi[0];
-  v[3] = hi[1];
+__device__ __forceinline__ uint32_t max2x16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
+
+// Magnitudes order as their bits.  `mags` of 16-bit values keeps two columns in a word; the first infinity
+// has the bits kInf.
+template <int kX>
+constexpr uint32_t kInf = kX == kBF16 ? 0x7f80u : kX == kF16 ? 0x7c00u : 0x7f800000u;
 
 template <int kX>
-__device__ __forceinline__ float widen(const void* p, int64_t i) {
-  if constexpr (kX == kBF16) return __uint_as_float(uint32_t(static_cast<const uint16_t*>(p)[i]) << 16);
-  if constexpr (kX == kF16) return float(static_cast<const _Float16*>(p)[i]);
-  if constexpr (kX == kF32) return static_cast<const float*>(p)[i];
+__device__ __forceinline__ uint32_t mag(uint32_t w) {
+  return w & (kX == kF32 ? 0x7fffffffu : 0x7fff7fffu);
 }
-
-// 8 consecutive values from element i of x; those behind the first n read as 0 and are not
-// touched in memory.  kVec: i is a multiple of 8 elements on a 16-byte boundary.
-template <int kX, bool kVec>
-__device__ __forceinline__ void load8(const void* x, int64_t i, int n, float* v) {
-  if (kVec && n >= 8) {
-    if constexpr (kX == kF32) {
-      const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(x) + i);
-      const u32x4 a = p[0], b = p[1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = __uint_as_float(a[j]);
-        v[4 + j] = __uint_as_float(b[j]);
-      }
-    } else {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kX == kBF16) {
-          v[2 * j] = __uint_as_float(a[j] << 16);
-          v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
-        } else {
-          typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-          const uint32_t w = a[j];
-          const f16x2 h = __builtin_bit_cast(f16x2, w);
-          v[2 * j] = float(h[0]);
-          v[2 * j + 1] = float(h[1]);
-        }
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < n ? widen<kX>(x, i + j) : 0.f;
-}
-
 template <int kX>
-__device__ __forceinline__ uint32_t narrow(float v) {  // one rounding, to nearest even
-  if constexpr (kX == kBF16) {
-    const __bf16 h = (__bf16)v;
-    return __builtin_bit_cast(uint16_t, h);
-  } else {
-    const _Float16 h = (_Float16)v;
-    return __builtin_bit_cast(uint16_t, h);
-  }
+__device__ __forceinline__ uint32_t max_mag(uint32_t a, uint32_t b) {
+  if constexpr (kX == kF32) return max(a, b);
+  else return max2x16(a, b);
+}
+// the same without what is not finite
+template <int kX>
+__device__ __forceinline__ uint32_t finite_mag(uint32_t w) {
+  const uint32_t m = mag<kX>(w);
+  if constexpr (kX == kF32) return m < kInf<kX> ? m : 0;
+  else return ((m & 0xffffu) < kInf<kX> ? m & 0xffffu : 0) | ((m >> 16) < kInf<kX> ? m & 0xffff0000u : 0);
+}
+// the larger of the two in a word
+template <int kX>
+__device__ __forceinline__ uint32_t widest(uint32_t m) {
+  if constexpr (kX == kF32) return m;
+  else return max(m & 0xffffu, m >> 16);
+}
+// a magnitude as the bits of a 32-bit float
+template <int kX>
+__device__ __forceinline__ uint32_t mag_bits(uint32_t m) {
+  if constexpr (kX == kF32) return m;
+  if constexpr (kX == kBF16) return m << 16;
+  if constexpr (kX == kF16) return __float_as_uint(float(__builtin_bit_cast(_Float16, uint16_t(m))));
 }
 
-template <int kX, bool kVec>
-__device__ __forceinline__ void store8(void* x, int64_t i, int n, const float* v) {
-  if (kVec && n >= 8) {
-    if constexpr (kX == kF32) {
-      u32x4 a, b;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j] = bits(v[j]);
-        b[j] = bits(v[4 + j]);
-      }
-      u32x4* p = reinterpret_cast<u32x4*>(static_cast<float*>(x) + i);
-      p[0] = a;
-      p[1] = b;
-    } else {
-      u32x4 a;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) a[j] = narrow<kX>(v[2 * j]) | (narrow<kX>(v[2 * j + 1]) << 16);
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(x) + i) = a;
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) {
-      if constexpr (kX == kF32) static_cast<float*>(x)[i + j] = v[j];
-      else static_cast<uint16_t*>(x)[i + j] = uint16_t(narrow<kX>(v[j]));
-    }
-}
-
-// the first n of 8 bytes; a tensor's rows start at multiples of 16 bytes and are padded to
-// them, so a whole 8-byte store never leaves the row (n >= 1)
-__device__ __forceinline__ void store_q8(uint8_t* q, u32x2 w) { *reinterpret_cast<u32x2*>(q) = w; }
-
-template <int kType>
-__device__ __forceinline__ u32x2 quantize8(const float* v, float inv) {
-  return u32x2{pack4<kType>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-               pack4<kType>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
-}
-
-__device__ __forceinline__ uint32_t max8(const float* v) {
+// largest finite magnitude of the eight
+template <int kX>
+__device__ __forceinline__ uint32_t max8(const Eight<kX>& v) {
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, finite_bits(v[j]));
+  for (int j = 0; j < Eight<kX>::kWords; ++j) m = max_mag<kX>(m, mag<kX>(v.w[j]));
+  m = widest<kX>(m);
+  if (m >= kInf<kX>) {  // hardly ever
+    m = 0;
+#pragma unroll
+    for (int j = 0; j < Eight<kX>::kWords; ++j) m = max_mag<kX>(m, finite_mag<kX>(v.w[j]));
+    m = widest<kX>(m);
+  }
   return m;
 }
 
-// largest of the 16 lanes that share a block's row
+// largest of 16 lanes next to each other: three xors and a mirror inside the lanes' data path
 __device__ __forceinline__ uint32_t max16(uint32_t m) {
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = max(m, uint32_t(__shfl_xor(int(m), d)));
+  m = max(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), 0xB1, 0xf, 0xf, true)));   // lane ^ 1
+  m = max(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), 0x4E, 0xf, 0xf, true)));   // lane ^ 2
+  m = max(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), 0x141, 0xf, 0xf, true)));  // mirrored in 8
+  m = max(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), 0x140, 0xf, 0xf, true)));  // mirrored in 16
   return m;
 }
+
+// two values in 8 bits, into the low or high half of a word
+template <int kX, int kType, bool kHigh>
+__device__ __forceinline__ s16x2 convert2(s16x2 old, uint32_t w, float scale) {
+  if constexpr (kX == kBF16) {
+    const bf16x2 v = __builtin_bit_cast(bf16x2, w);
+    if constexpr (kType == kE4M3) return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, v, scale, kHigh);
+    else return __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(old, v, scale, kHigh);
+  } else {
+    const f16x2 v = __builtin_bit_cast(f16x2, w);
+    if constexpr (kType == kE4M3) return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, v, scale, kHigh);
+    else return __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(old, v, scale, kHigh);
+  }
+}
+template <int kType, bool kHigh>
+__device__ __forceinline__ s16x2 convert2(s16x2 old, float a, float b, float scale) {
+  if constexpr (kType == kE4M3) return __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(old, a, b, scale, kHigh);
+  else return __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(old, a, b, scale, kHigh);
+}
+// four values: words of two 16-bit values each, or floats
+template <int kX, int kType>
+__device__ __forceinline__ uint32_t convert4(uint32_t a, uint32_t b, float scale) {
+  const s16x2 lo = convert2<kX, kType, false>(s16x2{0, 0}, a, scale);
+  return __builtin_bit_cast(uint32_t, convert2<kX, kType, true>(lo, b, scale));
+}
+template <int kType>
+__device__ __forceinline__ uint32_t convert4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, float scale) {
+  const s16x2 lo = convert2<kType, false>(s16x2{0, 0}, __uint_as_float(a), __uint_as_float(b), scale);
+  return __builtin_bit_cast(uint32_t, convert2<kType, true>(lo, __uint_as_float(c), __uint_as_float(d), scale));
+}
+template <int kX, int kType>
+__device__ __forceinline__ u32x2 convert8(const Eight<kX>& v, float scale) {
+  if constexpr (kX == kF32)
+    return u32x2{convert4<kType>(v.w[0], v.w[1], v.w[2], v.w[3], scale), convert4<kType>(v.w[4], v.w[5], v.w[6], v.w[7], scale)};
+  else
+    return u32x2{convert4<kX, kType>(v.w[0], v.w[1], scale), convert4<kX, kType>(v.w[2], v.w[3], scale)};
+}
+
+// A tensor's rows start at multiples of 16 bytes and are padded to them, so an 8-byte access at a
+// multiple of 8 below its columns never leaves the row.
+__device__ __forceinline__ void store_q8(uint8_t* q, u32x2 w) { *reinterpret_cast<u32x2*>(q) = w; }
 
 // u / d for u < 2^31: m = ceil(2^(31 + s) / d) with 2^(s-1) < d <= 2^s is at most 2^32 - 1
 struct FastDiv {
@@ -200,124 +195,197 @@ quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int cols, uint32_t
   if (u >= units) return;  // whole groups of 16 lanes
   const uint32_t row = div(u, nb), blk = u - row * nb.d;
   const int col = int(blk) * kFp8Block + (threadIdx.x & 15) * 8;
-  float v[8];
-  load8<kX, kVec>(x, int64_t(row) * ldx + col, cols - col, v);
-  const int e = block_exponent<kType>(max16(max8(v)));
-  if (col < cols) store_q8(out.q + int64_t(row) * out.ld + col, quantize8<kType>(v, inv_scale(e)));
-  if ((threadIdx.x & 15) == 0) out.scale[int64_t(row) * out.lds + blk] = uint8_t(e + 127);
+  const Eight<kX> v = load8<kX, kVec>(x, int64_t(row) * ldx + col, cols - col);
+  const int byte = scale_byte<kType>(mag_bits<kX>(max16(max8<kX>(v))));
+  if (col < cols) store_q8(out.q + int64_t(row) * out.ld + col, convert8<kX, kType>(v, scale_of(byte)));
+  if ((threadIdx.x & 15) == 0) out.scale[int64_t(row) * out.lds + blk] = uint8_t(byte);
 }
 
 // ---- a 128 x 128 tile: 256 threads, each 8 rows x 8 columns ----
 // Thread t holds rows (t/16)*8 + i and columns (t%16)*8 + j, so 16 lanes read a row's 128
 // values together, a row's largest is 4 exchanges between those lanes, and the 8 bytes of one
-// column are one 8-byte write into the transposed tile in LDS.
+// column are one 8-byte write into the transposed tile in LDS.  16-bit values stay as they were read,
+// two columns to a word, in maxima and conversions alike: 3 instructions a value, and few registers.
 //   square: one scale for the tile.   rows: a scale for each row (out) and each column (outT).
 // The LDS image is [column][row] bytes; the 8-byte slot of a column is swizzled by the column's
 // group of 8 so that the 16 lanes of a write, 8 columns apart, fall into different banks.
 __device__ __forceinline__ int slot(int col, int r8) { return col * 128 + ((r8 ^ ((col >> 3) & 15)) << 3); }
 
-template <int kX, int kType, bool kSquare, bool kVec>
-__global__ void __launch_bounds__(kQThreads)
-quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, uint32_t tiles_n,
-                     Fp8Out out, Fp8Out outT) {
-  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
-  __shared__ uint32_t colmax[4][128];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int64_t r0 = int64_t(blockIdx.x / tiles_n) * 128;
-  const int64_t c0 = int64_t(blockIdx.x % tiles_n) * 128;
-  const int r8 = t >> 4, cj = (t & 15) * 8;
-  const int64_t col = c0 + cj;
-  const int ncol = col < cols ? int(cols - col < 8 ? cols - col : 8) : 0;
-  float v[8][8];
+// columns 2 c and 2 c + 1 (16-bit: of word c; 32-bit: columns c) of 8 rows, each 8 bytes to its slot
+template <int kX, int kType, int kC>
+__device__ __forceinline__ void column_to_tile(const Eight<kX> (&v)[8], uint8_t* tile, int cj, int r8, int lo, int hi) {
+  if constexpr (kX == kF32) {
+    const float s = scale_of(lo);
+    *reinterpret_cast<u32x2*>(tile + slot(cj + kC, r8)) =
+        u32x2{convert4<kType>(v[0].w[kC], v[1].w[kC], v[2].w[kC], v[3].w[kC], s),
+              convert4<kType>(v[4].w[kC], v[5].w[kC], v[6].w[kC], v[7].w[kC], s)};
+  } else {
+    uint32_t a[4], b[4];  // the low and the high column, two rows to a word
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __builtin_amdgcn_perm(v[2 * i + 1].w[kC], v[2 * i].w[kC], 0x05040100u);
+      b[i] = __builtin_amdgcn_perm(v[2 * i + 1].w[kC], v[2 * i].w[kC], 0x07060302u);
+    }
+    const float s = scale_of(lo), t = scale_of(hi);
+    *reinterpret_cast<u32x2*>(tile + slot(cj + 2 * kC, r8)) =
+        u32x2{convert4<kX, kType>(a[0], a[1], s), convert4<kX, kType>(a[2], a[3], s)};
+    *reinterpret_cast<u32x2*>(tile + slot(cj + 2 * kC + 1, r8)) =
+        u32x2{convert4<kX, kType>(b[0], b[1], t), convert4<kX, kType>(b[2], b[3], t)};
+  }
+}
+
+// 16 lanes write 128 bytes of one column of the tile in LDS
+__device__ __forceinline__ void tile_to_rows(const uint8_t* tile, Fp8Out outT, int64_t rows, int64_t cols, int64_t r0,
+                                             int64_t c0) {
+  const int t = threadIdx.x;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t row = r0 + r8 * 8 + i;
-    load8<kX, kVec>(x, row * ldx + col, row < rows ? ncol : 0, v[i]);
-  }
-  int ecol[8];
-  if constexpr (kSquare) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, max8(v[i]));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = max(m, uint32_t(__shfl_xor(int(m), d)));
-    if (lane == 0) colmax[wave][0] = m;
-    __syncthreads();
-    m = max(max(colmax[0][0], colmax[1][0]), max(colmax[2][0], colmax[3][0]));
-    const int e = block_exponent<kType>(m);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ecol[j] = e;
-    const float inv = inv_scale(e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t row = r0 + r8 * 8 + i;
-      if (out.q && row < rows && ncol > 0) store_q8(out.q + row * out.ld + col, quantize8<kType>(v[i], inv));
-    }
-    if (t == 0) {
-      if (out.q) out.scale[(r0 / 128) * out.lds + c0 / 128] = uint8_t(e + 127);
-      if (outT.q) outT.scale[(c0 / 128) * outT.lds + r0 / 128] = uint8_t(e + 127);
-    }
-  } else {
-    uint32_t m[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m[j] = max(m[j], finite_bits(v[i][j]));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = max(m[j], uint32_t(__shfl_xor(int(m[j]), 16)));
-      m[j] = max(m[j], uint32_t(__shfl_xor(int(m[j]), 32)));
-    }
-    if (lane < 16) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) colmax[wave][cj + j] = m[j];
-    }
-    // rows, while the column maxima travel
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t row = r0 + r8 * 8 + i;
-      const int e = block_exponent<kType>(max16(max8(v[i])));
-      if (out.q && row < rows) {
-        if (ncol > 0) store_q8(out.q + row * out.ld + col, quantize8<kType>(v[i], inv_scale(e)));
-        if ((t & 15) == 0) out.scale[row * out.lds + c0 / 128] = uint8_t(e + 127);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = cj + j;
-      ecol[j] = block_exponent<kType>(max(max(colmax[0][c], colmax[1][c]), max(colmax[2][c], colmax[3][c])));
-    }
-    if (r8 == 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < ncol) outT.scale[(col + j) * outT.lds + r0 / 128] = uint8_t(ecol[j] + 127);
-    }
-  }
-  if (!outT.q) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float inv = inv_scale(ecol[j]);
-    u32x2 w;
-    w[0] = pack4<kType>(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
-    w[1] = pack4<kType>(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv);
-    *reinterpret_cast<u32x2*>(tile + slot(cj + j, r8)) = w;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {  // 16 lanes write 128 bytes of one column
     const int c = i * 16 + (t >> 4), k8 = t & 15;
     if (c0 + c < cols && r0 + k8 * 8 < rows)
       store_q8(outT.q + (c0 + c) * outT.ld + r0 + k8 * 8, *reinterpret_cast<const u32x2*>(tile + slot(c, k8)));
   }
 }
 
+template <int kX, int kType, bool kSquare, bool kVec>
+__global__ void __launch_bounds__(kQThreads, 4)
+quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, uint32_t tiles_n,
+                     Fp8Out out, Fp8Out outT) {
+  constexpr int kWords = Eight<kX>::kWords;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
+  __shared__ uint32_t colmax[4][16 * kWords];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int64_t r0 = int64_t(blockIdx.x / tiles_n) * 128;
+  const int64_t c0 = int64_t(blockIdx.x % tiles_n) * 128;
+  const int r8 = t >> 4, cj = (t & 15) * 8;
+  const int64_t col = c0 + cj;
+  const int ncol = col < cols ? int(cols - col < 8 ? cols - col : 8) : 0;
+  const int nrow = int(rows - r0 - r8 * 8 < 8 ? rows - r0 - r8 * 8 : 8);  // may be <= 0
+  Eight<kX> v[8];
+  const int64_t first = (r0 + r8 * 8) * ldx + col;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = load8<kX, kVec>(x, first + i * ldx, i < nrow ? ncol : 0);
+  // the columns' largest, packed as they were read
+  uint32_t m[kWords];
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) m[j] = mag<kX>(v[0].w[j]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) m[j] = max_mag<kX>(m[j], mag<kX>(v[i].w[j]));
+  uint32_t all = m[0];
+#pragma unroll
+  for (int j = 1; j < kWords; ++j) all = max_mag<kX>(all, m[j]);
+  if (widest<kX>(all) >= kInf<kX>) {  // hardly ever
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      m[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[j] = max_mag<kX>(m[j], finite_mag<kX>(v[i].w[j]));
+    }
+  }
+  uint8_t* const q = out.q + (r0 + r8 * 8) * out.ld + col;
+  int bytes[2 * kWords > 8 ? 8 : 2 * kWords];  // of the 8 columns
+  if constexpr (kSquare) {
+    all = m[0];
+#pragma unroll
+    for (int j = 1; j < kWords; ++j) all = max_mag<kX>(all, m[j]);
+    all = max16(widest<kX>(all));
+    all = max(all, uint32_t(__shfl_xor(int(all), 16)));
+    all = max(all, uint32_t(__shfl_xor(int(all), 32)));
+    if (lane == 0) colmax[wave][0] = all;
+    __syncthreads();
+    all = max(max(colmax[0][0], colmax[1][0]), max(colmax[2][0], colmax[3][0]));
+    const int byte = scale_byte<kType>(mag_bits<kX>(all));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bytes[j] = byte;
+    if (out.q && ncol > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < nrow) store_q8(q + i * out.ld, convert8<kX, kType>(v[i], scale_of(byte)));
+    }
+    if (t == 0) {
+      if (out.q) out.scale[(r0 / 128) * out.lds + c0 / 128] = uint8_t(byte);
+      if (outT.q) outT.scale[(c0 / 128) * outT.lds + r0 / 128] = uint8_t(byte);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      m[j] = max_mag<kX>(m[j], uint32_t(__shfl_xor(int(m[j]), 16)));
+      m[j] = max_mag<kX>(m[j], uint32_t(__shfl_xor(int(m[j]), 32)));
+    }
+    if (lane < 16) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) colmax[wave][lane * kWords + j] = m[j];
+    }
+    if (out.q) {  // rows, while the columns' maxima travel
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int byte = scale_byte<kType>(mag_bits<kX>(max16(max8<kX>(v[i]))));
+        if (i < nrow) {
+          if (ncol > 0) store_q8(q + i * out.ld, convert8<kX, kType>(v[i], scale_of(byte)));
+          if ((t & 15) == 0) out.scale[(r0 + r8 * 8 + i) * out.lds + c0 / 128] = uint8_t(byte);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      const int c = (t & 15) * kWords + j;
+      const uint32_t top = max_mag<kX>(max_mag<kX>(colmax[0][c], colmax[1][c]), max_mag<kX>(colmax[2][c], colmax[3][c]));
+      if constexpr (kX == kF32) {
+        bytes[j] = scale_byte<kType>(top);
+      } else {
+        bytes[2 * j] = scale_byte<kType>(mag_bits<kX>(top & 0xffffu));
+        bytes[2 * j + 1] = scale_byte<kType>(mag_bits<kX>(top >> 16));
+      }
+    }
+    if (r8 == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < ncol) outT.scale[(col + j) * outT.lds + r0 / 128] = uint8_t(bytes[j]);
+    }
+  }
+  if (!outT.q) return;
+  if constexpr (kX == kF32) {
+    column_to_tile<kX, kType, 0>(v, tile, cj, r8, bytes[0], 0);
+    column_to_tile<kX, kType, 1>(v, tile, cj, r8, bytes[1], 0);
+    column_to_tile<kX, kType, 2>(v, tile, cj, r8, bytes[2], 0);
+    column_to_tile<kX, kType, 3>(v, tile, cj, r8, bytes[3], 0);
+    column_to_tile<kX, kType, 4>(v, tile, cj, r8, bytes[4], 0);
+    column_to_tile<kX, kType, 5>(v, tile, cj, r8, bytes[5], 0);
+    column_to_tile<kX, kType, 6>(v, tile, cj, r8, bytes[6], 0);
+    column_to_tile<kX, kType, 7>(v, tile, cj, r8, bytes[7], 0);
+  } else {
+    column_to_tile<kX, kType, 0>(v, tile, cj, r8, bytes[0], bytes[1]);
+    column_to_tile<kX, kType, 1>(v, tile, cj, r8, bytes[2], bytes[3]);
+    column_to_tile<kX, kType, 2>(v, tile, cj, r8, bytes[4], bytes[5]);
+    column_to_tile<kX, kType, 3>(v, tile, cj, r8, bytes[6], bytes[7]);
+  }
+  __syncthreads();
+  tile_to_rows(tile, outT, rows, cols, r0, c0);
+}
+
 // ---- 8 bits -> 16 or 32 bits: exact but for the one rounding into f16 / bf16 (a value of 8
-// bits times a power of two has at most 4 significant bits) ----
-__device__ __forceinline__ float scaled(float v, int byte) {  // byte 255 is NaN
-  return byte == 255 ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(v, byte - 127);
+// bits times a power of two has at most 4 significant bits); a scale of NaN gives NaN ----
+template <int kX, int kType, bool kHigh>
+__device__ __forceinline__ void widen2(uint32_t w, float scale, uint32_t* out) {
+  if constexpr (kX == kF32) {
+    f32x2 v;
+    if constexpr (kType == kE4M3) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, kHigh);
+    else v = __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(w, scale, kHigh);
+    out[0] = __float_as_uint(v[0]);
+    out[1] = __float_as_uint(v[1]);
+  } else if constexpr (kX == kBF16) {
+    if constexpr (kType == kE4M3)
+      *out = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHigh));
+    else
+      *out = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, scale, kHigh));
+  } else {
+    if constexpr (kType == kE4M3)
+      *out = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, kHigh));
+    else
+      *out = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, scale, kHigh));
+  }
 }
 
 template <int kX, int kType, bool kVec>
@@ -329,24 +397,54 @@ dequantize_kernel(Fp8In in, int cols, uint32_t units, FastDiv nb, int row_shift,
   const int col = int(blk) * kFp8Block + (threadIdx.x & 15) * 8;
   if (col >= cols) return;
   const u32x2 w = *reinterpret_cast<const u32x2*>(in.q + int64_t(row) * in.ld + col);
-  const int s = in.scale[int64_t(row >> row_shift) * in.lds + blk];
-  float v[8];
-  unpack4<kType>(w[0], v);
-  unpack4<kType>(w[1], v + 4);
+  const float s = scale_of(in.scale[int64_t(row >> row_shift) * in.lds + blk]);
+  constexpr int kTwo = kX == kF32 ? 2 : 1;  // words of two values
+  Eight<kX> v;
+  widen2<kX, kType, false>(w[0], s, v.w);
+  widen2<kX, kType, true>(w[0], s, v.w + kTwo);
+  widen2<kX, kType, false>(w[1], s, v.w + 2 * kTwo);
+  widen2<kX, kType, true>(w[1], s, v.w + 3 * kTwo);
+  const int64_t i = int64_t(row) * ldx + col;
+  const int n = cols - col;
+  if (kVec && n >= 8) {
+    u32x4* p = reinterpret_cast<u32x4*>(static_cast<char*>(x) + i * (kX == kF32 ? 4 : 2));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = scaled(v[j], s);
-  store8<kX, kVec>(x, int64_t(row) * ldx + col, cols - col, v);
+    for (int j = 0; j < Eight<kX>::kWords / 4; ++j) p[j] = u32x4{v.w[4 * j], v.w[4 * j + 1], v.w[4 * j + 2], v.w[4 * j + 3]};
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) {
+      if constexpr (kX == kF32) static_cast<uint32_t*>(x)[i + j] = v.w[j];
+      else static_cast<uint16_t*>(x)[i + j] = uint16_t(v.w[j >> 1] >> (16 * (j & 1)));
+    }
 }
 
 // ---- transpose: the layout of a tile is that of quantize_tile_kernel ----
-// rows: every column of 128 rows gets its own scale.  Its largest magnitude is found without
-// rounding: |q| 2^(e - 16) is a float for every e (the shift keeps the largest below infinity),
-// and what falls below the smallest subnormal, which only blocks reach whose exponent is
-// clamped anyway, still counts as not zero.  The new value is q 2^(e - e'), rounded once: with
-// powers of two on both sides it changes only where it leaves the type's normal range, that is
-// 2^-14 below its block's largest (e4m3).
+// rows: every column of 128 rows gets its own scale.  Its largest magnitude is found without rounding:
+// the bits of |q| as a 32-bit float plus the row's scale byte in the exponent's place order the products
+// as unsigned integers (the exponents sum to at most 142 + 254 < 512).  The new value is q 2^(e - e'),
+// rounded once: with powers of two on both sides it changes only where it leaves the type's normal range,
+// that is 2^-14 below its block's largest (e4m3).
+template <int kType, bool kHigh>
+__device__ __forceinline__ f32x2 values2(uint32_t w) {
+  if constexpr (kType == kE4M3) return __builtin_amdgcn_cvt_pk_f32_fp8(int(w), kHigh);
+  else return __builtin_amdgcn_cvt_pk_f32_bf8(int(w), kHigh);
+}
+template <int kType>
+__device__ __forceinline__ void values8(u32x2 w, float* v) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2 lo = values2<kType, false>(w[h]), hi = values2<kType, true>(w[h]);
+    v[4 * h] = lo[0];
+    v[4 * h + 1] = lo[1];
+    v[4 * h + 2] = hi[0];
+    v[4 * h + 3] = hi[1];
+  }
+}
+
 template <int kType, bool kSquare>
-__global__ void __launch_bounds__(kQThreads)
+__global__ void __launch_bounds__(kQThreads, 4)
 transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out outT) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
   __shared__ uint32_t colmax[4][128];
@@ -356,16 +454,11 @@ transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out 
   const int r8 = t >> 4, cj = (t & 15) * 8;
   const int64_t col = c0 + cj;
   const bool on = col < cols;
+  const int nrow = int(rows - r0 - r8 * 8 < 8 ? rows - r0 - r8 * 8 : 8);
+  const uint8_t* const q = in.q + (r0 + r8 * 8) * in.ld + col;
   u32x2 w[8];
-  int e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = r0 + r8 * 8 + i;
-    const bool here = on && row < rows;
-    w[i] = here ? *reinterpret_cast<const u32x2*>(in.q + row * in.ld + col) : u32x2{0, 0};
-    e[i] = 127;
-    if (!kSquare && here) e[i] = in.scale[row * in.lds + c0 / 128];
-  }
+  for (int i = 0; i < 8; ++i) w[i] = on && i < nrow ? *reinterpret_cast<const u32x2*>(q + i * in.ld) : u32x2{0, 0};
   if constexpr (kSquare) {
     if (t == 0) outT.scale[(c0 / 128) * outT.lds + r0 / 128] = in.scale[(r0 / 128) * in.lds + c0 / 128];
 #pragma unroll
@@ -376,20 +469,24 @@ transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out 
       *reinterpret_cast<u32x2*>(tile + slot(cj + j, r8)) = o;
     }
   } else {
-    float v[8][8];
+    int e[8];  // the rows' scale bytes
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < nrow ? in.scale[(r0 + r8 * 8 + i) * in.lds + c0 / 128] : 127;
+    constexpr uint32_t kNan = kType == kE4M3 ? 0x7f7f7f7fu : 0x7e7e7e7eu;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e[i] == 255) w[i] = u32x2{kNan, kNan};
     uint32_t m[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) m[j] = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      unpack4<kType>(w[i][0], v[i]);
-      unpack4<kType>(w[i][1], v[i] + 4);
+      float v[8];
+      values8<kType>(w[i], v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (e[i] == 255) v[i][j] = __uint_as_float(0x7fc00000u);
-        const uint32_t b = finite_bits(__builtin_ldexpf(v[i][j], e[i] - 127 - 16));
-        const bool some = (bits(v[i][j]) & 0x7fffffffu) - 1u < 0x7f7fffffu;  // finite and not zero
-        m[j] = max(m[j], some && b == 0 ? 1u : b);
+        const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
+        m[j] = max(m[j], b - 1 < 0x7f7fffffu ? b + (uint32_t(e[i]) << 23) : 0u);  // finite and not zero
       }
     }
 #pragma unroll
@@ -408,33 +505,41 @@ transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out 
       const int c = cj + j;
       const uint32_t top = max(max(colmax[0][c], colmax[1][c]), max(colmax[2][c], colmax[3][c]));
       constexpr int p = kType == kE4M3 ? 8 : 15;
-      // as block_exponent, of the shifted magnitude
-      const int ee = int(top >> 23) - 127 - p + 16 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-      en[j] = top == 0 ? 0 : top < 0x800000u || ee < -127 ? -127 : ee;
+      // as scale_byte, the exponent's field being 127 too large
+      const int byte = int(top >> 23) - 127 - p + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+      en[j] = top == 0 ? 127 : byte < 0 ? 0 : byte;
     }
     if (r8 == 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (col + j < cols) outT.scale[(col + j) * outT.lds + r0 / 128] = uint8_t(en[j] + 127);
+        if (col + j < cols) outT.scale[(col + j) * outT.lds + r0 / 128] = uint8_t(en[j]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float q[8];
+    for (int j = 0; j < 8; j += 4) {  // four columns at a time: the floats of 8 rows x 4
+      uint32_t o[4][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = __builtin_ldexpf(v[i][j], e[i] - 127 - en[j]);
-      u32x2 o;
-      o[0] = pack4<kType>(q[0], q[1], q[2], q[3]);
-      o[1] = pack4<kType>(q[4], q[5], q[6], q[7]);
-      *reinterpret_cast<u32x2*>(tile + slot(cj + j, r8)) = o;
+      for (int h = 0; h < 2; ++h) {
+        float v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2 lo = values2<kType, false>(w[4 * h + i][j >> 2]), hi = values2<kType, true>(w[4 * h + i][j >> 2]);
+          v[i][0] = __builtin_ldexpf(lo[0], e[4 * h + i] - en[j]);
+          v[i][1] = __builtin_ldexpf(lo[1], e[4 * h + i] - en[j + 1]);
+          v[i][2] = __builtin_ldexpf(hi[0], e[4 * h + i] - en[j + 2]);
+          v[i][3] = __builtin_ldexpf(hi[1], e[4 * h + i] - en[j + 3]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const s16x2 lo = convert2<kType, false>(s16x2{0, 0}, v[0][k], v[1][k], 1.f);
+          o[k][h] = __builtin_bit_cast(uint32_t, convert2<kType, true>(lo, v[2][k], v[3][k], 1.f));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x2*>(tile + slot(cj + j + k, r8)) = u32x2{o[k][0], o[k][1]};
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = i * 16 + (t >> 4), k8 = t & 15;
-    if (c0 + c < cols && r0 + k8 * 8 < rows)
-      store_q8(outT.q + (c0 + c) * outT.ld + r0 + k8 * 8, *reinterpret_cast<const u32x2*>(tile + slot(c, k8)));
-  }
+  tile_to_rows(tile, outT, rows, cols, r0, c0);
 }
 
 bool wide_vec(const void* x, int xtype, int64_t ldx, int64_t rows) {
