@@ -123,6 +123,28 @@ __device__ __forceinline__ uint32_t max8(const Eight<kX>& v) {
   return m;
 }
 
+// the columns' largest finite magnitudes over 8 rows, packed as the values are
+template <int kX>
+__device__ __forceinline__ void column_maxima(const Eight<kX> (&v)[8], uint32_t (&m)[Eight<kX>::kWords]) {
+  constexpr int kWords = Eight<kX>::kWords;
+  uint32_t all = 0;
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    m[j] = mag<kX>(v[0].w[j]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m[j] = max_mag<kX>(m[j], mag<kX>(v[i].w[j]));
+    all = max_mag<kX>(all, m[j]);
+  }
+  if (widest<kX>(all) >= kInf<kX>) {  // hardly ever
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      m[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[j] = max_mag<kX>(m[j], finite_mag<kX>(v[i].w[j]));
+    }
+  }
+}
+
 // largest of 16 lanes next to each other: three xors and a mirror inside the lanes' data path
 __device__ __forceinline__ uint32_t max16(uint32_t m) {
   m = max(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), 0xB1, 0xf, 0xf, true)));   // lane ^ 1
@@ -234,6 +256,26 @@ __device__ __forceinline__ void column_to_tile(const Eight<kX> (&v)[8], uint8_t*
   }
 }
 
+template <int kX, int kType>
+__device__ __forceinline__ void columns_to_tile(const Eight<kX> (&v)[8], uint8_t* tile, int cj, int r8,
+                                                const int (&bytes)[8]) {
+  if constexpr (kX == kF32) {
+    column_to_tile<kX, kType, 0>(v, tile, cj, r8, bytes[0], 0);
+    column_to_tile<kX, kType, 1>(v, tile, cj, r8, bytes[1], 0);
+    column_to_tile<kX, kType, 2>(v, tile, cj, r8, bytes[2], 0);
+    column_to_tile<kX, kType, 3>(v, tile, cj, r8, bytes[3], 0);
+    column_to_tile<kX, kType, 4>(v, tile, cj, r8, bytes[4], 0);
+    column_to_tile<kX, kType, 5>(v, tile, cj, r8, bytes[5], 0);
+    column_to_tile<kX, kType, 6>(v, tile, cj, r8, bytes[6], 0);
+    column_to_tile<kX, kType, 7>(v, tile, cj, r8, bytes[7], 0);
+  } else {
+    column_to_tile<kX, kType, 0>(v, tile, cj, r8, bytes[0], bytes[1]);
+    column_to_tile<kX, kType, 1>(v, tile, cj, r8, bytes[2], bytes[3]);
+    column_to_tile<kX, kType, 2>(v, tile, cj, r8, bytes[4], bytes[5]);
+    column_to_tile<kX, kType, 3>(v, tile, cj, r8, bytes[6], bytes[7]);
+  }
+}
+
 // 16 lanes write 128 bytes of one column of the tile in LDS
 __device__ __forceinline__ void tile_to_rows(const uint8_t* tile, Fp8Out outT, int64_t rows, int64_t cols, int64_t r0,
                                              int64_t c0) {
@@ -247,7 +289,7 @@ __device__ __forceinline__ void tile_to_rows(const uint8_t* tile, Fp8Out outT, i
 }
 
 template <int kX, int kType, bool kSquare, bool kVec>
-__global__ void __launch_bounds__(kQThreads, 4)
+__global__ void __launch_bounds__(kQThreads, kX == kF32 ? 2 : 4)
 quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, uint32_t tiles_n,
                      Fp8Out out, Fp8Out outT) {
   constexpr int kWords = Eight<kX>::kWords;
@@ -264,29 +306,12 @@ quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int6
   const int64_t first = (r0 + r8 * 8) * ldx + col;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = load8<kX, kVec>(x, first + i * ldx, i < nrow ? ncol : 0);
-  // the columns' largest, packed as they were read
   uint32_t m[kWords];
-#pragma unroll
-  for (int j = 0; j < kWords; ++j) m[j] = mag<kX>(v[0].w[j]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < kWords; ++j) m[j] = max_mag<kX>(m[j], mag<kX>(v[i].w[j]));
-  uint32_t all = m[0];
-#pragma unroll
-  for (int j = 1; j < kWords; ++j) all = max_mag<kX>(all, m[j]);
-  if (widest<kX>(all) >= kInf<kX>) {  // hardly ever
-#pragma unroll
-    for (int j = 0; j < kWords; ++j) {
-      m[j] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m[j] = max_mag<kX>(m[j], finite_mag<kX>(v[i].w[j]));
-    }
-  }
+  column_maxima<kX>(v, m);
   uint8_t* const q = out.q + (r0 + r8 * 8) * out.ld + col;
-  int bytes[2 * kWords > 8 ? 8 : 2 * kWords];  // of the 8 columns
+  int bytes[8];  // of the columns
   if constexpr (kSquare) {
-    all = m[0];
+    uint32_t all = m[0];
 #pragma unroll
     for (int j = 1; j < kWords; ++j) all = max_mag<kX>(all, m[j]);
     all = max16(widest<kX>(all));
@@ -346,21 +371,7 @@ quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int6
     }
   }
   if (!outT.q) return;
-  if constexpr (kX == kF32) {
-    column_to_tile<kX, kType, 0>(v, tile, cj, r8, bytes[0], 0);
-    column_to_tile<kX, kType, 1>(v, tile, cj, r8, bytes[1], 0);
-    column_to_tile<kX, kType, 2>(v, tile, cj, r8, bytes[2], 0);
-    column_to_tile<kX, kType, 3>(v, tile, cj, r8, bytes[3], 0);
-    column_to_tile<kX, kType, 4>(v, tile, cj, r8, bytes[4], 0);
-    column_to_tile<kX, kType, 5>(v, tile, cj, r8, bytes[5], 0);
-    column_to_tile<kX, kType, 6>(v, tile, cj, r8, bytes[6], 0);
-    column_to_tile<kX, kType, 7>(v, tile, cj, r8, bytes[7], 0);
-  } else {
-    column_to_tile<kX, kType, 0>(v, tile, cj, r8, bytes[0], bytes[1]);
-    column_to_tile<kX, kType, 1>(v, tile, cj, r8, bytes[2], bytes[3]);
-    column_to_tile<kX, kType, 2>(v, tile, cj, r8, bytes[4], bytes[5]);
-    column_to_tile<kX, kType, 3>(v, tile, cj, r8, bytes[6], bytes[7]);
-  }
+  columns_to_tile<kX, kType>(v, tile, cj, r8, bytes);
   __syncthreads();
   tile_to_rows(tile, outT, rows, cols, r0, c0);
 }
@@ -421,30 +432,33 @@ dequantize_kernel(Fp8In in, int cols, uint32_t units, FastDiv nb, int row_shift,
 }
 
 // ---- transpose: the layout of a tile is that of quantize_tile_kernel ----
-// rows: every column of 128 rows gets its own scale.  Its largest magnitude is found without rounding:
-// the bits of |q| as a 32-bit float plus the row's scale byte in the exponent's place order the products
-// as unsigned integers (the exponents sum to at most 142 + 254 < 512).  The new value is q 2^(e - e'),
-// rounded once: with powers of two on both sides it changes only where it leaves the type's normal range,
-// that is 2^-14 below its block's largest (e4m3).
+// square: bytes move, scales move.  rows: every column of 128 rows gets its own scale; the new value is
+// q 2^(e - e'), rounded once: with powers of two on both sides it changes only where it leaves the type's
+// normal range, that is 2^-14 below its block's largest (e4m3).
+// While the tile's scales are within 2^64 of each other (always, in practice), its values relative to the
+// largest scale are exact in bf16, and the columns go the way of quantize_tile_kernel's.  Otherwise the
+// columns' largest are found by the bits of |q| as a 32-bit float plus the row's scale byte in the
+// exponent's place, which order the products as unsigned integers (exponents sum to at most 142 + 254 <
+// 512), and q is shifted by the difference of the exponents.
 template <int kType, bool kHigh>
 __device__ __forceinline__ f32x2 values2(uint32_t w) {
   if constexpr (kType == kE4M3) return __builtin_amdgcn_cvt_pk_f32_fp8(int(w), kHigh);
   else return __builtin_amdgcn_cvt_pk_f32_bf8(int(w), kHigh);
 }
 template <int kType>
-__device__ __forceinline__ void values8(u32x2 w, float* v) {
+__device__ __forceinline__ uint32_t shifted4(const uint32_t (&w)[4], int byte, const int (&shift)[4]) {
+  float v[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x2 lo = values2<kType, false>(w[h]), hi = values2<kType, true>(w[h]);
-    v[4 * h] = lo[0];
-    v[4 * h + 1] = lo[1];
-    v[4 * h + 2] = hi[0];
-    v[4 * h + 3] = hi[1];
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t one = (w[i] >> (8 * byte)) & 255u;
+    v[i] = __builtin_ldexpf(values2<kType, false>(one)[0], shift[i]);
   }
+  const s16x2 lo = convert2<kType, false>(s16x2{0, 0}, v[0], v[1], 1.f);
+  return __builtin_bit_cast(uint32_t, convert2<kType, true>(lo, v[2], v[3], 1.f));
 }
 
 template <int kType, bool kSquare>
-__global__ void __launch_bounds__(kQThreads, 4)
+__global__ void __launch_bounds__(kQThreads, 3)
 transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out outT) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
   __shared__ uint32_t colmax[4][128];
@@ -462,80 +476,111 @@ transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out 
   if constexpr (kSquare) {
     if (t == 0) outT.scale[(c0 / 128) * outT.lds + r0 / 128] = in.scale[(r0 / 128) * in.lds + c0 / 128];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      u32x2 o{0, 0};
+    for (int h = 0; h < 2; ++h) {  // columns 4 h .. + 4
+      uint32_t o[4][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i >> 2] |= ((w[i][j >> 2] >> (8 * (j & 3))) & 255u) << (8 * (i & 3));
-      *reinterpret_cast<u32x2*>(tile + slot(cj + j, r8)) = o;
+      for (int g = 0; g < 2; ++g) {  // of rows 4 g .. + 4: 4 x 4 bytes
+        const uint32_t a = w[4 * g][h], b = w[4 * g + 1][h], c = w[4 * g + 2][h], d = w[4 * g + 3][h];
+        const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x05010400u), ab2 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+        const uint32_t cd = __builtin_amdgcn_perm(d, c, 0x05010400u), cd2 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+        o[0][g] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+        o[1][g] = __builtin_amdgcn_perm(cd, ab, 0x07060302u);
+        o[2][g] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u);
+        o[3][g] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x2*>(tile + slot(cj + 4 * h + k, r8)) = u32x2{o[k][0], o[k][1]};
     }
   } else {
+    const uint8_t* const scales = in.scale + r0 * in.lds + c0 / 128;
+    // the tile's largest and smallest scale: each wave looks at all 128 rows
+    const int last = int(rows - r0 < 128 ? rows - r0 : 128) - 1;
+    const int s0 = scales[(lane < last ? lane : last) * in.lds], s1 = scales[(lane + 64 < last ? lane + 64 : last) * in.lds];
+    int top = max(s0, s1), low = 255 - min(s0, s1);
+    uint32_t both = uint32_t(top) | (uint32_t(low) << 16);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) both = max2x16(both, uint32_t(__shfl_xor(int(both), d)));
+    top = int(both & 0xffffu);
+    low = 255 - int(both >> 16);
     int e[8];  // the rows' scale bytes
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < nrow ? in.scale[(r0 + r8 * 8 + i) * in.lds + c0 / 128] : 127;
-    constexpr uint32_t kNan = kType == kE4M3 ? 0x7f7f7f7fu : 0x7e7e7e7eu;
+    for (int i = 0; i < 8; ++i) e[i] = scales[(r8 * 8 + i < last ? r8 * 8 + i : last) * in.lds];
+    int bytes[8];  // the columns'
+    if (top - low <= 64 && top < 255) {
+      Eight<kBF16> v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (e[i] == 255) w[i] = u32x2{kNan, kNan};
-    uint32_t m[8];
+      for (int i = 0; i < 8; ++i) {
+        const float s = scale_of(e[i] - top + 127);
+        widen2<kBF16, kType, false>(w[i][0], s, v[i].w);
+        widen2<kBF16, kType, true>(w[i][0], s, v[i].w + 1);
+        widen2<kBF16, kType, false>(w[i][1], s, v[i].w + 2);
+        widen2<kBF16, kType, true>(w[i][1], s, v[i].w + 3);
+      }
+      uint32_t m[4];
+      column_maxima<kBF16>(v, m);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = 0;
+      for (int j = 0; j < 4; ++j) {
+        m[j] = max2x16(m[j], uint32_t(__shfl_xor(int(m[j]), 16)));
+        m[j] = max2x16(m[j], uint32_t(__shfl_xor(int(m[j]), 32)));
+      }
+      if (lane < 16) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v[8];
-      values8<kType>(w[i], v);
+        for (int j = 0; j < 4; ++j) colmax[wave][lane * 4 + j] = m[j];
+      }
+      __syncthreads();
+      // a column's byte is at least 0, relative to the largest scale at least 127 - top
+      const int least = 127 - top;
+      int rel[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = (t & 15) * 4 + j;
+        const uint32_t a = max2x16(max2x16(colmax[0][c], colmax[1][c]), max2x16(colmax[2][c], colmax[3][c]));
+        const uint32_t lo = a & 0xffffu, hi = a >> 16;
+        rel[2 * j] = max(scale_byte<kType>(lo << 16), least);
+        rel[2 * j + 1] = max(scale_byte<kType>(hi << 16), least);
+        bytes[2 * j] = lo == 0 ? 127 : rel[2 * j] - least;
+        bytes[2 * j + 1] = hi == 0 ? 127 : rel[2 * j + 1] - least;
+      }
+      columns_to_tile<kBF16, kType>(v, tile, cj, r8, rel);
+    } else {
+      constexpr uint32_t kNan = kType == kE4M3 ? 0x7f7f7f7fu : 0x7e7e7e7eu;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (e[i] == 255) w[i] = u32x2{kNan, kNan};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
-        m[j] = max(m[j], b - 1 < 0x7f7fffffu ? b + (uint32_t(e[i]) << 23) : 0u);  // finite and not zero
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t one = (w[i][j >> 2] >> (8 * (j & 3))) & 255u;
+          const uint32_t b = __float_as_uint(values2<kType, false>(one)[0]) & 0x7fffffffu;
+          m = max(m, b - 1 < 0x7f7fffffu ? b + (uint32_t(e[i]) << 23) : 0u);  // finite and not zero
+        }
+        m = max(m, uint32_t(__shfl_xor(int(m), 16)));
+        m = max(m, uint32_t(__shfl_xor(int(m), 32)));
+        if (lane < 16) colmax[wave][cj + j] = m;
       }
-    }
+      __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = max(m[j], uint32_t(__shfl_xor(int(m[j]), 16)));
-      m[j] = max(m[j], uint32_t(__shfl_xor(int(m[j]), 32)));
-    }
-    if (lane < 16) {
+      for (int j = 0; j < 8; ++j) {
+        const int c = cj + j;
+        const uint32_t m = max(max(colmax[0][c], colmax[1][c]), max(colmax[2][c], colmax[3][c]));
+        constexpr int p = kType == kE4M3 ? 8 : 15;
+        // as scale_byte, the exponent's field being 127 too large
+        const int byte = int(m >> 23) - 127 - p + ((m & 0x7fffffu) > 0x600000u ? 1 : 0);
+        bytes[j] = m == 0 ? 127 : byte < 0 ? 0 : byte;
+        u32x2 o;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) colmax[wave][cj + j] = m[j];
-    }
-    __syncthreads();
-    int en[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = cj + j;
-      const uint32_t top = max(max(colmax[0][c], colmax[1][c]), max(colmax[2][c], colmax[3][c]));
-      constexpr int p = kType == kE4M3 ? 8 : 15;
-      // as scale_byte, the exponent's field being 127 too large
-      const int byte = int(top >> 23) - 127 - p + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-      en[j] = top == 0 ? 127 : byte < 0 ? 0 : byte;
+        for (int g = 0; g < 2; ++g)
+          o[g] = shifted4<kType>({w[4 * g][j >> 2], w[4 * g + 1][j >> 2], w[4 * g + 2][j >> 2], w[4 * g + 3][j >> 2]}, j & 3,
+                                 {e[4 * g] - bytes[j], e[4 * g + 1] - bytes[j], e[4 * g + 2] - bytes[j], e[4 * g + 3] - bytes[j]});
+        *reinterpret_cast<u32x2*>(tile + slot(c, r8)) = o;
+      }
     }
     if (r8 == 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (col + j < cols) outT.scale[(col + j) * outT.lds + r0 / 128] = uint8_t(en[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {  // four columns at a time: the floats of 8 rows x 4
-      uint32_t o[4][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x2 lo = values2<kType, false>(w[4 * h + i][j >> 2]), hi = values2<kType, true>(w[4 * h + i][j >> 2]);
-          v[i][0] = __builtin_ldexpf(lo[0], e[4 * h + i] - en[j]);
-          v[i][1] = __builtin_ldexpf(lo[1], e[4 * h + i] - en[j + 1]);
-          v[i][2] = __builtin_ldexpf(hi[0], e[4 * h + i] - en[j + 2]);
-          v[i][3] = __builtin_ldexpf(hi[1], e[4 * h + i] - en[j + 3]);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const s16x2 lo = convert2<kType, false>(s16x2{0, 0}, v[0][k], v[1][k], 1.f);
-          o[k][h] = __builtin_bit_cast(uint32_t, convert2<kType, true>(lo, v[2][k], v[3][k], 1.f));
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x2*>(tile + slot(cj + j + k, r8)) = u32x2{o[k][0], o[k][1]};
+        if (col + j < cols) outT.scale[(col + j) * outT.lds + r0 / 128] = uint8_t(bytes[j]);
     }
   }
   __syncthreads();

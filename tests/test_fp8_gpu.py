@@ -150,14 +150,20 @@ def test_every_value_of_the_types_survives():
             assert torch.equal(dequantize_fp8(q, s, wide).float(), x)
 
 
-def test_extreme_scales_given_from_outside():
-    """Scales of 2^-127, 2^127 and NaN, which quantize_fp8 itself does not make."""
-    q = torch.tensor([[1.0, -0.5, 448.0, 2.0 ** -9] * 32], device="cuda").to(E4M3).repeat(4, 1)
-    s = torch.tensor([[0], [254], [255], [127]], dtype=torch.uint8, device="cuda")
+@pytest.mark.parametrize("scales", [(0, 254, 255, 127), (0, 254, 100, 127), (0, 10, 40, 64), (190, 254, 200, 210),
+                                    (60, 127, 90, 100), (63, 127, 64, 127), (255, 255, 255, 255), (0, 0, 0, 0)])
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+def test_extreme_scales_given_from_outside(scales, dtype):
+    """Scales next to 2^-127 and 2^127, NaN, near and far from each other, which quantize_fp8 itself does not make."""
+    rows = torch.tensor([[1.0, -0.5, 448.0, 2.0 ** -9, 0.0] * 25, [1.75, 3.0, 1.0, 0.0, 0.0] * 25,
+                         [0.0, 0.0, 2.0 ** -9, 0.0, 0.0] * 25, [0.0, 1.0, 0.0, -2.0 ** -9, 0.0] * 25], device="cuda")
+    q = torch.zeros(4, 128, device="cuda").to(dtype)
+    q[:, :125] = rows.to(dtype)
+    s = torch.tensor(scales, dtype=torch.uint8, device="cuda").reshape(4, 1)
     s = torch.nn.functional.pad(s, (0, 3)).view(E8M0)[:, :1]
     same(dequantize_fp8(q, s, F32), values(q, s).float())
     qt, st = transpose_fp8(q, s)
-    want, e = quantized(values(q, s).T.contiguous(), E4M3)
+    want, e = quantized(values(q, s).T.contiguous(), dtype)
     assert torch.equal(st.view(torch.uint8).int(), (e + 127).int())
     same(values(qt, st), want)
 
