@@ -166,7 +166,7 @@ __device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64
     const int col = row_b + c * 8;
     uint16_t* dst = C + int64_t(row_a + row) * ldc + col;
     if (vec_c && col + 8 <= N) {
-      __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(dst));
+      *reinterpret_cast<i32x4*>(dst) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)

@@ -9,7 +9,7 @@ import json
 import os
 import sys
 
-from . import WORKLOADS, make, run
+from . import DTYPES, WORKLOADS, make, run
 
 
 def main(argv=None) -> int:
@@ -20,6 +20,8 @@ def main(argv=None) -> int:
     ap.add_argument("--size", type=int, default=4096)
     ap.add_argument("--iters", type=int, default=2)
     ap.add_argument("--comm-mb", type=float, default=16.0)
+    ap.add_argument("--dtype", choices=DTYPES, default="bf16",
+                    help="of the compute: fp8 = 8 bits with block scales (trainers: forward and backward pass)")
     args = ap.parse_args(argv)
     import torch
     world = int(os.environ.get("WORLD_SIZE", "1"))
@@ -31,7 +33,7 @@ def main(argv=None) -> int:
         if world == 1 and "MASTER_ADDR" not in os.environ:
             os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT="29531", RANK="0", WORLD_SIZE="1")
         dist.init_process_group("nccl" if gpu else "gloo")
-    kw = {"size": args.size, "iters": args.iters}
+    kw = {"size": args.size, "iters": args.iters, "dtype": args.dtype}
     if args.workload != "gemm":
         kw["comm_bytes"] = int(args.comm_mb * (1 << 20))
     res = run(make(args.workload, **kw), args.steps, args.warmup)

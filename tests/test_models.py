@@ -49,3 +49,28 @@ def test_models_cli_single_process():
     assert r.returncode == 0, r.stderr
     out = json.loads(r.stdout.strip().splitlines()[-1])
     assert out["workload"] == "gemm" and out["steps"] == 2
+
+
+def test_fp8_pods_on_cpu():
+    """Without a GPU the fp8 pods run the same shapes in fp32: a product, and a layer's two passes."""
+    p = GemmPod(size=64, iters=1, device="cpu", dtype="fp8")
+    assert p.step().flops == 2 * 64 ** 3
+    torch.testing.assert_close(p.c, p.a @ p.b.T)
+    with pytest.raises(ValueError, match="dtype"):
+        make("gemm", size=64, device="cpu", dtype="fp4")
+
+
+@pytest.mark.parametrize("name", ["dp", "ep"])
+def test_fp8_trainer_pods_two_ranks(name):
+    kw = {"size": 32, "iters": 2, "comm_bytes": 1 << 14, "device": "cpu", "dtype": "fp8"}
+    for r in spawn(workload_worker, 2, "gloo", args=(name, 3, kw)):
+        assert r["workload"] == name and r["dtype"] == "fp8" and r["tflops"] > 0
+        assert r["comm_bytes"] and all(v > 0 for v in r["comm_bytes"].values())
+
+
+def test_models_cli_fp8():
+    r = subprocess.run([sys.executable, "-m", "kubernetes_gpu_exporter_amd.models", "gemm", "--steps", "2",
+                        "--warmup", "0", "--size", "64", "--iters", "1", "--dtype", "fp8"], cwd=ROOT,
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    assert json.loads(r.stdout.strip().splitlines()[-1])["dtype"] == "fp8"
