@@ -3,6 +3,7 @@
 
 Outputs (all inside kubernetes_gpu_exporter_amd/, so they travel with the repo):
   _gpuexp<EXT_SUFFIX>        pybind11 module: C++ telemetry core + HIP sentinel + MFMA GEMM
+  _gpuexp_fp8<EXT_SUFFIX>    8-bit operators on torch tensors (HIP kernels + torch bindings; where torch is)
   _gpuexp_aqlpmc.so          device PMC plugin: aqlprofile PM4 on an owned HSA queue (default)
   _gpuexp_rocprof.so         rocprofiler-sdk device-counting plugin (alternative counter backend)
   libgpuexp_rccl_tracer.so   rocprofiler-sdk RCCL API-tracing tool (ROCP_TOOL_LIBRARIES)
@@ -15,6 +16,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -44,8 +46,9 @@ HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SENTINEL_HIP = ["gpuexp/sentinel.hip"]
 SENTINEL_HSACO = "gpuexp/sentinel_hsaco.hip"  # device-only code object for raw AQL dispatch
 CALIB_HSACO = "kernels/calib_hsaco.hip"       # PMC calibration workloads, dispatched on the PMC queue
-KERNELS_HIP = ["kernels/gemm_bf16.hip", "kernels/fp8_quant.hip", "kernels/gemm_fp8.hip", "kernels/linear_fp8.hip",
-               "kernels/probe_kernels.hip", "kernels/kernels_bindings.hip"]
+KERNELS_HIP = ["kernels/gemm_bf16.hip", "kernels/probe_kernels.hip", "kernels/kernels_bindings.hip"]
+FP8_HIP = ["kernels/fp8_quant.hip", "kernels/gemm_fp8.hip", "kernels/linear_fp8.hip"]
+FP8_CC = ["kernels/fp8_torch.cc"]  # against torch's headers: built where torch is installed
 ROCPROF_CC = ["gpuexp/rocprof_plugin.cc"]
 AQLPMC_CC = ["gpuexp/aql_pmc.cc"]
 TRACER_CC = ["gpuexp/rccl_tracer.cc"]
@@ -83,6 +86,12 @@ def _common_flags(sanitize: str | None) -> list[str]:
     return flags
 
 
+def torch_dir() -> Path | None:
+    """Where torch is installed, found without importing it."""
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).parent if spec and spec.origin else None
+
+
 def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | None) -> Path:
     src = CSRC / src_rel
     obj = BUILD / (src_rel.replace("/", "__") + ".o")
@@ -95,7 +104,11 @@ def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | Non
             # Host-side sanitizer only: GPU ASan is not available on this pool.
             cmd += ["-Xarch_host", f"-fsanitize={sanitize}", "-fno-gpu-sanitize"]
     else:
-        cmd = ["g++"] + _common_flags(sanitize)
+        cmd = ["g++"]
+        if src_rel in FP8_CC:  # torch's headers (its pybind11 among them) before ours
+            inc = torch_dir() / "include"
+            cmd += [f"-I{inc}", f"-I{inc / 'torch' / 'csrc' / 'api' / 'include'}", "-DUSE_ROCM"]
+        cmd += _common_flags(sanitize)
     cmd += ["-c", str(src), "-o", str(obj)]
     _run(cmd)
     return obj
@@ -150,6 +163,9 @@ def build(force: bool = False, jobs: int = 8, sanitize: str | None = None, verbo
     hdr = _hdr_mtime()
     BUILD.mkdir(parents=True, exist_ok=True)
     srcs = CORE_CC + SENTINEL_HIP + KERNELS_HIP
+    torch_lib = torch_dir() / "lib" if torch_dir() else None
+    if torch_lib:
+        srcs = srcs + FP8_HIP + FP8_CC
     extra = [s for s in ROCPROF_CC + AQLPMC_CC + TRACER_CC if (CSRC / s).exists()]
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         futs = {s: ex.submit(compile_one, s, hdr, force, sanitize) for s in srcs + extra}
@@ -160,6 +176,10 @@ def build(force: bool = False, jobs: int = 8, sanitize: str | None = None, verbo
                                  ["-lamdhip64", "-lhsa-runtime64"])),
         "kernels": str(link_hip([objs[s] for s in KERNELS_HIP], _ext("_gpuexp_kernels"), ["-lamdhip64"])),
     }
+    if torch_lib:
+        outputs["fp8"] = str(link_hip([objs[s] for s in FP8_HIP + FP8_CC], _ext("_gpuexp_fp8"),
+                                      [f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+                                       "-lamdhip64"]))
     if (CSRC / ROCPROF_CC[0]).exists():
         outputs["rocprof_plugin"] = str(link_plain([objs[ROCPROF_CC[0]]], PKG / "_gpuexp_rocprof.so",
                                                    ["-lrocprofiler-sdk", "-lhsa-runtime64", "-lpthread"]))

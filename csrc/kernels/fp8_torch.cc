@@ -1,0 +1,333 @@
+// torch bindings of the 8-bit operators: checks of arguments, allocation, autograd.  In C++ because a
+// small call is bound by the host: the launches of a training step take 20 us, its Python took 100.
+// Tensors come in and go out as torch tensors, work goes to torch's current stream of their device.
+// The documentation is in ops/fp8.py.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <optional>
+#include <tuple>
+
+#include "fp8_launch.h"
+
+namespace {
+
+using at::Tensor;
+using gpuexp::Fp8In;
+using gpuexp::Fp8Out;
+using gpuexp::kFp8Block;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Pair = std::tuple<Tensor, Tensor>;
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+void check(hipError_t e, const char* what) { TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e)); }
+
+// the current device and torch's current stream for the launches of a call
+struct On {
+  explicit On(const Tensor& t)
+      : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+  c10::DeviceGuard guard;
+  hipStream_t stream;
+};
+
+int fp8_type(at::ScalarType t) {
+  return t == at::kFloat8_e4m3fn ? gpuexp::kE4M3 : t == at::kFloat8_e5m2 ? gpuexp::kE5M2 : -1;
+}
+int wide_type(at::ScalarType t) {
+  return t == at::kBFloat16 ? gpuexp::kBF16 : t == at::kHalf ? gpuexp::kF16 : t == at::kFloat ? gpuexp::kF32 : -1;
+}
+
+template <typename... T>
+void check_gpu(const char* name, const Tensor& first, const T&... rest) {
+  TORCH_CHECK_VALUE(first.device().is_cuda() && (... && (rest.device() == first.device())), name,
+                    ": tensors must be on the same GPU, got ", first.device(), ((" " + rest.device().str()) + ...));
+}
+void check_gpu(const char* name, const Tensor& t) {
+  TORCH_CHECK_VALUE(t.device().is_cuda(), name, ": tensors must be on the same GPU, got ", t.device());
+}
+
+// bytes between the rows of a 1-byte tensor [rows, cols] whose rows start at multiples of `pad`
+int64_t row_stride(const char* name, const char* of, const Tensor& t, int64_t rows, int64_t cols, int64_t pad) {
+  if (!rows || !cols) return up(cols, pad);
+  TORCH_CHECK_VALUE(cols == 1 || t.stride(1) == 1, of, name, " must have its columns next to each other, got strides ",
+                    t.strides());
+  const int64_t ld = rows == 1 ? up(cols, pad) : t.stride(0);
+  const int64_t off = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % pad;
+  TORCH_CHECK_VALUE(ld % pad == 0 && ld >= cols && off == 0, of, name, "'s rows must start at multiples of ", pad,
+                    " bytes and not overlap (row stride ", ld, ", address % ", pad, " = ", off,
+                    "); quantize_fp8 makes such tensors");
+  return ld;
+}
+
+Fp8In operand(const char* name, const Tensor& q, const Tensor& scale) {
+  const int type = fp8_type(q.scalar_type());
+  TORCH_CHECK_TYPE(type >= 0, name, " must be float8_e4m3fn or float8_e5m2, got ", q.scalar_type());
+  TORCH_CHECK_TYPE(scale.scalar_type() == at::kFloat8_e8m0fnu, "the scales of ", name, " must be float8_e8m0fnu, got ",
+                   scale.scalar_type());
+  TORCH_CHECK_VALUE(q.dim() == 2 && scale.dim() == 2, name, " and its scales must be 2-dimensional, got ", q.sizes(),
+                    " and ", scale.sizes());
+  const int64_t rows = q.size(0), cols = q.size(1), nb = blocks(cols);
+  const bool per_row = scale.size(0) == rows;
+  TORCH_CHECK_VALUE(scale.size(1) == nb && (per_row || scale.size(0) == blocks(rows)), "the scales of ", name, " ",
+                    q.sizes(), " must be [", rows, ", ", nb, "] (blocks of 1 x 128) or [", blocks(rows), ", ", nb,
+                    "] (128 x 128), got ", scale.sizes());
+  Fp8In in{nullptr, nullptr, row_stride(name, "", q, rows, cols, 16),
+           row_stride(name, "the scales of ", scale, scale.size(0), nb, 4), per_row ? 1 : kFp8Block, type};
+  if (rows && cols) {  // (an empty view may have any address)
+    in.q = static_cast<const uint8_t*>(q.const_data_ptr());
+    in.scale = static_cast<const uint8_t*>(scale.const_data_ptr());
+  }
+  return in;
+}
+
+// columns next to each other, rows that do not overlap
+bool row_major(const Tensor& x) {
+  const int64_t rows = x.size(0), cols = x.size(1);
+  return !x.numel() || ((cols == 1 || x.stride(1) == 1) && (rows == 1 || x.stride(0) >= cols));
+}
+int64_t wide_stride(const Tensor& x) { return x.size(0) > 1 && x.size(1) ? x.stride(0) : x.size(1); }
+
+Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType type) {
+  return at::empty(size, like.options().dtype(type));
+}
+
+// [rows, cols] of 1-byte values whose rows start at multiples of `pad` bytes
+Tensor empty_rows(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int64_t pad) {
+  const int64_t ld = up(cols, pad);
+  const Tensor t = empty({rows, ld}, like, type);
+  return ld == cols ? t : t.narrow(1, 0, cols);
+}
+
+struct Made {  // a tensor in 8 bits and where a kernel writes it
+  Tensor q, scale;
+  Fp8Out out{};
+  Made() = default;
+  Made(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int block_rows)
+      : q(empty_rows(rows, cols, like, type, 16)),
+        scale(empty_rows((rows + block_rows - 1) / block_rows, blocks(cols), like, at::kFloat8_e8m0fnu, 4)),
+        out{static_cast<uint8_t*>(q.mutable_data_ptr()), static_cast<uint8_t*>(scale.mutable_data_ptr()), up(cols, 16),
+            up(blocks(cols), 4)} {}
+};
+
+std::pair<Made, Made> quantize(const Tensor& x, at::ScalarType dtype, int64_t block_rows, bool columns) {
+  TORCH_CHECK_TYPE(fp8_type(dtype) >= 0, "quantize_fp8 makes float8_e4m3fn or float8_e5m2, not ", dtype);
+  TORCH_CHECK_VALUE(block_rows == 1 || block_rows == kFp8Block, "block_rows is 1 or 128, got ", block_rows);
+  TORCH_CHECK_TYPE(wide_type(x.scalar_type()) >= 0, "x must be bfloat16, float16 or float32, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() == 2, "x must be 2-dimensional, got ", x.sizes());
+  TORCH_CHECK_VALUE(row_major(x), "x must be row-major with its columns next to each other, got strides ", x.strides());
+  check_gpu("quantize_fp8", x);
+  const int64_t m = x.size(0), k = x.size(1);
+  const On on(x);
+  Made out, out_t;
+  out = Made(m, k, x, dtype, int(block_rows));
+  if (columns) out_t = Made(k, m, x, dtype, int(block_rows));
+  if (m && k)
+    check(gpuexp::launch_quantize_fp8(x.const_data_ptr(), wide_type(x.scalar_type()), wide_stride(x), m, k,
+                                      fp8_type(dtype), int(block_rows), out.out, out_t.out, on.stream),
+          "quantize_fp8");
+  return {std::move(out), std::move(out_t)};
+}
+
+Pair quantize_fp8(const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
+  auto [out, none] = quantize(x, dtype, block_rows, false);
+  return {std::move(out.q), std::move(out.scale)};
+}
+
+std::tuple<Pair, Pair> quantize_fp8_both(const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
+  auto [out, out_t] = quantize(x, dtype, block_rows, true);
+  return {Pair{std::move(out.q), std::move(out.scale)}, Pair{std::move(out_t.q), std::move(out_t.scale)}};
+}
+
+Tensor dequantize_fp8(const Tensor& q, const Tensor& scale, at::ScalarType dtype) {
+  const Fp8In in = operand("q", q, scale);
+  TORCH_CHECK_TYPE(wide_type(dtype) >= 0, "dequantize_fp8 gives bfloat16, float16 or float32, not ", dtype);
+  check_gpu("dequantize_fp8", q, scale);
+  const int64_t rows = q.size(0), cols = q.size(1);
+  const On on(q);
+  Tensor x = empty({rows, cols}, q, dtype);
+  if (rows && cols)
+    check(gpuexp::launch_dequantize_fp8(in, rows, cols, x.mutable_data_ptr(), wide_type(dtype), cols, on.stream),
+          "dequantize_fp8");
+  return x;
+}
+
+Pair transpose_fp8(const Tensor& q, const Tensor& scale) {
+  const Fp8In in = operand("q", q, scale);
+  check_gpu("transpose_fp8", q, scale);
+  const int64_t rows = q.size(0), cols = q.size(1);
+  const On on(q);
+  Made out(cols, rows, q, q.scalar_type(), in.block_rows);
+  if (rows && cols) check(gpuexp::launch_transpose_fp8(in, rows, cols, out.out, on.stream), "transpose_fp8");
+  return {std::move(out.q), std::move(out.scale)};
+}
+
+Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
+                const std::optional<Tensor>& given, at::ScalarType out_dtype, int64_t variant) {
+  const Fp8In oa = operand("a", a, a_scale), ob = operand("b", b, b_scale);
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
+  TORCH_CHECK_VALUE(b.size(1) == K, "shape mismatch ", a.sizes(), " x ", b.sizes(), "^T");
+  const at::ScalarType dtype = given ? given->scalar_type() : out_dtype;
+  TORCH_CHECK_TYPE(dtype == at::kBFloat16 || dtype == at::kHalf, "gemm_fp8 writes bfloat16 or float16, not ", dtype);
+  if (given)
+    TORCH_CHECK_VALUE(given->dim() == 2 && given->size(0) == M && given->size(1) == N && row_major(*given),
+                      "out must be [", M, ", ", N, "] with its columns next to each other, got ", given->sizes(),
+                      ", strides ", given->strides());
+  TORCH_CHECK_VALUE(gpuexp::resolve_gemm_fp8_variant(M, N, K, int(variant)) >= 0, "variant ", variant,
+                    " does not take these sizes (", M, ", ", N, ", ", K, ")");
+  check_gpu("gemm_fp8", a, a_scale, b, b_scale, given ? *given : a);
+  const On on(a);
+  Tensor out = given ? *given : empty({M, N}, a, dtype);
+  if (M && N)
+    check(gpuexp::launch_gemm_fp8({oa, ob, out.mutable_data_ptr(), wide_stride(out), M, N, K, wide_type(dtype), int(variant)},
+                                  on.stream),
+          "gemm_fp8");
+  return out;
+}
+
+Tensor rows_of(const Tensor& x) { return row_major(x) ? x : x.contiguous(); }
+Tensor bytes(int64_t n, const Tensor& like) { return empty({n}, like, at::kByte); }
+
+// y = x w^T of x [M, K], w [N, K] and the workspace that the backward pass needs
+std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& w, bool want_dx, bool want_dw) {
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  const On on(x);
+  const gpuexp::LinearFp8Bytes need = gpuexp::linear_fp8_bytes(M, N, K, want_dx, want_dw);
+  Tensor y = empty({M, N}, x, x.scalar_type()), kept = bytes(need.kept, x), temp = bytes(need.forward_temp, x);
+  gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, x.const_data_ptr(), wide_stride(x), w.const_data_ptr(),
+                          wide_stride(w), wide_type(x.scalar_type()), wide_type(w.scalar_type()),
+                          static_cast<uint8_t*>(kept.mutable_data_ptr()), static_cast<uint8_t*>(temp.mutable_data_ptr())};
+  check(gpuexp::launch_linear_fp8_forward(a, y.mutable_data_ptr(), on.stream), "linear_fp8");
+  return {y, kept};
+}
+
+variable_list once(const variable_list& grads, variable_list results) {
+  // gradients of gradients are refused where they are asked for, not where the first ones are made
+  if (!at::GradMode::is_enabled() || !grads[0].requires_grad()) return results;
+  auto error = std::make_shared<torch::autograd::DelayedError>("linear_fp8 cannot be differentiated twice",
+                                                               int(results.size()));
+  return (*error)(std::move(results));
+}
+
+struct LinearFp8 : torch::autograd::Function<LinearFp8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+    const bool want_dx = x.requires_grad(), want_dw = w.requires_grad();
+    auto [y, kept] = ::forward(x, w, want_dx, want_dw);
+    ctx->save_for_backward({kept});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), w.size(0), x.size(1), want_dx, want_dw,
+                                                    int64_t(w.scalar_type())};
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor kept = ctx->get_saved_variables()[0];
+    const std::vector<int64_t> s = ctx->saved_data["sizes"].toIntVector();
+    const int64_t M = s[0], N = s[1], K = s[2];
+    const bool want_dx = s[3], want_dw = s[4];
+    const auto wtype = at::ScalarType(s[5]);
+    variable_list results(2);
+    {
+      at::AutoGradMode off(false);
+      const Tensor dy = rows_of(grads[0]);
+      const On on(dy);
+      if (want_dx) results[0] = empty({M, K}, dy, dy.scalar_type());
+      if (want_dw) results[1] = empty({N, K}, dy, wtype);
+      const Tensor temp = bytes(gpuexp::linear_fp8_bytes(M, N, K, want_dx, want_dw).backward_temp, dy);
+      gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, nullptr, 0, nullptr, 0, wide_type(dy.scalar_type()),
+                              wide_type(wtype), static_cast<uint8_t*>(kept.mutable_data_ptr()),
+                              static_cast<uint8_t*>(temp.mutable_data_ptr())};
+      check(gpuexp::launch_linear_fp8_backward(a, dy.const_data_ptr(), wide_stride(dy),
+                                               want_dx ? results[0].mutable_data_ptr() : nullptr,
+                                               want_dw ? results[1].mutable_data_ptr() : nullptr, on.stream),
+            "linear_fp8's backward pass");
+    }
+    return once(grads, std::move(results));
+  }
+};
+
+Tensor serve(const Tensor& x, const Tensor& w, const Tensor& scale) {
+  const Fp8In in = operand("weight", w, scale);
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  const On on(x);
+  Tensor y = empty({M, N}, x, x.scalar_type());
+  const Tensor temp = bytes(gpuexp::serve_fp8_bytes(M, N, K), x);
+  check(gpuexp::launch_serve_fp8(x.const_data_ptr(), wide_type(x.scalar_type()), wide_stride(x), in, M, N, K,
+                                 y.mutable_data_ptr(), static_cast<uint8_t*>(temp.mutable_data_ptr()), on.stream),
+        "linear_fp8");
+  return y;
+}
+
+struct ServeFp8 : torch::autograd::Function<ServeFp8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& scale) {
+    ctx->save_for_backward({w, scale});
+    return serve(x, w, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list results(3);
+    {
+      at::AutoGradMode off(false);
+      const auto [g, g_scale] = quantize_fp8(rows_of(grads[0]), at::kFloat8_e4m3fn, 1);
+      const auto [wt, wt_scale] = transpose_fp8(saved[0], saved[1]);
+      results[0] = gemm_fp8(g, g_scale, wt, wt_scale, std::nullopt, grads[0].scalar_type(), 0);
+    }
+    return once(grads, std::move(results));
+  }
+};
+
+Tensor linear_fp8(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& scale) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1), "shape mismatch ", x.sizes(),
+                    " x ", weight.sizes(), "^T");
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+                   "linear_fp8 takes bfloat16 or float16 activations, got ", x.scalar_type());
+  if (scale) {
+    TORCH_CHECK_VALUE(!weight.requires_grad(), "weights in 8 bits take no gradient");
+    operand("weight", weight, *scale);
+    check_gpu("linear_fp8", x, weight, *scale);
+  } else {
+    TORCH_CHECK_TYPE(weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kHalf,
+                     "linear_fp8 takes bfloat16 or float16 weights, or 8-bit ones with weight_scale, got ",
+                     weight.scalar_type());
+    check_gpu("linear_fp8", x, weight);
+  }
+  const int64_t K = x.size(-1);
+  int64_t M = 1;
+  for (int64_t d = 0; d < x.dim() - 1; ++d) M *= x.size(d);
+  const Tensor x2 = rows_of(x.dim() == 2 ? x : x.reshape({M, K}));
+  const bool grad = at::GradMode::is_enabled();
+  Tensor y;
+  if (scale) {
+    y = grad && x2.requires_grad() ? ServeFp8::apply(x2, weight, *scale) : serve(x2, weight, *scale);
+  } else {
+    const Tensor w2 = rows_of(weight);
+    y = grad && (x2.requires_grad() || w2.requires_grad()) ? LinearFp8::apply(x2, w2)
+                                                           : forward(x2, w2, false, false).first;
+  }
+  if (x.dim() == 2) return y;
+  std::vector<int64_t> size(x.sizes().begin(), x.sizes().end());
+  size.back() = weight.size(0);
+  return y.reshape(size);
+}
+
+}  // namespace
+
+// Loaded after torch, whose HIP runtime it then shares (see ops/gemm.py).
+PYBIND11_MODULE(_gpuexp_fp8, m) {
+  m.doc() = "8-bit floating point with block scales on torch tensors (ops/fp8.py)";
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("quantize_fp8_both", &quantize_fp8_both);
+  m.def("dequantize_fp8", &dequantize_fp8);
+  m.def("transpose_fp8", &transpose_fp8);
+  m.def("gemm_fp8", &gemm_fp8);
+  m.def("linear_fp8", &linear_fp8);
+  m.def("gemm_fp8_variant", &gpuexp::resolve_gemm_fp8_variant, py::arg("M"), py::arg("N"), py::arg("K"),
+        py::arg("variant") = 0,
+        "The kernel variant a gemm_fp8 call with these sizes runs (0 = auto resolved), -1 if they do not fit it. "
+        "Host-only: no GPU needed.");
+}

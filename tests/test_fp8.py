@@ -2,8 +2,8 @@
 import pytest
 import torch
 
-from kubernetes_gpu_exporter_amd.ops.fp8 import dequantize_fp8, gemm_fp8, linear_fp8, quantize_fp8, transpose_fp8
-from kubernetes_gpu_exporter_amd.ops.gemm import kernels
+from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_variant, linear_fp8, quantize_fp8,
+                                                 quantize_fp8_both, transpose_fp8)
 from tests.fp8_oracle import E4M3, E5M2, E8M0, pair, quantized, values
 
 
@@ -34,8 +34,9 @@ def test_types_are_refused():
 
 @pytest.mark.parametrize("block_rows", [0, 2, 64, 256])
 def test_block_rows_are_refused(block_rows):
-    with pytest.raises(ValueError, match="block_rows"):
-        quantize_fp8(torch.zeros(4, 128), block_rows=block_rows)
+    for call in (quantize_fp8, quantize_fp8_both):
+        with pytest.raises(ValueError, match="block_rows"):
+            call(torch.zeros(4, 128), block_rows=block_rows)
 
 
 def test_shapes_are_refused():
@@ -86,40 +87,23 @@ def test_weights_in_8_bits_take_no_gradient():
 
 def test_cpu_tensors_are_refused():
     a, s = q(4, 256)
-    for call in (lambda: quantize_fp8(torch.zeros(4, 256)), lambda: dequantize_fp8(a, s),
+    for call in (lambda: quantize_fp8(torch.zeros(4, 256)), lambda: quantize_fp8_both(torch.zeros(4, 256)),
+                 lambda: quantize_fp8(torch.zeros(4, 256), stream=0), lambda: dequantize_fp8(a, s),
                  lambda: transpose_fp8(a, s), lambda: gemm_fp8(a, s, a, s),
                  lambda: linear_fp8(torch.zeros(4, 256).bfloat16(), torch.zeros(8, 256).bfloat16())):
         with pytest.raises(ValueError, match="same GPU"):
             call()
 
 
-def test_native_calls_check_addresses_and_strides(native):
-    """The native entry points turn what their vector accesses cannot take into errors, before any launch."""
-    k = kernels()
-    good = (1 << 20, 1 << 20, 128, 4, 1, 0)
-    for bad in ((1 << 20 | 8, 1 << 20, 128, 4, 1, 0), (1 << 20, 1 << 20 | 2, 128, 4, 1, 0),
-                (1 << 20, 1 << 20, 120, 4, 1, 0), (1 << 20, 1 << 20, 112, 4, 1, 0), (1 << 20, 1 << 20, 128, 0, 1, 0),
-                (1 << 20, 1 << 20, 128, 4, 2, 0), (1 << 20, 1 << 20, 128, 4, 1, 2), (0, 0, 128, 4, 1, 0)):
-        with pytest.raises(ValueError):
-            k.gemm_fp8(*bad, *good, 1 << 20, 128, 4, 4, 128, 0, 0, 0)
-        with pytest.raises(ValueError):
-            k.gemm_fp8(*good, *bad, 1 << 20, 128, 4, 4, 128, 0, 0, 0)
-        with pytest.raises(ValueError):
-            k.transpose_fp8(*bad, 4, 128, 1 << 20, 1 << 20, 16, 4, 0)
-        with pytest.raises(ValueError):
-            k.dequantize_fp8(*bad, 4, 128, 1 << 20, 0, 128, 0)
-    for c, ldc, ctype in ((0, 4, 0), (1 << 20, 3, 0), (1 << 20 | 1, 4, 0), (1 << 20, 4, 2)):
-        with pytest.raises(ValueError):
-            k.gemm_fp8(*good, *good, c, ldc, 4, 4, 128, ctype, 0, 0)
+def test_variants_are_refused():
+    a, s = q(4, 128)
     for variant in (-1, 2, 99):  # 2, the 256x256 tile, takes K >= 144
         with pytest.raises(ValueError, match="variant"):
-            k.gemm_fp8(*good, *good, 1 << 20, 4, 4, 4, 128, 0, variant, 0)
-    with pytest.raises(ValueError):
-        k.quantize_fp8(1 << 20, 0, 127, 4, 128, 0, 1, 1 << 20, 1 << 20, 128, 4, 0, 0, 0, 0, 0)
-    with pytest.raises(ValueError):
-        k.quantize_fp8(1 << 20, 0, 128, 4, 128, 0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    with pytest.raises(RuntimeError):  # a launch of 2^32 threads and more
-        k.quantize_fp8(1 << 20, 0, 1 << 20, 1 << 20, 1 << 20, 0, 1, 1 << 20, 1 << 20, 1 << 20, 1 << 13, 0, 0, 0, 0, 0)
+            gemm_fp8(a, s, a, s, variant=variant)
+    b, t = q(17, 256)
+    for variant in (3, 6):  # few rows: up to 16
+        with pytest.raises(ValueError, match="variant"):
+            gemm_fp8(b, t, b, t, variant=variant)
 
 
 @pytest.mark.parametrize("dtype", [E4M3, E5M2])
@@ -147,5 +131,5 @@ def test_oracle_values_of_a_hand_made_pair():
     (17, 64, 64, 3, -1), (17, 64, 64, 6, -1), (16, 64, 64, 6, 6), (1, 1, 0, 0, 3), (100, 100, 0, 0, 4),
     (64, 64, 64, 7, -1), (64, 64, 64, -1, -1),
 ])
-def test_gemm_variant_resolution(native, M, N, K, variant, want):
-    assert kernels().gemm_fp8_variant(M, N, K, variant) == want
+def test_gemm_variant_resolution(M, N, K, variant, want):
+    assert gemm_fp8_variant(M, N, K, variant) == want

@@ -11,8 +11,8 @@ have both signs, in norm they stay under 2^-13 (measured alone: 1.5e-5 < 2^-16).
 import pytest
 import torch
 
-from kubernetes_gpu_exporter_amd.ops.fp8 import dequantize_fp8, gemm_fp8, linear_fp8, quantize_fp8, transpose_fp8
-from kubernetes_gpu_exporter_amd.ops.gemm import kernels
+from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_variant, linear_fp8, quantize_fp8,
+                                                 quantize_fp8_both, transpose_fp8)
 from tests.fp8_oracle import E4M3, E5M2, E8M0, pair, quantized, small_whole, values
 
 pytestmark = pytest.mark.gpu
@@ -84,17 +84,14 @@ def test_transpose_requantises_along_the_other_axis(m, k, dtype, block_rows):
 @pytest.mark.parametrize("m,k", [(1, 1), (5, 200), (128, 128), (300, 129), (257, 640)])
 @pytest.mark.parametrize("xdtype", [BF16, F32])
 def test_both_orientations_in_one_pass(m, k, xdtype):
-    from kubernetes_gpu_exporter_amd.ops import fp8
     x = activations(m, k, gen(m * k), xdtype)
     for block_rows in (1, 128):
-        (q, s), (qt, st) = fp8._quantize(x, E4M3, block_rows, columns=True)
+        (q, s), (qt, st) = quantize_fp8_both(x, E4M3, block_rows)
         want, e = quantized(x, E4M3, block_rows)
         same(values(q, s), want)
         want_t = quantized(x.T.contiguous(), E4M3)[0] if block_rows == 1 else want.T
         same(values(qt, st), want_t)
-        none, (qt2, st2) = fp8._quantize(x, E4M3, block_rows, rows=False, columns=True)
-        assert none is None
-        same(values(qt2, st2), want_t)
+
 
 
 @pytest.mark.parametrize("dtype,xdtype", [(E4M3, F32), (E5M2, F32), (E4M3, BF16), (E4M3, F16)])
@@ -195,7 +192,7 @@ GEMMS = [(1, 1, 1), (1, 16, 128), (1, 1000, 640), (2, 129, 127), (5, 64, 16), (1
 @pytest.mark.parametrize("m,n,k", GEMMS)
 @pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_is_exact_on_whole_numbers(m, n, k, variant):
-    if kernels().gemm_fp8_variant(m, n, k, variant) < 0:
+    if gemm_fp8_variant(m, n, k, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
     g = gen(m + n + k)
     for ta, tb, block_a, block_b, out in ((E4M3, E4M3, 1, 128, BF16), (E5M2, E4M3, 1, 1, F16), (E4M3, E5M2, 128, 128, F16),
@@ -229,7 +226,7 @@ def test_gemm_on_random_operands(m, n, k, out):
 def test_gemm_repeats_bit_for_bit(m, variant):
     """Sums are joined in a fixed order: the same call gives the same bits (a tile read
     before it landed, or loaded over while read, would show here)."""
-    if kernels().gemm_fp8_variant(m, 768, 4096, variant) < 0:
+    if gemm_fp8_variant(m, 768, 4096, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
     g = gen(m)
     a, sa = quantize_fp8(torch.randn(m, 4096, device="cuda", generator=g))
@@ -242,7 +239,7 @@ def test_gemm_repeats_bit_for_bit(m, variant):
 @pytest.mark.parametrize("m,n", [(3, 5), (16, 257), (130, 70), (300, 300), (512, 256)])
 @pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_into_a_view_leaves_the_rest(m, n, variant):
-    if kernels().gemm_fp8_variant(m, n, 384, variant) < 0:
+    if gemm_fp8_variant(m, n, 384, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
     g = gen(n)
     a, sa = pair(m, 384, g, pad=32)
@@ -267,7 +264,7 @@ def test_gemm_of_empty_sizes(m, n, k):
 @pytest.mark.parametrize("m,n,k", [(1, 40, 300), (20, 40, 300), (200, 300, 300), (512, 512, 500)])
 @pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
 def test_gemm_nan_and_inf_stay_in_their_row(m, n, k, variant):
-    if kernels().gemm_fp8_variant(m, n, k, variant) < 0:
+    if gemm_fp8_variant(m, n, k, variant) < 0:
         pytest.skip("the kernel does not take these sizes")
     g = gen(9)
     a, sa = pair(m, k, g, E5M2)
