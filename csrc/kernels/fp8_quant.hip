@@ -44,13 +44,16 @@ struct Eight {
   uint32_t w[kWords];
 };
 
+// 16 bytes at any element's address: one instruction (rows of odd length), as the memory unit takes
+// unaligned accesses
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
 // From element i of x; those behind the first n read as 0 and are not touched in memory.
-// kVec: i is a multiple of 8 elements on a 16-byte boundary.
-template <int kX, bool kVec>
+template <int kX>
 __device__ __forceinline__ Eight<kX> load8(const void* x, int64_t i, int n) {
   Eight<kX> v;
-  if (kVec && n >= 8) {
-    const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const char*>(x) + i * (kX == kF32 ? 4 : 2));
+  if (n >= 8) {
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(static_cast<const char*>(x) + i * (kX == kF32 ? 4 : 2));
 #pragma unroll
     for (int j = 0; j < Eight<kX>::kWords; ++j) v.w[j] = p[j >> 2][j & 3];
     return v;
@@ -210,14 +213,14 @@ __device__ __forceinline__ uint32_t div(uint32_t u, FastDiv f) {
 }
 
 // ---- 1 x 128 blocks along the rows: 16 lanes hold a block, 8 values each ----
-template <int kX, int kType, bool kVec>
+template <int kX, int kType>
 __global__ void __launch_bounds__(kQThreads)
 quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int cols, uint32_t units, FastDiv nb, Fp8Out out) {
   const uint32_t u = blockIdx.x * (kQThreads / 16) + (threadIdx.x >> 4);
   if (u >= units) return;  // whole groups of 16 lanes
   const uint32_t row = div(u, nb), blk = u - row * nb.d;
   const int col = int(blk) * kFp8Block + (threadIdx.x & 15) * 8;
-  const Eight<kX> v = load8<kX, kVec>(x, int64_t(row) * ldx + col, cols - col);
+  const Eight<kX> v = load8<kX>(x, int64_t(row) * ldx + col, cols - col);
   const int byte = scale_byte<kType>(mag_bits<kX>(max16(max8<kX>(v))));
   if (col < cols) store_q8(out.q + int64_t(row) * out.ld + col, convert8<kX, kType>(v, scale_of(byte)));
   if ((threadIdx.x & 15) == 0) out.scale[int64_t(row) * out.lds + blk] = uint8_t(byte);
@@ -288,7 +291,7 @@ __device__ __forceinline__ void tile_to_rows(const uint8_t* tile, Fp8Out outT, i
   }
 }
 
-template <int kX, int kType, bool kSquare, bool kVec>
+template <int kX, int kType, bool kSquare>
 __global__ void __launch_bounds__(kQThreads, kX == kF32 ? 2 : 4)
 quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, uint32_t tiles_n,
                      Fp8Out out, Fp8Out outT) {
@@ -305,7 +308,7 @@ quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int6
   Eight<kX> v[8];
   const int64_t first = (r0 + r8 * 8) * ldx + col;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = load8<kX, kVec>(x, first + i * ldx, i < nrow ? ncol : 0);
+  for (int i = 0; i < 8; ++i) v[i] = load8<kX>(x, first + i * ldx, i < nrow ? ncol : 0);
   uint32_t m[kWords];
   column_maxima<kX>(v, m);
   uint8_t* const q = out.q + (r0 + r8 * 8) * out.ld + col;
@@ -399,7 +402,7 @@ __device__ __forceinline__ void widen2(uint32_t w, float scale, uint32_t* out) {
   }
 }
 
-template <int kX, int kType, bool kVec>
+template <int kX, int kType>
 __global__ void __launch_bounds__(kQThreads)
 dequantize_kernel(Fp8In in, int cols, uint32_t units, FastDiv nb, int row_shift, void* __restrict__ x, int64_t ldx) {
   const uint32_t u = blockIdx.x * (kQThreads / 16) + (threadIdx.x >> 4);
@@ -417,8 +420,8 @@ dequantize_kernel(Fp8In in, int cols, uint32_t units, FastDiv nb, int row_shift,
   widen2<kX, kType, true>(w[1], s, v.w + 3 * kTwo);
   const int64_t i = int64_t(row) * ldx + col;
   const int n = cols - col;
-  if (kVec && n >= 8) {
-    u32x4* p = reinterpret_cast<u32x4*>(static_cast<char*>(x) + i * (kX == kF32 ? 4 : 2));
+  if (n >= 8) {
+    u32x4_any* p = reinterpret_cast<u32x4_any*>(static_cast<char*>(x) + i * (kX == kF32 ? 4 : 2));
 #pragma unroll
     for (int j = 0; j < Eight<kX>::kWords / 4; ++j) p[j] = u32x4{v.w[4 * j], v.w[4 * j + 1], v.w[4 * j + 2], v.w[4 * j + 3]};
     return;
@@ -587,11 +590,6 @@ transpose_kernel(Fp8In in, int64_t rows, int64_t cols, uint32_t tiles_n, Fp8Out 
   tile_to_rows(tile, outT, rows, cols, r0, c0);
 }
 
-bool wide_vec(const void* x, int xtype, int64_t ldx, int64_t rows) {
-  const int64_t size = xtype == kF32 ? 4 : 2;
-  return reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows <= 1 || (ldx * size) % 16 == 0);
-}
-
 template <typename F>
 void by_types(int xtype, int type, F f) {
   auto t = [&](auto x) {
@@ -616,18 +614,16 @@ hipError_t launch_quantize_fp8(const void* x, int xtype, int64_t ldx, int64_t ro
   if (!count_ok(rows, cols)) return hipErrorInvalidValue;
   if (rows == 0 || cols == 0) return hipSuccess;
   const uint32_t nb = uint32_t((cols + 127) / 128);
-  const bool vec = wide_vec(x, xtype, ldx, rows);
   by_types(xtype, type, [&](auto kx, auto kt) {
     constexpr int X = decltype(kx)::value, T = decltype(kt)::value;
     if (block_rows == 1 && !outT.q) {
       const uint32_t units = uint32_t(rows) * nb;
-      auto k = vec ? quantize_rows_kernel<X, T, true> : quantize_rows_kernel<X, T, false>;
+      auto k = quantize_rows_kernel<X, T>;
       hipLaunchKernelGGL(k, dim3((units + 15) / 16), dim3(kQThreads), 0, stream, x, ldx, int(cols), units,
                          fast_div(nb), out);
     } else {
       const uint32_t tiles = uint32_t((rows + 127) / 128) * nb;
-      auto k = block_rows == 1 ? (vec ? quantize_tile_kernel<X, T, false, true> : quantize_tile_kernel<X, T, false, false>)
-                               : (vec ? quantize_tile_kernel<X, T, true, true> : quantize_tile_kernel<X, T, true, false>);
+      auto k = block_rows == 1 ? quantize_tile_kernel<X, T, false> : quantize_tile_kernel<X, T, true>;
       hipLaunchKernelGGL(k, dim3(tiles), dim3(kQThreads), 0, stream, x, ldx, rows, cols, nb, out, outT);
     }
   });
@@ -639,10 +635,9 @@ hipError_t launch_dequantize_fp8(Fp8In in, int64_t rows, int64_t cols, void* x, 
   if (!count_ok(rows, cols)) return hipErrorInvalidValue;
   if (rows == 0 || cols == 0) return hipSuccess;
   const uint32_t nb = uint32_t((cols + 127) / 128), units = uint32_t(rows) * nb;
-  const bool vec = wide_vec(x, xtype, ldx, rows);
   by_types(xtype, in.type, [&](auto kx, auto kt) {
     constexpr int X = decltype(kx)::value, T = decltype(kt)::value;
-    auto k = vec ? dequantize_kernel<X, T, true> : dequantize_kernel<X, T, false>;
+    auto k = dequantize_kernel<X, T>;
     hipLaunchKernelGGL(k, dim3((units + 15) / 16), dim3(kQThreads), 0, stream, in, int(cols), units, fast_div(nb),
                        in.block_rows == 1 ? 0 : 7, x, ldx);
   });

@@ -155,7 +155,7 @@ __device__ __forceinline__ void tile_to_lds(uint8_t* smem, int row0, int col0, i
 }
 template <int kBM, int kBN, int kThreads>
 __device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64_t ldc, int M, int N, int row_a,
-                                         int row_b, int vec_c) {
+                                         int row_b) {
   constexpr int kChunks = kBN / 8;
 #pragma unroll 4
   for (int p = 0; p < kBM * kChunks / kThreads; ++p) {
@@ -165,8 +165,9 @@ __device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64
     const i32x4 v = *reinterpret_cast<const i32x4*>(smem + row * kBN * 2 + ((c ^ (row & (kChunks - 1) & 31)) << 4));
     const int col = row_b + c * 8;
     uint16_t* dst = C + int64_t(row_a + row) * ldc + col;
-    if (vec_c && col + 8 <= N) {
-      *reinterpret_cast<i32x4*>(dst) = v;
+    if (col + 8 <= N) {
+      typedef i32x4 wide_t __attribute__((aligned(2)));  // (one store at any address)
+      *reinterpret_cast<wide_t*>(dst) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -186,7 +187,7 @@ __device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64
 // K tile, and the next quad's loaded then, which the count covers.
 template <int kA, int kB, typename TC, int kBM, int kBN, int kStages>
 __global__ void __launch_bounds__(256, 1)
-gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int vec_c) {
+gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K) {
   constexpr int kStage = (kBM + kBN) * kBK, kScales = kStages * kStage, kRows = kBM + kBN;
   constexpr int kMI = kBM / 64, kNI = kBN / 64, kLoads = kRows / 32;  // 32-row fragments and loads per wave
   static_assert((kStages == 2 || kStages == 4) && kBM * kBN * 2 <= kScales, "slots are t % 4's, and C fits");
@@ -336,7 +337,7 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
     for (int j = 0; j < kNI; ++j)
       tile_to_lds<kBN, TC>(smem, wm * (kBM / 2) + i * 32, wn * (kBN / 2) + j * 32, lane, acc[i][j]);
   __syncthreads();
-  lds_to_c<kBM, kBN, 256>(smem, C, ldc, A.rows, B.rows, row_a, row_b, vec_c);
+  lds_to_c<kBM, kBN, 256>(smem, C, ldc, A.rows, B.rows, row_a, row_b);
 }
 
 // ---- 256 x 256 tile, 8 waves, two barriers per phase ----
@@ -382,7 +383,7 @@ __device__ __forceinline__ void barrier_after_mfma() {
 
 template <int kA, int kB, typename TC>
 __global__ void __launch_bounds__(512, 1)
-gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int vec_c) {
+gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[kScales256 + 2 * 2048];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -558,7 +559,7 @@ gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
       for (int i = 0; i < 2; ++i)
         tile_to_lds<256, TC>(smem, wr * 128 + m * 64 + i * 32, wc * 64 + n * 32, lane, acc[m][n][i]);
   __syncthreads();
-  lds_to_c<256, 256, 512>(smem, C, ldc, A.rows, B.rows, row_a, row_b, vec_c);
+  lds_to_c<256, 256, 512>(smem, C, ldc, A.rows, B.rows, row_a, row_b);
 }
 
 // ---- up to 16 rows of A (tokens of a decoding step): B goes from memory straight to registers ----
@@ -573,7 +574,7 @@ constexpr int kQuad = 4 * kBK;
 
 template <int kA, int kB, int kR>
 __global__ void __launch_bounds__(1024)
-gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int c_is_f16, int vec_c) {
+gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int c_is_f16) {
   __shared__ f32x4 part[16 * kR * 64];  // [wave][kR][lane]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -652,9 +653,10 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = c_is_f16 ? to16<_Float16>(v[e]) : to16<__bf16>(v[e]);
     uint16_t* dst = C + int64_t(row) * ldc + col;
-    if (vec_c && col + 4 <= B.rows) {
+    if (col + 4 <= B.rows) {
       typedef __attribute__((ext_vector_type(4))) uint16_t u16x4;
-      *reinterpret_cast<u16x4*>(dst) = u16x4{h[0], h[1], h[2], h[3]};
+      typedef u16x4 wide_t __attribute__((aligned(2)));  // (one store at any address)
+      *reinterpret_cast<wide_t*>(dst) = u16x4{h[0], h[1], h[2], h[3]};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -733,10 +735,9 @@ void launch_rows(const GemmFp8Args& g, Operand oa, Operand ob, hipStream_t strea
   const int64_t quads = ((g.K & ~int64_t(15)) + kQuad - 1) / kQuad;
   int waves = 1;
   while (waves < 16 && waves < quads) waves *= 2;
-  const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 8 == 0 && g.ldc % 4 == 0;
   hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kR>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
                      dim3(waves * 64), 0, stream, oa, ob, static_cast<uint16_t*>(g.c), g.ldc, int(g.K),
-                     g.ctype == kF16, vec_c);
+                     g.ctype == kF16);
 }
 
 }  // namespace
@@ -749,7 +750,6 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
   const int64_t tiles = variant == 3 || variant == 6 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
   if (tiles >= (int64_t(1) << 22)) return hipErrorInvalidValue;  // 2^32 threads
-  const int vec_c = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc % 8 == 0;
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
     const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
@@ -759,12 +759,12 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
       else launch_rows<a, b, 2>(g, oa, ob, stream);
     } else if (variant == 2) {
       hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
-                         c, g.ldc, int(g.K), vec_c);
+                         c, g.ldc, int(g.K));
     } else {
       auto k = variant == 1   ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 4>
                : variant == 5 ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 2>
                               : gemm_fp8_tile_kernel<a, b, decltype(tc), 64, 64, 4>;
-      hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K), vec_c);
+      hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K));
     }
   });
   return hipGetLastError();
