@@ -58,15 +58,24 @@ __device__ __forceinline__ Eight<kX> load8(const void* x, int64_t i, int n) {
     for (int j = 0; j < Eight<kX>::kWords; ++j) v.w[j] = p[j >> 2][j & 3];
     return v;
   }
+  // a row's end: the loads go out together (behind the end the first value again)
+  uint32_t one[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) one[j] = 0;
+  if (n > 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t at = i + (j < n ? j : 0);
+      if constexpr (kX == kF32) one[j] = static_cast<const uint32_t*>(x)[at];
+      else one[j] = static_cast<const uint16_t*>(x)[at];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) one[j] = j < n ? one[j] : 0;
 #pragma unroll
   for (int j = 0; j < Eight<kX>::kWords; ++j) {
-    if constexpr (kX == kF32) {
-      v.w[j] = j < n ? static_cast<const uint32_t*>(x)[i + j] : 0;
-    } else {
-      const uint16_t* p = static_cast<const uint16_t*>(x) + i;
-      v.w[j] = 2 * j < n ? p[2 * j] : 0;
-      if (2 * j + 1 < n) v.w[j] |= uint32_t(p[2 * j + 1]) << 16;
-    }
+    if constexpr (kX == kF32) v.w[j] = one[j];
+    else v.w[j] = one[2 * j] | (one[2 * j + 1] << 16);
   }
   return v;
 }
