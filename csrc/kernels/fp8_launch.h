@@ -50,6 +50,10 @@ struct GemmFp8Args {
 // the kernel that a call runs (0 resolved), or -1 if the sizes do not fit it
 int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant);
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream);
+// the same for x[M][ldx] in bf16 or f16, quantised on its way (blocks of 1 x 128, e4m3), where it takes x
+bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K);
+hipError_t launch_gemm_fp8_wide(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K,
+                                void* y, hipStream_t stream);
 
 // y[M][N] = x[M][K] . w[N][K]^T in 8 bits and its backward pass, several launches behind one call.
 // Two workspaces in device memory: `kept` holds between the passes what the backward pass reads (x in
@@ -72,8 +76,8 @@ LinearFp8Bytes linear_fp8_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, b
 hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream);
 hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
                                       hipStream_t stream);
-// the same with a weight that is in 8 bits already; temp: x in 8 bits (serve_fp8_bytes)
-int64_t serve_fp8_bytes(int64_t M, int64_t N, int64_t K);
+// the same with a weight that is in 8 bits already; temp: x in 8 bits, where the product does not make it
+int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K);
 hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
                             uint8_t* temp, hipStream_t stream);
 

@@ -256,9 +256,12 @@ Tensor serve(const Tensor& x, const Tensor& w, const Tensor& scale) {
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const On on(x);
   Tensor y = empty({M, N}, x, x.scalar_type());
-  const Tensor temp = bytes(gpuexp::serve_fp8_bytes(M, N, K), x);
+  const int64_t need = gpuexp::serve_fp8_bytes(x.const_data_ptr(), wide_stride(x), M, N, K);
+  Tensor temp;
+  if (need) temp = bytes(need, x);
   check(gpuexp::launch_serve_fp8(x.const_data_ptr(), wide_type(x.scalar_type()), wide_stride(x), in, M, N, K,
-                                 y.mutable_data_ptr(), static_cast<uint8_t*>(temp.mutable_data_ptr()), on.stream),
+                                 y.mutable_data_ptr(), need ? static_cast<uint8_t*>(temp.mutable_data_ptr()) : nullptr,
+                                 on.stream),
         "linear_fp8");
   return y;
 }

@@ -16,10 +16,10 @@
 // past the end gets an offset past the buffer's end and reads zeros, so ragged sizes need no other
 // path; where K ends inside a 16-byte chunk, that chunk is a step of its own with its rest zeroed, so
 // what follows the last value in a row has no effect.
-#include "fp8_launch.h"
-
 #include <cmath>
 #include <type_traits>
+
+#include "fp8_device.h"
 
 namespace gpuexp {
 
@@ -143,7 +143,6 @@ __device__ __forceinline__ f32x16 mfma32(const i32x8& a, const i32x8& b, f32x16 
 // xored with the row so that the 32 rows fall into different banks.
 template <int kBN, typename TC>
 __device__ __forceinline__ void tile_to_lds(uint8_t* smem, int row0, int col0, int lane, const f32x16& v) {
-  typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
   const int row = row0 + (lane & 31);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -572,7 +571,32 @@ gemm_fp8_256_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc,
 // B is the matrix instruction's first operand: a lane then holds 4 columns of C next to each other.
 constexpr int kQuad = 4 * kBK;
 
-template <int kA, int kB, int kR>
+// 32 values of 16 bits in 8, with the scale byte of the block they share with the lanes 16, 32 and 48 on
+template <int kType, int kX>
+__device__ __forceinline__ void quantize32(const i32x4 (&w)[4], i32x8& out, int& byte) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max_mag<kX>(m, mag<kX>(uint32_t(w[i >> 2][i & 3])));
+  m = widest<kX>(m);
+  if (m >= kInf<kX>) {  // hardly ever
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max_mag<kX>(m, finite_mag<kX>(uint32_t(w[i >> 2][i & 3])));
+    m = widest<kX>(m);
+  }
+  m = max(m, uint32_t(__shfl_xor(int(m), 16)));
+  m = max(m, uint32_t(__shfl_xor(int(m), 32)));
+  byte = scale_byte<kType>(mag_bits<kX>(m));
+  const float scale = scale_of(byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    out[i] = int(convert4<kX, kType>(uint32_t(w[i >> 1][(i & 1) * 2]), uint32_t(w[i >> 1][(i & 1) * 2 + 1]), scale));
+}
+
+// kWide >= 0: A is [M][ld] values of 16 bits (WideType kWide, K a multiple of 16), quantised to kA on
+// their way as quantize_fp8 does: a lane has 32 values of a row's block, its three neighbours 16 lanes
+// apart the others.
+template <int kA, int kB, int kR, int kWide>
 __global__ void __launch_bounds__(1024)
 gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, int c_is_f16) {
   __shared__ f32x4 part[16 * kR * 64];  // [wave][kR][lane]
@@ -582,7 +606,7 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   const int K16 = K & ~15;
   const int nk = (K16 + kBK - 1) / kBK, quads = (nk + 3) / 4;
   const int q0 = quads * wave / waves, q1 = quads * (wave + 1) / waves;
-  const rsrc_t ra = tile_rsrc(A, 0, 16, K), rb = tile_rsrc(B, row_b, 16 * kR, K);
+  const rsrc_t ra = tile_rsrc(A, 0, 16, kWide < 0 ? K : 2 * K), rb = tile_rsrc(B, row_b, 16 * kR, K);
   const int l15 = lane & 15, chunk = (lane >> 4) * 16;  // this lane's chunks of a block: chunk, chunk + 64
 
   const uint32_t* psb[kR];
@@ -592,8 +616,9 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
     n = (n < B.rows ? n : B.rows - 1) >> B.shift;
     psb[r] = reinterpret_cast<const uint32_t*>(B.scale + int64_t(n) * B.lds);
   }
-  const int ma = (l15 < A.rows ? l15 : A.rows - 1) >> A.shift;
-  const uint32_t* psa = reinterpret_cast<const uint32_t*>(A.scale + int64_t(ma) * A.lds);
+  const uint32_t* psa = nullptr;
+  if constexpr (kWide < 0)
+    psa = reinterpret_cast<const uint32_t*>(A.scale + int64_t((l15 < A.rows ? l15 : A.rows - 1) >> A.shift) * A.lds);
   // one scale block (128 bytes of K) of 16 rows; past K16 zeros
   auto load = [&](rsrc_t rsrc, uint32_t at, int k) {
     const i32x4 lo = __builtin_bit_cast(
@@ -602,23 +627,45 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk + 64 < K16 - k ? at + 64 : kOob, k, 0));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  const uint32_t at_a = uint32_t(l15) * uint32_t(A.ld) + chunk, at_b = uint32_t(l15) * uint32_t(B.ld) + chunk;
+  const uint32_t at_a = uint32_t(l15) * uint32_t(A.ld) + (kWide < 0 ? chunk : 2 * chunk), at_b = uint32_t(l15) * uint32_t(B.ld) + chunk;
 
   f32x4 acc[kR];
 #pragma unroll
   for (int r = 0; r < kR; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int q = q0; q < q1; ++q) {
     i32x8 a[4], b[kR][4];
-    uint32_t sb[kR];
+    i32x4 wide[4][4];  // of a block, the values of chunk and of chunk + 64
+    uint32_t sb[kR], sa = 0;
+    if constexpr (kWide >= 0) {  // first: loads complete in order, and A is quantised while B comes
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = q * kQuad + i * kBK;
+          const bool in = (j < 2 ? chunk : chunk + 64) < K - k;
+          wide[i][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                     ra, in ? at_a + (j >> 1) * 128 + (j & 1) * 16 : kOob, 2 * k, 0));
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int r = 0; r < kR; ++r) b[r][i] = load(rb, at_b + r * 16 * uint32_t(B.ld), q * kQuad + i * kBK);
-      a[i] = load(ra, at_a, q * kQuad + i * kBK);
+      if constexpr (kWide < 0) a[i] = load(ra, at_a, q * kQuad + i * kBK);
     }
 #pragma unroll
     for (int r = 0; r < kR; ++r) sb[r] = psb[r][q];
-    uint32_t sa = psa[q];
+    if constexpr (kWide < 0) {
+      sa = psa[q];
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int byte;
+        quantize32<kA, kWide>(wide[i], a[i], byte);
+        sa |= uint32_t(byte) << (8 * i);
+      }
+    }
     // behind K the scales are whatever pads their rows, and the values are zeros: 2^0 will do
     const int blocks = nk - q * 4;
     const uint32_t pad = blocks >= 4 ? 0u : 0xffffffffu << (8 * blocks);
@@ -632,7 +679,7 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
       acc[r] = mfma<kB, kA, 3>(b[r][3], a[3], acc[r], int(sb[r]), int(sa));
     }
   }
-  if (K != K16 && wave == waves - 1) {
+  if (kWide < 0 && K != K16 && wave == waves - 1) {
     const i32x8 a = tail_frag(ra, A.ld, l15, lane < 16, K);
     const int s = tail_scale(A, l15, K);
 #pragma unroll
@@ -730,12 +777,12 @@ int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
 
 namespace {
 
-template <int a, int b, int kR>
+template <int a, int b, int kR, int kWide = -1>
 void launch_rows(const GemmFp8Args& g, Operand oa, Operand ob, hipStream_t stream) {
   const int64_t quads = ((g.K & ~int64_t(15)) + kQuad - 1) / kQuad;
   int waves = 1;
   while (waves < 16 && waves < quads) waves *= 2;
-  hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kR>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
+  hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kR, kWide>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
                      dim3(waves * 64), 0, stream, oa, ob, static_cast<uint16_t*>(g.c), g.ldc, int(g.K),
                      g.ctype == kF16);
 }
@@ -767,6 +814,39 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
       hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K));
     }
   });
+  return hipGetLastError();
+}
+
+// Every block quantises the rows of x that it needs, which up to 2^24 weights costs less than a launch of
+// its own (one and 16 tokens, us, this way / two launches: 512 x 512 2.8 / 4.1 and 3.0 / 4.8, 4096 x 4096
+// 7.5 / 8.4 and 9.4 / 9.8) and beyond more (8192 x 8192 20.4 / 17.4 and 28.4 / 19.7).  The vector loads
+// of x want its rows at multiples of 16 bytes and no row to end inside 16 values.
+bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
+  return M >= 1 && M <= 16 && K >= 1 && K % 16 == 0 && K <= 8192 && N * K <= (int64_t(1) << 24) &&
+         reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || (ldx % 8 == 0 && ldx <= (int64_t(1) << 21)));
+}
+
+hipError_t launch_gemm_fp8_wide(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K,
+                                void* y, hipStream_t stream) {
+  if (!gemm_fp8_takes_wide(x, ldx, M, N, K) || !side_ok(w, N, K) || (N + 15) / 16 >= (int64_t(1) << 22))
+    return hipErrorInvalidValue;
+  if (N == 0) return hipSuccess;
+  GemmFp8Args g{};
+  g.c = y;
+  g.ldc = N;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.ctype = type;
+  const Operand oa{static_cast<const uint8_t*>(x), nullptr, 2 * (M == 1 ? K : ldx), 0, int(M), 0};
+  const Operand ob = operand(w, N);
+  auto by_b = [&](auto tb) {
+    constexpr int b = decltype(tb)::value;
+    if (type == kBF16) launch_rows<kE4M3, b, 1, kBF16>(g, oa, ob, stream);
+    else launch_rows<kE4M3, b, 1, kF16>(g, oa, ob, stream);
+  };
+  if (w.type == kE4M3) by_b(std::integral_constant<int, kE4M3>{});
+  else by_b(std::integral_constant<int, kE5M2>{});
   return hipGetLastError();
 }
 

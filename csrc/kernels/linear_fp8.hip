@@ -84,10 +84,13 @@ hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, in
   return hipSuccess;
 }
 
-int64_t serve_fp8_bytes(int64_t M, int64_t N, int64_t K) { return Piece{M, K, 0, 1}.end(); }
+int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
+  return gemm_fp8_takes_wide(x, ldx, M, N, K) ? 0 : Piece{M, K, 0, 1}.end();
+}
 
 hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
                             uint8_t* temp, hipStream_t stream) {
+  if (gemm_fp8_takes_wide(x, ldx, M, N, K)) return launch_gemm_fp8_wide(x, type, ldx, w, M, N, K, y, stream);
   const Piece xq{M, K, 0, 1};
   GPUEXP_RETURN_IF(launch_quantize_fp8(x, type, ldx, M, K, kE4M3, 1, xq.out(temp), {}, stream));
   return gemm(xq.in(temp), w, M, N, K, y, type, stream);

@@ -435,6 +435,22 @@ def test_linear_with_weights_in_8_bits(m, n, k, dtype):
     assert float((gx.double() - want).norm()) <= (half + 2.0 ** -13) * float(want.norm()) + tiny * want.numel() ** 0.5
 
 
+@pytest.mark.parametrize("m", [1, 2, 7, 16, 17])
+@pytest.mark.parametrize("n,k", [(64, 64), (300, 1024), (1000, 4096), (33, 8192), (5000, 48), (256, 1000), (4096, 4608)])
+def test_serving_quantises_as_quantize_fp8_does(m, n, k):
+    """A few tokens' activations may be quantised inside the product: the same bits as in two calls, for rows at any
+    address and distance."""
+    g = gen(m * n)
+    wq, ws = quantize_fp8(torch.randn(n, k, device="cuda", generator=g) * 0.1, block_rows=128)
+    base = torch.randn(m * (k + 24) + 8, device="cuda", generator=g)
+    base = base * torch.exp(3 * torch.randn(base.shape, device="cuda", generator=g))
+    for dtype in (BF16, F16):
+        for offset, ld in ((0, k), (8, k + 8), (0, k + 24), (1, k), (0, k + 3)):
+            x = base.clamp(-60000, 60000).to(dtype)[offset:offset + m * ld].view(m, ld)[:, :k]
+            got = linear_fp8(x, wq, ws)
+            assert torch.equal(got, gemm_fp8(*quantize_fp8(x), wq, ws, out_dtype=dtype)), (dtype, offset, ld)
+
+
 def test_linear_nan_tokens_stay_in_their_rows():
     g = gen(8)
     for m in (3, 40, 300):
