@@ -25,7 +25,11 @@ from __future__ import annotations
 
 import torch  # (first: the native module shares torch's HIP runtime)
 
-from .. import _gpuexp_fp8 as _native
+try:
+    from .. import _gpuexp_fp8 as _native
+except ImportError as e:
+    raise ImportError(f"native module _gpuexp_fp8 is not built; run `python build_native.py` where torch is "
+                      f"installed: {e}") from e
 
 
 def _elsewhere(stream, *tensors):
