@@ -207,9 +207,13 @@ std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& w, bool want_dx
   return {y, kept};
 }
 
-variable_list once(const variable_list& grads, variable_list results) {
-  // gradients of gradients are refused where they are asked for, not where the first ones are made
-  if (!at::GradMode::is_enabled() || !grads[0].requires_grad()) return results;
+variable_list once(variable_list results) {
+  // Gradients of gradients are refused where they are asked for, not where the first ones are made; also for a
+  // constant dy, since dx depends on the weight and dw on x.
+  if (!at::GradMode::is_enabled()) return results;
+  for (Tensor& t : results) {  // DelayedError hangs its refusal only on tensors that take a gradient
+    if (t.defined()) t.set_requires_grad(true);
+  }
   auto error = std::make_shared<torch::autograd::DelayedError>("linear_fp8 cannot be differentiated twice",
                                                                int(results.size()));
   return (*error)(std::move(results));
@@ -247,7 +251,7 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
                                                want_dw ? results[1].mutable_data_ptr() : nullptr, on.stream),
             "linear_fp8's backward pass");
     }
-    return once(grads, std::move(results));
+    return once(std::move(results));
   }
 };
 
@@ -280,7 +284,7 @@ struct ServeFp8 : torch::autograd::Function<ServeFp8> {
       const auto [wt, wt_scale] = transpose_fp8(saved[0], saved[1]);
       results[0] = gemm_fp8(g, g_scale, wt, wt_scale, std::nullopt, grads[0].scalar_type(), 0);
     }
-    return once(grads, std::move(results));
+    return once(std::move(results));
   }
 };
 

@@ -409,8 +409,18 @@ def test_linear_keeps_8_bits_for_the_backward_pass():
 def test_linear_double_backward_is_refused():
     x = torch.randn(8, 64, device="cuda", dtype=BF16).requires_grad_()
     w = torch.randn(8, 64, device="cuda", dtype=BF16).requires_grad_()
-    (gx,) = torch.autograd.grad(linear_fp8(x, w).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
+    (gx,) = torch.autograd.grad(linear_fp8(x, w).sum(), x, create_graph=True)  # a constant dy: dx depends on w alone
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        gx.sum().backward()
+    s = torch.ones((), device="cuda", dtype=BF16, requires_grad=True)
+    for leaves in ((x, w), (x,), (w,)):
+        y = linear_fp8(*(t if any(t is u for u in leaves) else t.detach() for t in (x, w)))
+        grads = torch.autograd.grad((y * s).sum(), leaves, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated twice"):
+            sum(t.sum() for t in grads).backward()
+    wq, ws = quantize_fp8(w.detach(), block_rows=128)
+    (gx,) = torch.autograd.grad((linear_fp8(x, wq, ws) * s).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated twice"):
         gx.sum().backward()
 
 
