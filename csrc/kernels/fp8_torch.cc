@@ -184,6 +184,7 @@ Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
   check_gpu("gemm_fp8", a, a_scale, b, b_scale, given ? *given : a);
   const On on(a);
   Tensor out = given ? *given : empty({M, N}, a, dtype);
+  if (given) out.unsafeGetTensorImpl()->bump_version();  // an in-place change, to whoever saved `out`
   if (M && N)
     check(gpuexp::launch_gemm_fp8({oa, ob, out.mutable_data_ptr(), wide_stride(out), M, N, K, wide_type(dtype), int(variant)},
                                   on.stream),

@@ -390,6 +390,61 @@ def test_linear_of_one_gradient_only_and_broadcast_gradients():
         assert tuple(ye.shape) == (*shape[:-1], 128) and ge.shape == xe.shape and not bool(gw.any())
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (17, 300, 130), (257, 384, 1000), (1030, 640, 512)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_is_the_operators_in_turn(m, n, k, dtype):
+    """A layer's passes, the operators one after the other as a program would call them, and the two orientations in
+    one pass: the same bits."""
+    g = gen(m + k)
+    x = torch.randn(m, k, device="cuda", generator=g).to(dtype).requires_grad_()
+    w = (torch.randn(n, k, device="cuda", generator=g) * 0.05).to(dtype).requires_grad_()
+    grad = torch.randn(m, n, device="cuda", generator=g).to(dtype)
+    y = linear_fp8(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), grad)
+    kept, weight, dy, dy_t = (quantize_fp8(x.detach()), quantize_fp8(w.detach(), block_rows=128), quantize_fp8(grad),
+                              quantize_fp8(grad.T.contiguous()))
+    assert torch.equal(y, gemm_fp8(*kept, *weight, out_dtype=dtype))
+    assert torch.equal(dx, gemm_fp8(*dy, *transpose_fp8(*weight), out_dtype=dtype))
+    assert torch.equal(dw, gemm_fp8(*dy_t, *transpose_fp8(*kept), out_dtype=dtype))
+    both, both_w = quantize_fp8_both(grad), quantize_fp8_both(w.detach(), block_rows=128)
+    assert torch.equal(dx, gemm_fp8(*both[0], *both_w[1], out_dtype=dtype))
+    assert torch.equal(dw, gemm_fp8(*both[1], *transpose_fp8(*kept), out_dtype=dtype))
+
+
+def test_activations_kept_in_8_bits_between_the_passes():
+    """quantize_fp8 / dequantize_fp8 as torch's hooks on saved tensors: what an activation function keeps goes to 8
+    bits, its gradient is taken where the checkpoint says the input was; around layers in 8 bits."""
+    g = gen(21)
+    x = torch.randn(200, 384, device="cuda", generator=g).to(BF16).requires_grad_()
+    w1, w2 = ((torch.randn(r, c, device="cuda", generator=g) * 0.05).to(BF16).requires_grad_() for r, c in ((512, 384), (256, 512)))
+    grad = torch.randn(200, 256, device="cuda", generator=g).to(BF16)
+    h = linear_fp8(x, w1)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: quantize_fp8(t.detach()), lambda p: dequantize_fp8(*p)):
+        act = torch.nn.functional.silu(h)
+    y = linear_fp8(act, w2)
+    got = torch.autograd.grad(y, (x, w1, w2), grad)
+    # the same by hand
+    ha = h.detach()
+    a = torch.nn.functional.silu(ha).requires_grad_()
+    da, dw2 = torch.autograd.grad(linear_fp8(a, w2), (a, w2), grad)
+    back = dequantize_fp8(*quantize_fp8(ha)).requires_grad_()
+    (dh,) = torch.autograd.grad(torch.nn.functional.silu(back), back, da)
+    dx, dw1 = torch.autograd.grad(linear_fp8(x, w1), (x, w1), dh)
+    for a_, b_ in zip(got, (dx, dw1, dw2)):
+        assert torch.equal(a_, b_)
+
+
+def test_out_counts_as_changed():
+    """A tensor that autograd saved and gemm_fp8 then wrote into is reported, as after any in-place change."""
+    a, sa = quantize_fp8(torch.randn(8, 128, device="cuda"))
+    out = torch.ones(8, 8, device="cuda", dtype=BF16)
+    p = torch.ones(8, 8, device="cuda", dtype=BF16, requires_grad=True)
+    z = (p * out).sum()
+    gemm_fp8(a, sa, a, sa, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
 def test_linear_keeps_8_bits_for_the_backward_pass():
     """Between the passes the layer holds its input in 8 bits (and the 8-bit weight), no 16-bit copy."""
     x = torch.randn(4096, 2048, device="cuda", dtype=BF16).requires_grad_()
