@@ -27,7 +27,11 @@ using Pair = std::tuple<Tensor, Tensor>;
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
-void check(hipError_t e, const char* what) { TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e)); }
+void check(hipError_t e, const char* what) {
+  TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": larger than the kernels index (fewer than 2^31 rows, rows of at "
+                    "most 4 MiB in 8 bits, fewer than 2^35 values to quantise)");
+  TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+}
 
 // the current device and torch's current stream for the launches of a call
 struct On {

@@ -796,7 +796,8 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   if (variant < 0) return hipErrorInvalidValue;
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
   const int64_t tiles = variant == 3 || variant == 6 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
-  if (tiles >= (int64_t(1) << 22)) return hipErrorInvalidValue;  // 2^32 threads
+  const int64_t threads = variant == 3 || variant == 6 ? 1024 : variant == 2 ? 512 : 256;
+  if (tiles * threads >= (int64_t(1) << 32)) return hipErrorInvalidValue;
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
     const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
