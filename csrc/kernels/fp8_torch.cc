@@ -27,9 +27,12 @@ using Pair = std::tuple<Tensor, Tensor>;
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
+// the longest row of a product's operand: a tile of 256 of them has to fit in a buffer's 31 bits
+constexpr int64_t kLongest = int64_t(1) << 22;
+
 void check(hipError_t e, const char* what) {
-  TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": larger than the kernels index (fewer than 2^31 rows, rows of at "
-                    "most 4 MiB in 8 bits, fewer than 2^35 values to quantise)");
+  TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": larger than the kernels index (fewer than 2^31 rows, rows at most "
+                    "4 MiB apart in 8 bits, fewer than 2^35 values to quantise)");
   TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
 }
 
@@ -95,6 +98,15 @@ Fp8In operand(const char* name, const Tensor& q, const Tensor& scale) {
 bool row_major(const Tensor& x) {
   const int64_t rows = x.size(0), cols = x.size(1);
   return !x.numel() || ((cols == 1 || x.stride(1) == 1) && (rows == 1 || x.stride(0) >= cols));
+}
+// whether the memory from the first to the last value of each meets
+bool overlap(const Tensor& x, const Tensor& y) {
+  if (!x.numel() || !y.numel()) return false;
+  const auto begin = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
+  const auto end = [&](const Tensor& t) {
+    return begin(t) + ((t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1) + 1) * t.element_size();
+  };
+  return begin(x) < end(y) && begin(y) < end(x);
 }
 int64_t wide_stride(const Tensor& x) { return x.size(0) > 1 && x.size(1) ? x.stride(0) : x.size(1); }
 
@@ -186,9 +198,16 @@ Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
   TORCH_CHECK_VALUE(gpuexp::resolve_gemm_fp8_variant(M, N, K, int(variant)) >= 0, "variant ", variant,
                     " does not take these sizes (", M, ", ", N, ", ", K, ")");
   check_gpu("gemm_fp8", a, a_scale, b, b_scale, given ? *given : a);
+  TORCH_CHECK_VALUE(K <= kLongest, "gemm_fp8: rows of at most ", kLongest, " values, got ", K);
   const On on(a);
   Tensor out = given ? *given : empty({M, N}, a, dtype);
-  if (given) out.unsafeGetTensorImpl()->bump_version();  // an in-place change, to whoever saved `out`
+  if (given) {
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && given->requires_grad()), "out takes a gradient, which gemm_fp8 "
+                      "has none to give");
+    for (const Tensor* t : {&a, &a_scale, &b, &b_scale})
+      TORCH_CHECK_VALUE(!overlap(*given, *t), "out must not overlap an input");
+    out.unsafeGetTensorImpl()->bump_version();  // an in-place change, to whoever saved `out`
+  }
   if (M && N)
     check(gpuexp::launch_gemm_fp8({oa, ob, out.mutable_data_ptr(), wide_stride(out), M, N, K, wide_type(dtype), int(variant)},
                                   on.stream),
@@ -312,14 +331,17 @@ Tensor linear_fp8(const Tensor& x, const Tensor& weight, const std::optional<Ten
   int64_t M = 1;
   for (int64_t d = 0; d < x.dim() - 1; ++d) M *= x.size(d);
   const Tensor x2 = rows_of(x.dim() == 2 ? x : x.reshape({M, K}));
-  const bool grad = at::GradMode::is_enabled();
+  const bool grad = at::GradMode::is_enabled(), want_dx = grad && x2.requires_grad(),
+             want_dw = grad && weight.requires_grad();
+  TORCH_CHECK_VALUE(K <= kLongest && (!want_dx || weight.size(0) <= kLongest) && (!want_dw || M <= kLongest),
+                    "linear_fp8: at most ", kLongest, " inputs, for x's gradient as many outputs and for the weight's as "
+                    "many rows of x, got ", K, ", ", weight.size(0), " and ", M);
   Tensor y;
   if (scale) {
-    y = grad && x2.requires_grad() ? ServeFp8::apply(x2, weight, *scale) : serve(x2, weight, *scale);
+    y = want_dx ? ServeFp8::apply(x2, weight, *scale) : serve(x2, weight, *scale);
   } else {
     const Tensor w2 = rows_of(weight);
-    y = grad && (x2.requires_grad() || w2.requires_grad()) ? LinearFp8::apply(x2, w2)
-                                                           : forward(x2, w2, false, false).first;
+    y = want_dx || want_dw ? LinearFp8::apply(x2, w2) : forward(x2, w2, false, false).first;
   }
   if (x.dim() == 2) return y;
   std::vector<int64_t> size(x.sizes().begin(), x.sizes().end());

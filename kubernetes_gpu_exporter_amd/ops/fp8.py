@@ -15,6 +15,8 @@ at multiples of 16 bytes and rows of scale at multiples of 4: the functions here
   gemm_fp8                        C = A B^T of two such operands on the matrix cores
   linear_fp8                      a linear layer on these, for training and for serving
 
+Only linear_fp8 takes part in autograd; what the others return carries no gradient.
+
 Everything runs on torch's current stream of the tensors' device, or on `stream` (a raw handle as
 in ops.gemm): then results are allocated on that stream, the inputs are kept from reuse until it
 is done with them, and ordering against other streams is the caller's.  All calls can be captured
@@ -88,7 +90,7 @@ def transpose_fp8(q, scale, stream=None):
 
 def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=None, variant: int = 0):
     """out[M, N] = a[M, K] @ b[N, K]^T for operands in 8 bits with their block scales; each may be
-    e4m3 or e5m2 and have blocks of 1 x 128 or 128 x 128.  Any M, N, K >= 0 (K = 0 gives zeros).
+    e4m3 or e5m2 and have blocks of 1 x 128 or 128 x 128.  Any M, N and K <= 2^22 (K = 0 gives zeros).
     Sums are held in 32 bits and rounded once into bf16 or f16 (`out_dtype`, or `out`'s type; `out`
     needs its columns next to each other, its rows may be further apart; it must not overlap an
     input).  The matrix instruction drops a product 2^-14 and more below the largest of the 32 it
@@ -112,7 +114,8 @@ def linear_fp8(x, weight, weight_scale=None):
     Training: `weight` in bf16 or f16.  Both operands are quantised to e4m3 (x in blocks of 1 x 128,
     the weight 128 x 128).  For the backward pass x is kept as its 8-bit checkpoint, half the memory
     of the activation; dx = Q(dy) W with the kept 8-bit weight, dW = Q(dy^T) x with the checkpoint
-    transposed (as transpose_fp8 does).  A double backward is refused.
+    transposed (as transpose_fp8 does).  A double backward is refused.  K is at most 2^22, and so is N
+    where x takes a gradient and the number of x's rows where the weight takes one.
 
     Serving: `weight` in 8 bits with its `weight_scale`, as quantize_fp8(w, block_rows=128) gives
     them; x may take a gradient, the weight takes none."""

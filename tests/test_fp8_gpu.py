@@ -445,6 +445,37 @@ def test_out_counts_as_changed():
         z.backward()
 
 
+def test_out_is_refused_where_it_cannot_be_written():
+    a, sa = quantize_fp8(torch.randn(8, 128, device="cuda"))
+    with pytest.raises(ValueError, match="gradient"):
+        gemm_fp8(a, sa, a, sa, out=torch.ones(8, 8, device="cuda", dtype=BF16, requires_grad=True))
+    store = torch.zeros(4096, device="cuda", dtype=torch.uint8)
+    q = store[:1024].view(8, 128).view(E4M3)
+    for first in (0, 896, 1008):
+        with pytest.raises(ValueError, match="overlap"):
+            gemm_fp8(q, sa, a, sa, out=store[first:first + 128].view(BF16).view(8, 8))
+    gemm_fp8(q, sa, a, sa, out=store[1024:1152].view(BF16).view(8, 8))
+    assert not bool(store.any())
+
+
+def test_rows_longer_than_a_buffer_are_refused():
+    k = 2**22
+    x = torch.zeros(2, k + 1, device="cuda", dtype=BF16)
+    q, s = quantize_fp8(x)  # (a checkpoint may be as long as memory is)
+    assert torch.equal(dequantize_fp8(q, s), x)
+    with pytest.raises(ValueError, match="4194304"):
+        gemm_fp8(q, s, q, s)
+    with pytest.raises(ValueError, match="4194304"):
+        linear_fp8(x, x)
+    long = torch.zeros(k + 1, 8, device="cuda", dtype=BF16, requires_grad=True)
+    short = torch.zeros(4, 8, device="cuda", dtype=BF16, requires_grad=True)
+    assert linear_fp8(long, short.detach()).shape == (k + 1, 4) and linear_fp8(short.detach(), long).shape == (4, k + 1)
+    with pytest.raises(ValueError, match="4194304"):
+        linear_fp8(long, short)
+    with pytest.raises(ValueError, match="4194304"):
+        linear_fp8(short, long)
+
+
 def test_linear_keeps_8_bits_for_the_backward_pass():
     """Between the passes the layer holds its input in 8 bits (and the 8-bit weight), no 16-bit copy."""
     x = torch.randn(4096, 2048, device="cuda", dtype=BF16).requires_grad_()
