@@ -46,9 +46,15 @@ struct GemmFp8Args {
   int ctype;
   int variant;  // 0: by the sizes; 1: 128 x 128 tile, 2: 256 x 256 (K >= 144), 3: few rows (M <= 16), 4: 64 x 64,
                 // 5: 128 x 128 with two K tiles in LDS, so two blocks per CU, 6: few rows, 32 of B per wave
+  int parts;    // of K, multiplied by different blocks: 0: by the sizes; more than one: variants 1 and 4, at most 16
+  void* temp;   // gemm_fp8_temp_bytes, read and written during the call
 };
-// the kernel that a call runs (0 resolved), or -1 if the sizes do not fit it
-int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant);
+// what a call runs (0 resolved); variant -1 if the sizes do not fit it
+struct GemmFp8Plan {
+  int variant, parts;
+};
+GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts);
+int64_t gemm_fp8_temp_bytes(int64_t M, int64_t N, const GemmFp8Plan& plan);
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream);
 // the same for x[M][ldx] in bf16 or f16, quantised on its way (blocks of 1 x 128, e4m3), where it takes x
 bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K);

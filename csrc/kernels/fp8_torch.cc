@@ -114,6 +114,8 @@ Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType type) {
   return at::empty(size, like.options().dtype(type));
 }
 
+Tensor bytes(int64_t n, const Tensor& like) { return empty({n}, like, at::kByte); }
+
 // [rows, cols] of 1-byte values whose rows start at multiples of `pad` bytes
 Tensor empty_rows(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int64_t pad) {
   const int64_t ld = up(cols, pad);
@@ -185,7 +187,7 @@ Pair transpose_fp8(const Tensor& q, const Tensor& scale) {
 }
 
 Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
-                const std::optional<Tensor>& given, at::ScalarType out_dtype, int64_t variant) {
+                const std::optional<Tensor>& given, at::ScalarType out_dtype, int64_t variant, int64_t parts) {
   const Fp8In oa = operand("a", a, a_scale), ob = operand("b", b, b_scale);
   const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
   TORCH_CHECK_VALUE(b.size(1) == K, "shape mismatch ", a.sizes(), " x ", b.sizes(), "^T");
@@ -195,8 +197,9 @@ Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
     TORCH_CHECK_VALUE(given->dim() == 2 && given->size(0) == M && given->size(1) == N && row_major(*given),
                       "out must be [", M, ", ", N, "] with its columns next to each other, got ", given->sizes(),
                       ", strides ", given->strides());
-  TORCH_CHECK_VALUE(gpuexp::resolve_gemm_fp8_variant(M, N, K, int(variant)) >= 0, "variant ", variant,
-                    " does not take these sizes (", M, ", ", N, ", ", K, ")");
+  const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, int(variant), int(parts));
+  TORCH_CHECK_VALUE(plan.variant >= 0, "variant ", variant, " with ", parts, " parts does not take these sizes (", M, ", ",
+                    N, ", ", K, ")");
   check_gpu("gemm_fp8", a, a_scale, b, b_scale, given ? *given : a);
   TORCH_CHECK_VALUE(K <= kLongest, "gemm_fp8: rows of at most ", kLongest, " values, got ", K);
   const On on(a);
@@ -208,15 +211,18 @@ Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
       TORCH_CHECK_VALUE(!overlap(*given, *t), "out must not overlap an input");
     out.unsafeGetTensorImpl()->bump_version();  // an in-place change, to whoever saved `out`
   }
-  if (M && N)
-    check(gpuexp::launch_gemm_fp8({oa, ob, out.mutable_data_ptr(), wide_stride(out), M, N, K, wide_type(dtype), int(variant)},
+  if (M && N) {
+    Tensor temp;
+    if (const int64_t need = gpuexp::gemm_fp8_temp_bytes(M, N, plan)) temp = bytes(need, a);
+    check(gpuexp::launch_gemm_fp8({oa, ob, out.mutable_data_ptr(), wide_stride(out), M, N, K, wide_type(dtype),
+                                   plan.variant, plan.parts, temp.defined() ? temp.mutable_data_ptr() : nullptr},
                                   on.stream),
           "gemm_fp8");
+  }
   return out;
 }
 
 Tensor rows_of(const Tensor& x) { return row_major(x) ? x : x.contiguous(); }
-Tensor bytes(int64_t n, const Tensor& like) { return empty({n}, like, at::kByte); }
 
 // y = x w^T of x [M, K], w [N, K] and the workspace that the backward pass needs
 std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& w, bool want_dx, bool want_dw) {
@@ -306,7 +312,7 @@ struct ServeFp8 : torch::autograd::Function<ServeFp8> {
       at::AutoGradMode off(false);
       const auto [g, g_scale] = quantize_fp8(rows_of(grads[0]), at::kFloat8_e4m3fn, 1);
       const auto [wt, wt_scale] = transpose_fp8(saved[0], saved[1]);
-      results[0] = gemm_fp8(g, g_scale, wt, wt_scale, std::nullopt, grads[0].scalar_type(), 0);
+      results[0] = gemm_fp8(g, g_scale, wt, wt_scale, std::nullopt, grads[0].scalar_type(), 0, 0);
     }
     return once(std::move(results));
   }
@@ -360,8 +366,10 @@ PYBIND11_MODULE(_gpuexp_fp8, m) {
   m.def("transpose_fp8", &transpose_fp8);
   m.def("gemm_fp8", &gemm_fp8);
   m.def("linear_fp8", &linear_fp8);
-  m.def("gemm_fp8_variant", &gpuexp::resolve_gemm_fp8_variant, py::arg("M"), py::arg("N"), py::arg("K"),
-        py::arg("variant") = 0,
-        "The kernel variant a gemm_fp8 call with these sizes runs (0 = auto resolved), -1 if they do not fit it. "
-        "Host-only: no GPU needed.");
+  m.def("gemm_fp8_plan", [](int64_t M, int64_t N, int64_t K, int variant, int parts) {
+    const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, variant, parts);
+    return std::make_pair(plan.variant, plan.parts);
+  }, py::arg("M"), py::arg("N"), py::arg("K"), py::arg("variant") = 0, py::arg("parts") = 0,
+     "The kernel variant and the parts of K a gemm_fp8 call with these sizes runs (0 resolved); variant -1 if they do "
+     "not fit it. Host-only: no GPU needed.");
 }

@@ -175,18 +175,43 @@ __device__ __forceinline__ void lds_to_c(const uint8_t* smem, uint16_t* C, int64
   }
 }
 
+// the place, in f32x4, of a tile's sums over part `part` of K: [part][tile][32 x 32 fragment][4][lane]
+template <int kBM, int kBN>
+__device__ __forceinline__ int64_t part_at(int M, int N, int part, int tile_m, int tile_n) {
+  const int64_t nbn = (N + kBN - 1) / kBN, nbm = (M + kBM - 1) / kBM;
+  return ((part * nbm + tile_m) * nbn + tile_n) * (kBM * kBN / 4);
+}
+
+template <typename TC>
+__device__ __forceinline__ void store4(uint16_t* dst, const f32x4& v, int columns) {
+  typedef __attribute__((ext_vector_type(4))) uint16_t u16x4;
+  const u16x4 h{to16<TC>(v[0]), to16<TC>(v[1]), to16<TC>(v[2]), to16<TC>(v[3])};
+  if (columns >= 4) {
+    typedef u16x4 wide_t __attribute__((aligned(2)));  // (one store at any address)
+    *reinterpret_cast<wide_t*>(dst) = h;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < columns) dst[e] = h[e];
+  }
+}
+
 // ---- 128 x 128 and 64 x 64 tiles, 4 waves, 2 or 4 tiles of K in LDS ----
 // For sizes with too few 256 x 256 tiles to fill the card.  Waves are 2 x 2, each with a quarter of the
 // tile.  While K tile t is multiplied from registers, t + 1 is read from LDS and t + kStages is loaded
 // into the buffer that t left; one barrier per K tile.  Behind it every wave has its part of tile t + 1
 // (a counted wait: loads complete in order) and has tile t in registers.  Past the end of K the loads go
 // on out of range, so the count holds.  The K loop is unrolled by 4, so with 2 or 4 stages every LDS
-// address is a constant (6 stages of 64 x 64, with more in flight, took 19 us where 4 take 15, at
-// 64 x 8192 x 8192).  The scales come as in the 256 x 256 kernel; a quad's words are read with its first
-// K tile, and the next quad's loaded then, which the count covers.
+// address is a constant.  The scales come as in the 256 x 256 kernel; a quad's words are read with its
+// first K tile, and the next quad's loaded then, which the count covers.
+// From memory a CU gets 22 bytes a clock this way, 0.31 us for a K tile of 64 x 64, and 8 stages get no
+// more.  So where there are fewer tiles than CUs, K is cut into parts at multiples of 512 (a row's four
+// scales are one word), blockIdx.y of them: TC = float stores the sums of a part in 32 bits as the lanes
+// hold them, and join_parts_kernel adds them.
 template <int kA, int kB, typename TC, int kBM, int kBN, int kStages>
 __global__ void __launch_bounds__(256, 1)
-gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K) {
+gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc, int K, float* __restrict__ sums) {
+  constexpr bool kParts = std::is_same_v<TC, float>;
   constexpr int kStage = (kBM + kBN) * kBK, kScales = kStages * kStage, kRows = kBM + kBN;
   constexpr int kMI = kBM / 64, kNI = kBN / 64, kLoads = kRows / 32;  // 32-row fragments and loads per wave
   static_assert((kStages == 2 || kStages == 4) && kBM * kBN * 2 <= kScales, "slots are t % 4's, and C fits");
@@ -196,7 +221,11 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   const int wm = wave >> 1, wn = wave & 1;
   int row_a, row_b;
   tile_of_block<kBM, kBN, 8>(A.rows, B.rows, row_a, row_b);
-  const int K16 = K & ~15, nk = (K16 + kBK - 1) / kBK;
+  const int quads = (K + 4 * kBK - 1) / (4 * kBK);
+  // this block's quads of K, and its K tiles and bytes, without a last part of 16 bytes
+  const int q0 = kParts ? int(quads * blockIdx.y / gridDim.y) : 0;
+  const int q1 = kParts ? int(quads * (blockIdx.y + 1) / gridDim.y) : quads;
+  const int end = q1 == quads ? K & ~15 : q1 * 4 * kBK, t0 = q0 * 4, nk = (end + kBK - 1) / kBK;
   const rsrc_t ra = tile_rsrc(A, row_a, kBM, K), rb = tile_rsrc(B, row_b, kBN, K);
 
   // load i of a wave covers rows (wave + 4 i) * 8 .. + 8 of [A rows, B rows]
@@ -205,7 +234,7 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   const uint32_t va = uint32_t(lrow) * uint32_t(A.ld) + chunk, vb = uint32_t(lrow) * uint32_t(B.ld) + chunk;
   auto stage = [&](int t, int slot) {  // slot: t % kStages
     uint8_t* buf = smem + slot * kStage;
-    const bool in = chunk < K16 - t * kBK;
+    const bool in = chunk < end - t * kBK;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = (wave + 4 * i) * 8;
@@ -224,7 +253,6 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   int srow = (of_a ? row_a + wave * 64 : row_b + wave * 64 - kBM) + lane;
   srow = (srow < S.rows ? srow : S.rows - 1) >> S.shift;
   const uint8_t* sptr = S.scale + int64_t(srow) * S.lds;
-  const int quads = (nk + 3) / 4;
   auto stage_scales = [&](int quad) {
     typedef __attribute__((address_space(1))) void* gptr_t;
     if (loads_scales)
@@ -293,17 +321,17 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (nk > 0) {
-    stage_scales(0);
-    stage_scales(1);
+  if (nk > t0) {
+    stage_scales(q0);
+    stage_scales(q0 + 1);
 #pragma unroll
-    for (int t = 0; t < kStages; ++t) stage(t, t);
+    for (int t = 0; t < kStages; ++t) stage(t0 + t, t);
     wait_vm<(kStages - 1) * kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read_scales(0, sa, sb);
+    read_scales(q0, sa, sb);
     read(0, af[0], bf[0]);
-    for (int t = 0;; t += 4) {
+    for (int t = t0;; t += 4) {
       tile(t, std::integral_constant<int, 0>{});
       if (t + 1 >= nk) break;
       tile(t + 1, std::integral_constant<int, 1>{});
@@ -316,7 +344,7 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();  // no load in flight, every wave's reads done: LDS is free
   }
-  if (K != K16) {
+  if (end != K && q1 == quads) {
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
       const int x = wm * (kBM / 2) + i * 32 + (lane & 31);
@@ -330,13 +358,48 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
       }
     }
   }
+  if constexpr (kParts) {
+    f32x4* at = reinterpret_cast<f32x4*>(sums) + part_at<kBM, kBN>(A.rows, B.rows, blockIdx.y, row_a / kBM, row_b / kBN);
 #pragma unroll
-  for (int i = 0; i < kMI; ++i)
+    for (int i = 0; i < kMI; ++i)
 #pragma unroll
-    for (int j = 0; j < kNI; ++j)
-      tile_to_lds<kBN, TC>(smem, wm * (kBM / 2) + i * 32, wn * (kBN / 2) + j * 32, lane, acc[i][j]);
-  __syncthreads();
-  lds_to_c<kBM, kBN, 256>(smem, C, ldc, A.rows, B.rows, row_a, row_b);
+      for (int j = 0; j < kNI; ++j) {
+        const int f = (wm * kMI + i) * (kBN / 32) + wn * kNI + j;
+        if (row_a + (wm * kMI + i) * 32 < A.rows && row_b + (wn * kNI + j) * 32 < B.rows)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            at[(f * 4 + g) * 64 + lane] = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kMI; ++i)
+#pragma unroll
+      for (int j = 0; j < kNI; ++j)
+        tile_to_lds<kBN, TC>(smem, wm * (kBM / 2) + i * 32, wn * (kBN / 2) + j * 32, lane, acc[i][j]);
+    __syncthreads();
+    lds_to_c<kBM, kBN, 256>(smem, C, ldc, A.rows, B.rows, row_a, row_b);
+  }
+}
+
+// C from the parts' sums, added in the parts' order.  A thread has 4 columns of a row, as they lie in
+// the matrix instruction's result.
+template <typename TC, int kBM, int kBN>
+__global__ void __launch_bounds__(256)
+join_parts_kernel(const f32x4* __restrict__ sums, uint16_t* __restrict__ C, int64_t ldc, int M, int N, int parts) {
+  constexpr int kOf = kBM * kBN / 4;  // threads of a tile
+  const int64_t nbn = (N + kBN - 1) / kBN;
+  const int64_t tile = int64_t(blockIdx.x) / (kOf / 256);
+  const int at = int(blockIdx.x % (kOf / 256)) * 256 + threadIdx.x;
+  const int lane = at & 63, g = (at >> 6) & 3, f = at >> 8;
+  const int row = int(tile / nbn) * kBM + f / (kBN / 32) * 32 + (lane & 31);
+  const int col = int(tile % nbn) * kBN + f % (kBN / 32) * 32 + g * 8 + (lane >> 5) * 4;
+  if (row >= M || col >= N) return;
+  const int64_t step = part_at<kBM, kBN>(M, N, 1, 0, 0);
+  const f32x4* from = sums + tile * kOf + at;
+  f32x4 v = *from;
+#pragma unroll 4
+  for (int p = 1; p < parts; ++p) v += from[p * step];
+  store4<TC>(C + int64_t(row) * ldc + col, v, N - col);
 }
 
 // ---- 256 x 256 tile, 8 waves, two barriers per phase ----
@@ -750,17 +813,18 @@ double tile_us(int variant, int64_t M, int64_t N, double nk) {
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
   const double r = double((M + edge - 1) / edge) * double((N + edge - 1) / edge) / 256, whole = std::ceil(r);
   switch (variant) {
-    case 1: return r <= 1 ? 4 + (0.36 + 0.14 * r) * nk : whole * (3 + 0.5 * nk);
+    case 1: return r <= 1 ? 5.5 + (0.36 + 0.14 * r) * nk : whole * (3 + 0.5 * nk);
     case 2: return r <= 1 ? 6 + 6 * r + (0.85 + 0.4 * r * r) * nk : 6 + whole * (10 + 1.28 * nk);
     case 4: return r <= 1 ? 3 + 0.16 * nk : 2 + r * (1.2 + 0.19 * nk);
-    default: return r <= 1 ? 3 + (0.35 + 0.3 * r) * nk : 2 + r * (1.9 + 0.43 * nk);
+    default: return r <= 1 ? 4.5 + (0.35 + 0.3 * r) * nk : 2 + r * (1.9 + 0.43 * nk);
   }
 }
 
 // 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows (M <= 16), 4 = 64 x 64 tile,
 // 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU), 6 = few rows, 32 of B per wave;
 // -1: not these sizes.
-int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
+namespace {
+int resolve(int64_t M, int64_t N, int64_t K, int variant) {
   const bool two_k_tiles = K >= kBK + 16;
   if (variant < 0 || variant > 6 || (variant == 2 && !two_k_tiles) || ((variant == 3 || variant == 6) && M > 16)) return -1;
   if (variant != 0) return variant;
@@ -773,6 +837,56 @@ int resolve_gemm_fp8_variant(int64_t M, int64_t N, int64_t K, int variant) {
   for (int v : {1, 5, 2})
     if ((v != 2 || two_k_tiles) && tile_us(v, M, N, double(K) / kBK) < tile_us(best, M, N, double(K) / kBK)) best = v;
   return best;
+}
+
+}  // namespace
+
+namespace {
+
+// The same where each of `parts` blocks takes its part of K, at most one block for a CU, with the second
+// kernel that adds the parts' sums (3 us and their bytes).  Between the times of a B that is in the
+// last-level cache and of one that comes from memory (0.17 and 0.31 us a K tile of 64 x 64); from memory,
+// whole / in parts, us:
+//   17 x 1024 x 8192  18.4 / 8.7 (16)    64 x 4096 x 4096   12.6 / 10.4 (4)    512 x 4096 x 14336   64 / 51 (2)
+//   64 x 1024 x 8192  21.5 / 9.6 (8)     64 x 4096 x 14336  39.1 / 18.0 (4)    256 x 2048 x 16384   38 / 23 (8)
+double parts_us(int variant, int64_t M, int64_t N, int64_t K, int parts) {
+  const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
+  const double nk = double((quads + parts - 1) / parts * 4);
+  const double join = parts == 1 ? 0 : 3 + double(parts) * double((M + 31) / 32 * 32) * double(N) * 8 / 4.2e6;
+  return (variant == 4 ? 3 + 0.24 * nk : 4 + 0.55 * nk) + join;
+}
+
+}  // namespace
+
+GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts) {
+  GemmFp8Plan plan{resolve(M, N, K, variant), parts};
+  const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
+  const auto tiles = [&](int v) {
+    const int64_t edge = v == 4 ? 64 : 128;
+    return ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+  };
+  if (parts == 0) {
+    plan.parts = 1;
+    if (plan.variant < 0 || variant != 0 || M == 0 || N == 0) return plan;
+    const int v = plan.variant;
+    // up to 16 tokens the few-rows kernel takes what one CU needs for its 16 rows of B and all of A
+    double best = v == 3 ? 2 + double(K) / kBK * (0.08 + 0.003 * double(M))
+                  : (v == 4 || v == 1) && tiles(v) <= 256 ? parts_us(v, M, N, K, 1)
+                  : v == 6 ? 0 : tile_us(v, M, N, double(K) / kBK);
+    best -= 1.5;  // a launch more, and a workspace
+    for (int u : {4, 1})
+      for (int p = 2; p <= 16 && p <= quads && tiles(u) * p <= 256; ++p)
+        if (const double us = parts_us(u, M, N, K, p); us < best) best = us, plan = {u, p};
+  } else if (parts < 0 || parts > 16 ||
+             (parts > 1 && ((plan.variant != 1 && plan.variant != 4) || variant == 0 || parts > quads))) {
+    plan.variant = -1;
+  }
+  return plan;
+}
+
+int64_t gemm_fp8_temp_bytes(int64_t M, int64_t N, const GemmFp8Plan& plan) {
+  const int64_t edge = plan.variant == 4 ? 64 : 128;
+  return plan.variant < 0 || plan.parts <= 1 ? 0 : plan.parts * ((M + edge - 1) / edge) * ((N + edge - 1) / edge) * edge * edge * 4;
 }
 
 namespace {
@@ -792,12 +906,13 @@ void launch_rows(const GemmFp8Args& g, Operand oa, Operand ob, hipStream_t strea
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   if (g.M < 0 || g.N < 0 || g.K < 0 || !side_ok(g.a, g.M, g.K) || !side_ok(g.b, g.N, g.K)) return hipErrorInvalidValue;
   if (g.M == 0 || g.N == 0) return hipSuccess;
-  const int variant = resolve_gemm_fp8_variant(g.M, g.N, g.K, g.variant);
-  if (variant < 0) return hipErrorInvalidValue;
+  const GemmFp8Plan plan = plan_gemm_fp8(g.M, g.N, g.K, g.variant, g.parts);
+  const int variant = plan.variant, parts = plan.parts;
+  if (variant < 0 || (parts > 1 && !g.temp)) return hipErrorInvalidValue;
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
   const int64_t tiles = variant == 3 || variant == 6 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
   const int64_t threads = variant == 3 || variant == 6 ? 1024 : variant == 2 ? 512 : 256;
-  if (tiles * threads >= (int64_t(1) << 32)) return hipErrorInvalidValue;
+  if (tiles * (parts > 1 && parts < 16 ? 16 : parts) * threads >= (int64_t(1) << 32)) return hipErrorInvalidValue;
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
     const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
@@ -808,11 +923,23 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
     } else if (variant == 2) {
       hipLaunchKernelGGL((gemm_fp8_256_kernel<a, b, decltype(tc)>), dim3(uint32_t(tiles)), dim3(512), 0, stream, oa, ob,
                          c, g.ldc, int(g.K));
+    } else if (parts > 1) {
+      float* sums = static_cast<float*>(g.temp);
+      auto run = [&](auto edge_tag) {
+        constexpr int e = decltype(edge_tag)::value;
+        hipLaunchKernelGGL((gemm_fp8_tile_kernel<a, b, float, e, e, 4>), dim3(uint32_t(tiles), uint32_t(parts)), dim3(256),
+                           0, stream, oa, ob, nullptr, 0, int(g.K), sums);
+        hipLaunchKernelGGL((join_parts_kernel<decltype(tc), e, e>), dim3(uint32_t(tiles * (e * e / 1024))), dim3(256), 0,
+                           stream, reinterpret_cast<const f32x4*>(sums), c, g.ldc, int(g.M), int(g.N), parts);
+      };
+      if (variant == 1) run(std::integral_constant<int, 128>{});
+      else run(std::integral_constant<int, 64>{});
     } else {
       auto k = variant == 1   ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 4>
                : variant == 5 ? gemm_fp8_tile_kernel<a, b, decltype(tc), 128, 128, 2>
                               : gemm_fp8_tile_kernel<a, b, decltype(tc), 64, 64, 4>;
-      hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K));
+      hipLaunchKernelGGL(k, dim3(uint32_t(tiles)), dim3(256), 0, stream, oa, ob, c, g.ldc, int(g.K),
+                         static_cast<float*>(nullptr));
     }
   });
   return hipGetLastError();

@@ -4,6 +4,8 @@
 //   backward   dy -> Q(dy) and Q(dy^T) in one pass over dy, dx = Q(dy) Q(w), dw = Q(dy^T) T(Q(x))^T
 //              with T the kept x transposed and requantised along the tokens
 // Host code only; one call from Python per pass, since a small step is bound by the host.
+#include <algorithm>
+
 #include "fp8_launch.h"
 
 namespace gpuexp {
@@ -24,9 +26,18 @@ struct Piece {
   Fp8In in(const uint8_t* base) const { return {base + at, base + scales_at(), ld(), lds(), block_rows, kE4M3}; }
 };
 
+// a product and what it needs of a workspace
+int64_t gemm_bytes(int64_t M, int64_t N, int64_t K) {
+  return up(gemm_fp8_temp_bytes(M, N, plan_gemm_fp8(M, N, K, 0, 0)), 256);
+}
+hipError_t gemm(Fp8In a, Fp8In b, int64_t M, int64_t N, int64_t K, void* c, int ctype, void* temp, hipStream_t stream) {
+  return launch_gemm_fp8({a, b, c, N, M, N, K, ctype, 0, 0, temp}, stream);
+}
+
 struct Plan {
   Piece xq, wq, wt;      // forward: x, w; w transposed
   Piece gq, gt, xt;      // backward: dy, dy transposed, x transposed
+  int64_t forward_sums, backward_sums;  // of products whose K is cut into parts; the two backward products take turns
   LinearFp8Bytes bytes;
   Plan(int64_t M, int64_t N, int64_t K, bool dx, bool dw) : bytes{0, 0, 0} {
     auto take = [](Piece& p, int64_t& at, int64_t rows, int64_t cols, int block_rows) {
@@ -43,12 +54,12 @@ struct Plan {
       take(gt, bytes.backward_temp, N, M, 1);
       take(xt, bytes.backward_temp, K, M, 1);
     }
+    forward_sums = bytes.forward_temp;
+    backward_sums = bytes.backward_temp;
+    bytes.forward_temp += gemm_bytes(M, N, K);
+    bytes.backward_temp += std::max(dx ? gemm_bytes(M, K, N) : 0, dw ? gemm_bytes(N, K, M) : 0);
   }
 };
-
-hipError_t gemm(Fp8In a, Fp8In b, int64_t M, int64_t N, int64_t K, void* c, int ctype, hipStream_t stream) {
-  return launch_gemm_fp8({a, b, c, N, M, N, K, ctype, 0}, stream);
-}
 
 #define GPUEXP_RETURN_IF(call)                   \
   if (hipError_t e_ = (call); e_ != hipSuccess) \
@@ -66,7 +77,7 @@ hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_
   GPUEXP_RETURN_IF(launch_quantize_fp8(a.x, a.type, a.ldx, a.M, a.K, kE4M3, 1, p.xq.out(x_at), {}, stream));
   GPUEXP_RETURN_IF(launch_quantize_fp8(a.w, a.wtype, a.ldw, a.N, a.K, kE4M3, kFp8Block, p.wq.out(a.temp),
                                        a.want_dx ? p.wt.out(a.kept) : Fp8Out{}, stream));
-  return gemm(p.xq.in(x_at), p.wq.in(a.temp), a.M, a.N, a.K, y, a.type, stream);
+  return gemm(p.xq.in(x_at), p.wq.in(a.temp), a.M, a.N, a.K, y, a.type, a.temp + p.forward_sums, stream);
 }
 
 hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
@@ -76,16 +87,16 @@ hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, in
                                        a.want_dx ? p.gq.out(a.temp) : Fp8Out{},
                                        a.want_dw ? p.gt.out(a.temp) : Fp8Out{}, stream));
   if (a.want_dx)
-    GPUEXP_RETURN_IF(gemm(p.gq.in(a.temp), p.wt.in(a.kept), a.M, a.K, a.N, dx, a.type, stream));
+    GPUEXP_RETURN_IF(gemm(p.gq.in(a.temp), p.wt.in(a.kept), a.M, a.K, a.N, dx, a.type, a.temp + p.backward_sums, stream));
   if (a.want_dw) {
     GPUEXP_RETURN_IF(launch_transpose_fp8(p.xq.in(a.kept), a.M, a.K, p.xt.out(a.temp), stream));
-    GPUEXP_RETURN_IF(gemm(p.gt.in(a.temp), p.xt.in(a.temp), a.N, a.K, a.M, dw, a.wtype, stream));
+    GPUEXP_RETURN_IF(gemm(p.gt.in(a.temp), p.xt.in(a.temp), a.N, a.K, a.M, dw, a.wtype, a.temp + p.backward_sums, stream));
   }
   return hipSuccess;
 }
 
 int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
-  return gemm_fp8_takes_wide(x, ldx, M, N, K) ? 0 : Piece{M, K, 0, 1}.end();
+  return gemm_fp8_takes_wide(x, ldx, M, N, K) ? 0 : Piece{M, K, 0, 1}.end() + gemm_bytes(M, N, K);
 }
 
 hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
@@ -93,7 +104,7 @@ hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64
   if (gemm_fp8_takes_wide(x, ldx, M, N, K)) return launch_gemm_fp8_wide(x, type, ldx, w, M, N, K, y, stream);
   const Piece xq{M, K, 0, 1};
   GPUEXP_RETURN_IF(launch_quantize_fp8(x, type, ldx, M, K, kE4M3, 1, xq.out(temp), {}, stream));
-  return gemm(xq.in(temp), w, M, N, K, y, type, stream);
+  return gemm(xq.in(temp), w, M, N, K, y, type, temp + xq.end(), stream);
 }
 
 }  // namespace gpuexp

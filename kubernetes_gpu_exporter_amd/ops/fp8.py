@@ -88,7 +88,8 @@ def transpose_fp8(q, scale, stream=None):
     return _native.transpose_fp8(q, scale)
 
 
-def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=None, variant: int = 0):
+def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=None, variant: int = 0,
+             parts: int = 0):
     """out[M, N] = a[M, K] @ b[N, K]^T for operands in 8 bits with their block scales; each may be
     e4m3 or e5m2 and have blocks of 1 x 128 or 128 x 128.  Any M, N and K <= 2^22 (K = 0 gives zeros).
     Sums are held in 32 bits and rounded once into bf16 or f16 (`out_dtype`, or `out`'s type; `out`
@@ -96,16 +97,23 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, stream=
     input).  The matrix instruction drops a product 2^-14 and more below the largest of the 32 it
     adds at once.  variant 0 picks the kernel by the sizes; 1 / 2 force the 128x128 / 256x256 tile
     (the latter for K >= 144), 3 / 6 the kernel for few rows (M <= 16) with 16 / 32 rows of b per
-    wave, 4 the 64x64 tile, 5 the 128x128 tile with two blocks per CU."""
+    wave, 4 the 64x64 tile, 5 the 128x128 tile with two blocks per CU.  Where tiles are few and K is long, K is
+    cut into parts, multiplied by blocks of their own into 32 bits and added in order by a second kernel;
+    parts forces their number (variants 1 and 4, at most 16 and at most one for each 512 of K; 1: none)."""
     if stream is not None:
         with _elsewhere(stream, a, a_scale, b, b_scale, *([] if out is None else [out])):
-            return _native.gemm_fp8(a, a_scale, b, b_scale, out, out_dtype, variant)
-    return _native.gemm_fp8(a, a_scale, b, b_scale, out, out_dtype, variant)
+            return _native.gemm_fp8(a, a_scale, b, b_scale, out, out_dtype, variant, parts)
+    return _native.gemm_fp8(a, a_scale, b, b_scale, out, out_dtype, variant, parts)
 
 
 def gemm_fp8_variant(M: int, N: int, K: int, variant: int = 0) -> int:
     """The kernel variant that gemm_fp8 runs for these sizes (0 resolved), -1 if they do not fit it."""
-    return _native.gemm_fp8_variant(M, N, K, variant)
+    return _native.gemm_fp8_plan(M, N, K, variant)[0]
+
+
+def gemm_fp8_parts(M: int, N: int, K: int, variant: int = 0) -> int:
+    """The number of parts into which gemm_fp8 cuts K for these sizes."""
+    return _native.gemm_fp8_plan(M, N, K, variant)[1]
 
 
 def linear_fp8(x, weight, weight_scale=None):

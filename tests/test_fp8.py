@@ -2,8 +2,8 @@
 import pytest
 import torch
 
-from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_variant, linear_fp8, quantize_fp8,
-                                                 quantize_fp8_both, transpose_fp8)
+from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_parts, gemm_fp8_variant,
+                                                 linear_fp8, quantize_fp8, quantize_fp8_both, transpose_fp8)
 from tests.fp8_oracle import E4M3, E5M2, E8M0, pair, quantized, values
 
 
@@ -106,6 +106,13 @@ def test_variants_are_refused():
             gemm_fp8(b, t, b, t, variant=variant)
 
 
+def test_parts_are_refused():
+    a, s = q(4, 1024)
+    for variant, parts in ((1, -1), (1, 3), (4, 17), (0, 2), (2, 2), (3, 2), (5, 2), (6, 2)):  # 2 units of 512 in K
+        with pytest.raises(ValueError, match="parts"):
+            gemm_fp8(a, s, a, s, variant=variant, parts=parts)
+
+
 @pytest.mark.parametrize("dtype", [E4M3, E5M2])
 def test_oracle_matches_torch_rounding(dtype):
     """The oracle's rounding is torch's own cast where no scale applies (largest value = the type's)."""
@@ -133,3 +140,10 @@ def test_oracle_values_of_a_hand_made_pair():
 ])
 def test_gemm_variant_resolution(M, N, K, variant, want):
     assert gemm_fp8_variant(M, N, K, variant) == want
+
+
+@pytest.mark.parametrize("M,N,K,parts", [
+    (64, 4096, 8192, 4), (64, 1024, 8192, 8), (1, 1024, 8192, 1), (16, 1024, 8192, 16), (256, 4096, 8192, 1),
+    (64, 1024, 2048, 1), (64, 64, 0, 1), (0, 64, 8192, 1), (8192, 8192, 8192, 1)])
+def test_gemm_parts_of_k(M, N, K, parts):
+    assert gemm_fp8_parts(M, N, K) == parts

@@ -11,8 +11,8 @@ have both signs, in norm they stay under 2^-13 (measured alone: 1.5e-5 < 2^-16).
 import pytest
 import torch
 
-from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_variant, linear_fp8, quantize_fp8,
-                                                 quantize_fp8_both, transpose_fp8)
+from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_parts, gemm_fp8_variant,
+                                                 linear_fp8, quantize_fp8, quantize_fp8_both, transpose_fp8)
 from tests.fp8_oracle import E4M3, E5M2, E8M0, pair, quantized, small_whole, values
 
 pytestmark = pytest.mark.gpu
@@ -252,6 +252,28 @@ def test_gemm_into_a_view_leaves_the_rest(m, n, variant):
     assert bool((whole == 77.0).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 1, 513), (17, 33, 1025), (40, 100, 1039), (64, 64, 1536), (65, 129, 4096), (128, 200, 2050),
+                                   (100, 1, 5000), (300, 260, 8192), (129, 383, 8200)])
+@pytest.mark.parametrize("variant", [1, 4])
+@pytest.mark.parametrize("parts", [2, 3, 7, 16])
+def test_gemm_with_k_in_parts(m, n, k, variant, parts):
+    parts = min(parts, (k + 511) // 512)
+    g = gen(m + n + k)
+    for ta, tb, block_a, block_b, out in ((E4M3, E4M3, 1, 128, BF16), (E5M2, E5M2, 128, 1, F16)):
+        a, sa = pair(m, k, g, ta, block_a, spread=2, pad=16)
+        b, sb = pair(n, k, g, tb, block_b, spread=1)
+        want = exact_product(a, sa, b, sb)
+        assert float(want.abs().max()) < 2.0 ** 20
+        whole = torch.full((m + 2, n + 7), 77.0, device="cuda", dtype=out)
+        del_me = torch.full((16 * (m + 128) * (n + 128),), float("nan"), device="cuda")  # what the next workspace holds
+        del del_me
+        same(gemm_fp8(a, sa, b, sb, out=whole[1:m + 1, 3:n + 3], variant=variant, parts=parts), want.float().to(out))
+        whole[1:m + 1, 3:n + 3] = 77.0
+        assert bool((whole == 77.0).all())
+        for _ in range(3):
+            same(gemm_fp8(a, sa, b, sb, out_dtype=out, variant=variant, parts=parts), want.float().to(out))
+
+
 @pytest.mark.parametrize("m,n,k", [(4, 6, 0), (0, 6, 128), (4, 0, 128), (0, 0, 0), (700, 300, 0)])
 def test_gemm_of_empty_sizes(m, n, k):
     a, sa = quantize_fp8(torch.zeros(m, k, device="cuda"))
@@ -390,7 +412,8 @@ def test_linear_of_one_gradient_only_and_broadcast_gradients():
         assert tuple(ye.shape) == (*shape[:-1], 128) and ge.shape == xe.shape and not bool(gw.any())
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (17, 300, 130), (257, 384, 1000), (1030, 640, 512)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (17, 300, 130), (257, 384, 1000), (1030, 640, 512), (33, 520, 8200),
+                                   (8200, 260, 500), (40, 8192, 300)])  # the last: K in parts for y, dw, dx
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_linear_is_the_operators_in_turn(m, n, k, dtype):
     """A layer's passes, the operators one after the other as a program would call them, and the two orientations in
@@ -592,6 +615,35 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         got = [o.clone() for o in outs]
         want = (*step(x.detach().requires_grad_(), w.detach().requires_grad_(), grad), linear_fp8(token, wq, ws))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_products_in_parts_captured_and_replayed():
+    """All three products of a step with K in parts, and a serving step's, each with a workspace of its own."""
+    g = gen(13)
+    big = [torch.randn(s, device="cuda", generator=g).to(BF16) for s in ((40, 8192), (256, 8192), (4096, 200), (300, 200))]
+    x, w, x2, w2 = (t.requires_grad_() for t in big)
+    wq, ws = quantize_fp8(w.detach(), block_rows=128)
+    assert gemm_fp8_parts(40, 256, 8192) > 1 and gemm_fp8_parts(300, 200, 4096) > 1
+    grad, grad2 = (torch.randn(s, device="cuda", generator=g).to(BF16) for s in ((40, 256), (4096, 300)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w, grad), step(x2, w2, grad2), linear_fp8(x.detach(), wq, ws)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = (*step(x, w, grad), *step(x2, w2, grad2), linear_fp8(x.detach(), wq, ws))
+    for seed in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, device="cuda", generator=gen(seed)))
+            x2.copy_(torch.randn(x2.shape, device="cuda", generator=gen(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        one, two = ([t.detach().requires_grad_() for t in pair_] for pair_ in ((x, w), (x2, w2)))
+        want = (*step(*one, grad), *step(*two, grad2), linear_fp8(x.detach(), wq, ws))
         for a, b in zip(got, want):
             assert torch.equal(a, b)
 
