@@ -948,10 +948,12 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
 // Every block quantises the rows of x that it needs, which up to 2^24 weights costs less than a launch of
 // its own (one and 16 tokens, us, this way / two launches: 512 x 512 2.8 / 4.1 and 3.0 / 4.8, 4096 x 4096
 // 7.5 / 8.4 and 9.4 / 9.8) and beyond more (8192 x 8192 20.4 / 17.4 and 28.4 / 19.7).  The vector loads
-// of x want its rows at multiples of 16 bytes and no row to end inside 16 values.
+// of x want its rows at multiples of 16 bytes and no row to end inside 16 values.  Nor where the product
+// takes K in parts (16 x 1024 x 8192: 13.2 / 11.1).
 bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
   return M >= 1 && M <= 16 && K >= 1 && K % 16 == 0 && K <= 8192 && N * K <= (int64_t(1) << 24) &&
-         reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || (ldx % 8 == 0 && ldx <= (int64_t(1) << 21)));
+         reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || (ldx % 8 == 0 && ldx <= (int64_t(1) << 21))) &&
+         plan_gemm_fp8(M, N, K, 0, 0).parts == 1;
 }
 
 hipError_t launch_gemm_fp8_wide(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K,
