@@ -682,13 +682,18 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
   const uint32_t* psa = nullptr;
   if constexpr (kWide < 0)
     psa = reinterpret_cast<const uint32_t*>(A.scale + int64_t((l15 < A.rows ? l15 : A.rows - 1) >> A.shift) * A.lds);
-  // one scale block (128 bytes of K) of 16 rows; past K16 zeros
-  auto load = [&](rsrc_t rsrc, uint32_t at, int k) {
-    const i32x4 lo = __builtin_bit_cast(
-        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk < K16 - k ? at : kOob, k, 0));
-    const i32x4 hi = __builtin_bit_cast(
-        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk + 64 < K16 - k ? at + 64 : kOob, k, 0));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  // One scale block (128 bytes of K) of 16 rows; past K16 zeros.  `first`: which of its two chunks a lane
+  // loads first.  Every other row of A the other half of its line: 16 x 64 bytes of equal halves take the
+  // first-level cache twice as long (16 x 1024 x 4096 6.3 us, so 4.7).  B's rows so too where the card is
+  // not full (16 x 1024 x 16384 18.2 / 15.5); else whole lines in turn come faster from memory.  32 rows of
+  // B gain nothing (16 x 8192 x 8192 15.9 / 16.8).
+  const int first_a = kR == 1 ? (l15 & 1) * 64 : 0, first_b = gridDim.x < 256 ? first_a : 0;
+  auto load = [&](rsrc_t rsrc, uint32_t at, int k, int first) {
+    const i32x4 x = __builtin_bit_cast(
+        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk + first < K16 - k ? at + first : kOob, k, 0));
+    const i32x4 y = __builtin_bit_cast(
+        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, chunk + (first ^ 64) < K16 - k ? at + (first ^ 64) : kOob, k, 0));
+    return __builtin_shufflevector(first ? y : x, first ? x : y, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   const uint32_t at_a = uint32_t(l15) * uint32_t(A.ld) + (kWide < 0 ? chunk : 2 * chunk), at_b = uint32_t(l15) * uint32_t(B.ld) + chunk;
 
@@ -713,8 +718,8 @@ gemm_fp8_rows_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int r = 0; r < kR; ++r) b[r][i] = load(rb, at_b + r * 16 * uint32_t(B.ld), q * kQuad + i * kBK);
-      if constexpr (kWide < 0) a[i] = load(ra, at_a, q * kQuad + i * kBK);
+      for (int r = 0; r < kR; ++r) b[r][i] = load(rb, at_b + r * 16 * uint32_t(B.ld), q * kQuad + i * kBK, first_b);
+      if constexpr (kWide < 0) a[i] = load(ra, at_a, q * kQuad + i * kBK, first_a);
     }
 #pragma unroll
     for (int r = 0; r < kR; ++r) sb[r] = psb[r][q];
