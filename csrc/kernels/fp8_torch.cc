@@ -32,7 +32,7 @@ constexpr int64_t kLongest = int64_t(1) << 22;
 
 void check(hipError_t e, const char* what) {
   TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": larger than the kernels index (fewer than 2^31 rows, rows at most "
-                    "4 MiB apart in 8 bits, fewer than 2^35 values to quantise)");
+                    "4 MiB apart in 8 bits, fewer than 2^35 values to quantise, fewer than 2^23 tiles of a product)");
   TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
 }
 

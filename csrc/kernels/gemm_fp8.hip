@@ -807,85 +807,67 @@ bool side_ok(const Fp8In& in, int64_t rows, int64_t K) {
 
 }  // namespace
 
-// What a call takes on this card, in microseconds, by the tile: measured over 23 sizes from 33 x 4096 x
-// 4096 to 8192^3, which these lines fit within 20 % and order rightly but for near ties.  `r` is rounds
-// of 256 blocks, `nk` tiles of K.  Up to one round a block has a CU to itself and a K tile costs what its
-// loads take, the more the more blocks load at once; beyond it rounds add up, whole ones where one block
-// fills a CU.  Examples (128 x 128, 128 x 128 two per CU, 256 x 256, 64 x 64; us):
-//   256 x 4096 x 4096   16.2  15.9  36.4   8.6        2048 x 4096 x 4096  38.9  33.1  38.9   51.9
-//   1024 x 4096 x 4096  20.4  24.7  37.5  26.7        4096 x 4096 x 4096  76.4  64.0  55.9  101.3
-double tile_us(int variant, int64_t M, int64_t N, double nk) {
+namespace {
+
+// What a call takes on this card, in microseconds, by the kernel and the parts of K: a line in the tiles
+// of K (`nk`) for each round of 256 blocks, whose slope grows with the part of the card that loads at
+// once.  In parts there is a second kernel and its bytes, and 1 us for a launch and a workspace more.
+// The numbers are those of 600 random sizes (1 to 8192 x 64 to 16384 x 128 to 16384, B in the caches and
+// from memory) with which the choice costs least: on 400 others 0.7 % (caches) and 1.2 % (memory) against
+// the fastest kernel in the mean.  Examples,
+// B from memory, us:                          128 x 128   two per CU   256 x 256   64 x 64
+//   256 x 4096 x 4096                          21.9        30.3         42.7        12.1
+//   1024 x 4096 x 4096                         23.1        31.4         42.4        33.6
+//   4096 x 4096 x 4096 (from the caches)       76.4        64.0         55.9        101.3
+//                                             few rows   32 of B per wave   64 x 64
+//   1 / 16 x 4096 x 8192                       9.4 / 10.9   11.6 / 15.1      18.7 / 19.1
+//   1 / 16 x 8192 x 8192                       16.0 / 19.4  14.2 / 16.0      19.5 / 20.0
+//   1 / 16 x 16384 x 2048                      8.5 / 9.9    8.8 / 9.6        8.3 / 8.4
+//                                             whole   in parts
+//   17 x 1024 x 8192                           18.4    8.7 (16 of 64 x 64)
+//   64 x 4096 x 14336                          39.1    18.0 (4 of 64 x 64)
+//   512 x 4096 x 14336                         64      51 (2 of 128 x 128)
+double estimate_us(int variant, int64_t M, int64_t N, int64_t K, int parts) {
+  const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
+  const double nk = parts > 1 ? double((quads + parts - 1) / parts * 4) : double(K) / kBK;
+  auto rounds = [](double r) { return r <= 1 ? 1 : std::ceil(r); };
+  if (variant == 3) return 1.1 + rounds(double((N + 15) / 16) / 256) * (0.19 + (0.068 + 0.002 * double(M)) * nk);
+  if (variant == 6) return 2 + rounds(double((N + 31) / 32) / 256) * (0.1 + (0.117 + 0.001 * double(M)) * nk);
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
-  const double r = double((M + edge - 1) / edge) * double((N + edge - 1) / edge) / 256, whole = std::ceil(r);
-  switch (variant) {
-    case 1: return r <= 1 ? 5.5 + (0.36 + 0.14 * r) * nk : whole * (3 + 0.5 * nk);
-    case 2: return r <= 1 ? 6 + 6 * r + (0.85 + 0.4 * r * r) * nk : 6 + whole * (10 + 1.28 * nk);
-    case 4: return r <= 1 ? 3 + 0.16 * nk : 2 + r * (1.2 + 0.19 * nk);
-    default: return r <= 1 ? 4.5 + (0.35 + 0.3 * r) * nk : 2 + r * (1.9 + 0.43 * nk);
-  }
-}
-
-// 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows (M <= 16), 4 = 64 x 64 tile,
-// 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU), 6 = few rows, 32 of B per wave;
-// -1: not these sizes.
-namespace {
-int resolve(int64_t M, int64_t N, int64_t K, int variant) {
-  const bool two_k_tiles = K >= kBK + 16;
-  if (variant < 0 || variant > 6 || (variant == 2 && !two_k_tiles) || ((variant == 3 || variant == 6) && M > 16)) return -1;
-  if (variant != 0) return variant;
-  // Up to 16 tokens: 16 rows of B per wave, or 32, which reads A half as often, where that still fills
-  // the card, or 64 x 64 tiles, which read A once, where B is very wide.  One and 16 tokens, weights
-  // from memory, us:  4096 x 8192  10.1 / 11.7 / 18.7 and 12.9 / 15.1 / 19.2
-  //   8192 x 8192  16.4 / 15.0 / 21.4 and 21.6 / 17.0 / 22.4     16384 x 2048  9.2 / 8.9 / 8.3 and 11.9 / 9.6 / 8.4
-  if (M <= 16) return N >= 16384 && (K <= 2048 || M > 8) ? 4 : N >= 8192 && K >= 2048 && (M > 4 || K >= 8192) ? 6 : 3;
-  int best = 4;
-  for (int v : {1, 5, 2})
-    if ((v != 2 || two_k_tiles) && tile_us(v, M, N, double(K) / kBK) < tile_us(best, M, N, double(K) / kBK)) best = v;
-  return best;
+  const double r = double((M + edge - 1) / edge) * double((N + edge - 1) / edge) * parts / 256, full = r < 1 ? r : 1;
+  const double us = variant == 1   ? 2.2 + rounds(r) * (3.7 + (0.38 + 0.14 * full) * nk)
+                    : variant == 2 ? 0.3 + rounds(r) * (13 + (1.05 + 0.2 * full) * nk)
+                    : variant == 4 ? 2.7 + rounds(r) * (1 + (0.165 + 0.05 * full) * nk)
+                                   : 3.9 + rounds(r) * (1.9 + (0.4 + 0.125 * full) * nk);
+  return parts == 1 ? us : us + 2 + double(parts) * double((M + 31) / 32 * 32) * double(N) * 8 / 4.6e6;
 }
 
 }  // namespace
 
-namespace {
-
-// The same where each of `parts` blocks takes its part of K, at most one block for a CU, with the second
-// kernel that adds the parts' sums (3 us and their bytes).  Between the times of a B that is in the
-// last-level cache and of one that comes from memory (0.17 and 0.31 us a K tile of 64 x 64); from memory,
-// whole / in parts, us:
-//   17 x 1024 x 8192  18.4 / 8.7 (16)    64 x 4096 x 4096   12.6 / 10.4 (4)    512 x 4096 x 14336   64 / 51 (2)
-//   64 x 1024 x 8192  21.5 / 9.6 (8)     64 x 4096 x 14336  39.1 / 18.0 (4)    256 x 2048 x 16384   38 / 23 (8)
-double parts_us(int variant, int64_t M, int64_t N, int64_t K, int parts) {
-  const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
-  const double nk = double((quads + parts - 1) / parts * 4);
-  const double join = parts == 1 ? 0 : 3 + double(parts) * double((M + 31) / 32 * 32) * double(N) * 8 / 4.2e6;
-  return (variant == 4 ? 3 + 0.24 * nk : 4 + 0.55 * nk) + join;
-}
-
-}  // namespace
-
+// variant 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows (M <= 16), 4 = 64 x 64
+// tile, 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU), 6 = few rows, 32 of B per wave;
+// parts 0 = by the sizes, with a variant 1
 GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts) {
-  GemmFp8Plan plan{resolve(M, N, K, variant), parts};
+  const auto takes = [&](int v) { return v == 2 ? K >= kBK + 16 : v == 3 || v == 6 ? M <= 16 : v >= 1 && v <= 5; };
   const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
-  const auto tiles = [&](int v) {
-    const int64_t edge = v == 4 ? 64 : 128;
-    return ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
-  };
-  if (parts == 0) {
-    plan.parts = 1;
-    if (plan.variant < 0 || variant != 0 || M == 0 || N == 0) return plan;
-    const int v = plan.variant;
-    // up to 16 tokens the few-rows kernel takes what one CU needs for its 16 rows of B and all of A
-    double best = v == 3 ? 2 + double(K) / kBK * (0.08 + 0.003 * double(M))
-                  : (v == 4 || v == 1) && tiles(v) <= 256 ? parts_us(v, M, N, K, 1)
-                  : v == 6 ? 0 : tile_us(v, M, N, double(K) / kBK);
-    best -= 1.5;  // a launch more, and a workspace
-    for (int u : {4, 1})
-      for (int p = 2; p <= 16 && p <= quads && tiles(u) * p <= 256; ++p)
-        if (const double us = parts_us(u, M, N, K, p); us < best) best = us, plan = {u, p};
-  } else if (parts < 0 || parts > 16 ||
-             (parts > 1 && ((plan.variant != 1 && plan.variant != 4) || variant == 0 || parts > quads))) {
-    plan.variant = -1;
+  if (variant != 0) {
+    const bool ok = takes(variant) && parts >= 0 &&
+                    (parts <= 1 || ((variant == 1 || variant == 4) && parts <= 16 && parts <= quads));
+    return {ok ? variant : -1, parts > 1 ? parts : 1};
   }
+  if (parts < 0 || parts > 1) return {-1, 1};
+  GemmFp8Plan plan{4, 1};
+  double best = estimate_us(4, M, N, K, 1);
+  const auto consider = [&](int v, int p) {
+    if (const double us = estimate_us(v, M, N, K, p); us < best) best = us, plan = {v, p};
+  };
+  for (int v : {1, 5, 2, 3, 6})
+    if (takes(v)) consider(v, 1);
+  if (parts == 0 && M > 0 && N > 0)
+    for (int v : {4, 1}) {
+      const int64_t edge = v == 4 ? 64 : 128, tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+      for (int p = 2; p <= 16 && p <= quads && tiles * p <= 512; ++p) consider(v, p);
+    }
   return plan;
 }
 
