@@ -75,14 +75,14 @@ struct LinearFp8Args {
   uint8_t* kept;
   uint8_t* temp;
 };
-struct LinearFp8Bytes {
-  int64_t kept, forward_temp, backward_temp;
-};
-LinearFp8Bytes linear_fp8_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);
+int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);
+int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);   // temp
+int64_t linear_fp8_backward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);  // temp
 hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream);
 hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
                                       hipStream_t stream);
-// the same with a weight that is in 8 bits already; temp: x in 8 bits, where the product does not make it
+// the same with a weight that is in 8 bits already; temp: x in 8 bits, where the product
+// does not make it, and the product's own
 int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K);
 hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
                             uint8_t* temp, hipStream_t stream);

@@ -228,8 +228,9 @@ Tensor rows_of(const Tensor& x) { return row_major(x) ? x : x.contiguous(); }
 std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& w, bool want_dx, bool want_dw) {
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const On on(x);
-  const gpuexp::LinearFp8Bytes need = gpuexp::linear_fp8_bytes(M, N, K, want_dx, want_dw);
-  Tensor y = empty({M, N}, x, x.scalar_type()), kept = bytes(need.kept, x), temp = bytes(need.forward_temp, x);
+  Tensor y = empty({M, N}, x, x.scalar_type()),
+         kept = bytes(gpuexp::linear_fp8_kept_bytes(M, N, K, want_dx, want_dw), x),
+         temp = bytes(gpuexp::linear_fp8_forward_bytes(M, N, K, want_dx, want_dw), x);
   gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, x.const_data_ptr(), wide_stride(x), w.const_data_ptr(),
                           wide_stride(w), wide_type(x.scalar_type()), wide_type(w.scalar_type()),
                           static_cast<uint8_t*>(kept.mutable_data_ptr()), static_cast<uint8_t*>(temp.mutable_data_ptr())};
@@ -272,7 +273,7 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
       const On on(dy);
       if (want_dx) results[0] = empty({M, K}, dy, dy.scalar_type());
       if (want_dw) results[1] = empty({N, K}, dy, wtype);
-      const Tensor temp = bytes(gpuexp::linear_fp8_bytes(M, N, K, want_dx, want_dw).backward_temp, dy);
+      const Tensor temp = bytes(gpuexp::linear_fp8_backward_bytes(M, N, K, want_dx, want_dw), dy);
       gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, nullptr, 0, nullptr, 0, wide_type(dy.scalar_type()),
                               wide_type(wtype), static_cast<uint8_t*>(kept.mutable_data_ptr()),
                               static_cast<uint8_t*>(temp.mutable_data_ptr())};

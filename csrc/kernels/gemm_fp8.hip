@@ -827,19 +827,17 @@ namespace {
 //   17 x 1024 x 8192                           18.4    8.7 (16 of 64 x 64)
 //   64 x 4096 x 14336                          39.1    18.0 (4 of 64 x 64)
 //   512 x 4096 x 14336                         64      51 (2 of 128 x 128)
-double estimate_us(int variant, int64_t M, int64_t N, int64_t K, int parts) {
-  const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
-  const double nk = parts > 1 ? double((quads + parts - 1) / parts * 4) : double(K) / kBK;
-  auto rounds = [](double r) { return r <= 1 ? 1 : std::ceil(r); };
-  if (variant == 3) return 1.1 + rounds(double((N + 15) / 16) / 256) * (0.19 + (0.068 + 0.002 * double(M)) * nk);
-  if (variant == 6) return 2 + rounds(double((N + 31) / 32) / 256) * (0.1 + (0.117 + 0.001 * double(M)) * nk);
-  const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
-  const double r = double((M + edge - 1) / edge) * double((N + edge - 1) / edge) * parts / 256, full = r < 1 ? r : 1;
-  const double us = variant == 1   ? 2.2 + rounds(r) * (3.7 + (0.38 + 0.14 * full) * nk)
-                    : variant == 2 ? 0.3 + rounds(r) * (13 + (1.05 + 0.2 * full) * nk)
-                    : variant == 4 ? 2.7 + rounds(r) * (1 + (0.165 + 0.05 * full) * nk)
-                                   : 3.9 + rounds(r) * (1.9 + (0.4 + 0.125 * full) * nk);
-  return parts == 1 ? us : us + 2 + double(parts) * double((M + 31) / 32 * 32) * double(N) * 8 / 4.6e6;
+double estimate_us(int variant, int64_t M, int64_t blocks, double nk) {
+  const double rounds = blocks <= 256 ? 1 : double((blocks + 255) >> 8);
+  const double full = blocks < 256 ? double(blocks) * (1.0 / 256) : 1;
+  switch (variant) {
+    case 1: return 2.2 + rounds * (3.7 + (0.38 + 0.14 * full) * nk);
+    case 2: return 0.3 + rounds * (13 + (1.05 + 0.2 * full) * nk);
+    case 3: return 1.1 + rounds * (0.19 + (0.068 + 0.002 * double(M)) * nk);
+    case 4: return 2.7 + rounds * (1 + (0.165 + 0.05 * full) * nk);
+    case 5: return 3.9 + rounds * (1.9 + (0.4 + 0.125 * full) * nk);
+    default: return 2 + rounds * (0.1 + (0.117 + 0.001 * double(M)) * nk);
+  }
 }
 
 }  // namespace
@@ -856,18 +854,29 @@ GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int part
     return {ok ? variant : -1, parts > 1 ? parts : 1};
   }
   if (parts < 0 || parts > 1) return {-1, 1};
+  const double nk = double(K) * (1.0 / kBK);
+  const auto tiles = [&](int edge) { return ((M + edge - 1) / edge) * ((N + edge - 1) / edge); };
+  const int64_t of_64 = tiles(64), of_128 = tiles(128);
   GemmFp8Plan plan{4, 1};
-  double best = estimate_us(4, M, N, K, 1);
-  const auto consider = [&](int v, int p) {
-    if (const double us = estimate_us(v, M, N, K, p); us < best) best = us, plan = {v, p};
+  double best = estimate_us(4, M, of_64, nk);
+  const auto consider = [&](int v, int p, double us) {
+    if (us < best) best = us, plan = {v, p};
   };
-  for (int v : {1, 5, 2, 3, 6})
-    if (takes(v)) consider(v, 1);
-  if (parts == 0 && M > 0 && N > 0)
-    for (int v : {4, 1}) {
-      const int64_t edge = v == 4 ? 64 : 128, tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
-      for (int p = 2; p <= 16 && p <= quads && tiles * p <= 512; ++p) consider(v, p);
+  consider(1, 1, estimate_us(1, M, of_128, nk));
+  consider(5, 1, estimate_us(5, M, of_128, nk));
+  if (takes(2)) consider(2, 1, estimate_us(2, M, tiles(256), nk));
+  if (takes(3)) {
+    consider(3, 1, estimate_us(3, M, (N + 15) / 16, nk));
+    consider(6, 1, estimate_us(6, M, (N + 31) / 32, nk));
+  }
+  if (parts == 0 && of_128 > 0) {
+    const double join = double((M + 31) / 32 * 32) * double(N) * (8 / 4.6e6);  // a part's sums, written and read
+    for (int p = 2; p <= 16 && p <= quads && of_128 * p <= 512; ++p) {
+      const double part = double((int(quads) + p - 1) / p * 4), more = 2 + p * join;
+      if (of_64 * p <= 512) consider(4, p, estimate_us(4, M, of_64 * p, part) + more);
+      consider(1, p, estimate_us(1, M, of_128 * p, part) + more);
     }
+  }
   return plan;
 }
 
@@ -932,15 +941,15 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Every block quantises the rows of x that it needs, which up to 2^24 weights costs less than a launch of
-// its own (one and 16 tokens, us, this way / two launches: 512 x 512 2.8 / 4.1 and 3.0 / 4.8, 4096 x 4096
-// 7.5 / 8.4 and 9.4 / 9.8) and beyond more (8192 x 8192 20.4 / 17.4 and 28.4 / 19.7).  The vector loads
-// of x want its rows at multiples of 16 bytes and no row to end inside 16 values.  Nor where the product
-// takes K in parts (16 x 1024 x 8192: 13.2 / 11.1).
+// Every block quantises the rows of x that it needs, which up to 2^24 weights, and 2^25 for up to 8 tokens,
+// costs no more than a launch of its own (1 and 16 tokens, us, this way / two launches: 512 x 512 2.9 / 4.6
+// and 3.0 / 5.1, 4096 x 4096 7.6 / 8.4 and 9.2 / 9.0, 16384 x 2048 10.5 / 11.2 and 14.5 / 12.2) and beyond
+// more (8 x 8192 x 8192 23.2 / 17.3); likewise up to 2^16 values of x (16 x 1024 x 8192 13.2 / 11.1).  The vector loads of x want its rows at multiples of 16
+// bytes and no row to end inside 16 values.
 bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
-  return M >= 1 && M <= 16 && K >= 1 && K % 16 == 0 && K <= 8192 && N * K <= (int64_t(1) << 24) &&
-         reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || (ldx % 8 == 0 && ldx <= (int64_t(1) << 21))) &&
-         plan_gemm_fp8(M, N, K, 0, 0).parts == 1;
+  return M >= 1 && M <= 16 && K >= 1 && K % 16 == 0 && K <= 8192 && M * K <= 65536 &&
+         N * K <= (int64_t(1) << (M <= 8 ? 25 : 24)) &&
+         reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || (ldx % 8 == 0 && ldx <= (int64_t(1) << 21)));
 }
 
 hipError_t launch_gemm_fp8_wide(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K,

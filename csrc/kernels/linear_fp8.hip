@@ -26,19 +26,23 @@ struct Piece {
   Fp8In in(const uint8_t* base) const { return {base + at, base + scales_at(), ld(), lds(), block_rows, kE4M3}; }
 };
 
-// a product and what it needs of a workspace
-int64_t gemm_bytes(int64_t M, int64_t N, int64_t K) {
-  return up(gemm_fp8_temp_bytes(M, N, plan_gemm_fp8(M, N, K, 0, 0)), 256);
-}
-hipError_t gemm(Fp8In a, Fp8In b, int64_t M, int64_t N, int64_t K, void* c, int ctype, void* temp, hipStream_t stream) {
-  return launch_gemm_fp8({a, b, c, N, M, N, K, ctype, 0, 0, temp}, stream);
-}
+// a product, and where in a workspace it keeps the sums of the parts of K
+struct Product {
+  int64_t M, N, K;
+  GemmFp8Plan plan;
+  Product(int64_t M, int64_t N, int64_t K) : M(M), N(N), K(K), plan(plan_gemm_fp8(M, N, K, 0, 0)) {}
+  int64_t bytes() const { return up(gemm_fp8_temp_bytes(M, N, plan), 256); }
+  hipError_t run(Fp8In a, Fp8In b, void* c, int ctype, void* temp, hipStream_t stream) const {
+    return launch_gemm_fp8({a, b, c, N, M, N, K, ctype, plan.variant, plan.parts, temp}, stream);
+  }
+};
 
 struct Plan {
   Piece xq, wq, wt;      // forward: x, w; w transposed
   Piece gq, gt, xt;      // backward: dy, dy transposed, x transposed
-  int64_t forward_sums, backward_sums;  // of products whose K is cut into parts; the two backward products take turns
-  LinearFp8Bytes bytes;
+  struct {
+    int64_t kept, forward_temp, backward_temp;
+  } bytes;  // without the products' sums, which follow in a pass's workspace
   Plan(int64_t M, int64_t N, int64_t K, bool dx, bool dw) : bytes{0, 0, 0} {
     auto take = [](Piece& p, int64_t& at, int64_t rows, int64_t cols, int block_rows) {
       p = {rows, cols, at, block_rows};
@@ -54,10 +58,6 @@ struct Plan {
       take(gt, bytes.backward_temp, N, M, 1);
       take(xt, bytes.backward_temp, K, M, 1);
     }
-    forward_sums = bytes.forward_temp;
-    backward_sums = bytes.backward_temp;
-    bytes.forward_temp += gemm_bytes(M, N, K);
-    bytes.backward_temp += std::max(dx ? gemm_bytes(M, K, N) : 0, dw ? gemm_bytes(N, K, M) : 0);
   }
 };
 
@@ -67,8 +67,18 @@ struct Plan {
 
 }  // namespace
 
-LinearFp8Bytes linear_fp8_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
-  return Plan(M, N, K, want_dx, want_dw).bytes;
+int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
+  return Plan(M, N, K, want_dx, want_dw).bytes.kept;
+}
+
+int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
+  return Plan(M, N, K, want_dx, want_dw).bytes.forward_temp + Product(M, N, K).bytes();
+}
+
+// the two products take turns at the same place
+int64_t linear_fp8_backward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
+  return Plan(M, N, K, want_dx, want_dw).bytes.backward_temp +
+         std::max(want_dx ? Product(M, K, N).bytes() : 0, want_dw ? Product(N, K, M).bytes() : 0);
 }
 
 hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream) {
@@ -77,26 +87,27 @@ hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_
   GPUEXP_RETURN_IF(launch_quantize_fp8(a.x, a.type, a.ldx, a.M, a.K, kE4M3, 1, p.xq.out(x_at), {}, stream));
   GPUEXP_RETURN_IF(launch_quantize_fp8(a.w, a.wtype, a.ldw, a.N, a.K, kE4M3, kFp8Block, p.wq.out(a.temp),
                                        a.want_dx ? p.wt.out(a.kept) : Fp8Out{}, stream));
-  return gemm(p.xq.in(x_at), p.wq.in(a.temp), a.M, a.N, a.K, y, a.type, a.temp + p.forward_sums, stream);
+  return Product(a.M, a.N, a.K).run(p.xq.in(x_at), p.wq.in(a.temp), y, a.type, a.temp + p.bytes.forward_temp, stream);
 }
 
 hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
                                       hipStream_t stream) {
   const Plan p(a.M, a.N, a.K, a.want_dx, a.want_dw);
+  uint8_t* sums = a.temp + p.bytes.backward_temp;
   GPUEXP_RETURN_IF(launch_quantize_fp8(dy, a.type, lddy, a.M, a.N, kE4M3, 1,
                                        a.want_dx ? p.gq.out(a.temp) : Fp8Out{},
                                        a.want_dw ? p.gt.out(a.temp) : Fp8Out{}, stream));
   if (a.want_dx)
-    GPUEXP_RETURN_IF(gemm(p.gq.in(a.temp), p.wt.in(a.kept), a.M, a.K, a.N, dx, a.type, a.temp + p.backward_sums, stream));
+    GPUEXP_RETURN_IF(Product(a.M, a.K, a.N).run(p.gq.in(a.temp), p.wt.in(a.kept), dx, a.type, sums, stream));
   if (a.want_dw) {
     GPUEXP_RETURN_IF(launch_transpose_fp8(p.xq.in(a.kept), a.M, a.K, p.xt.out(a.temp), stream));
-    GPUEXP_RETURN_IF(gemm(p.gt.in(a.temp), p.xt.in(a.temp), a.N, a.K, a.M, dw, a.wtype, a.temp + p.backward_sums, stream));
+    GPUEXP_RETURN_IF(Product(a.N, a.K, a.M).run(p.gt.in(a.temp), p.xt.in(a.temp), dw, a.wtype, sums, stream));
   }
   return hipSuccess;
 }
 
 int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
-  return gemm_fp8_takes_wide(x, ldx, M, N, K) ? 0 : Piece{M, K, 0, 1}.end() + gemm_bytes(M, N, K);
+  return gemm_fp8_takes_wide(x, ldx, M, N, K) ? 0 : Piece{M, K, 0, 1}.end() + Product(M, N, K).bytes();
 }
 
 hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
@@ -104,7 +115,7 @@ hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64
   if (gemm_fp8_takes_wide(x, ldx, M, N, K)) return launch_gemm_fp8_wide(x, type, ldx, w, M, N, K, y, stream);
   const Piece xq{M, K, 0, 1};
   GPUEXP_RETURN_IF(launch_quantize_fp8(x, type, ldx, M, K, kE4M3, 1, xq.out(temp), {}, stream));
-  return gemm(xq.in(temp), w, M, N, K, y, type, temp + xq.end(), stream);
+  return Product(M, N, K).run(xq.in(temp), w, y, type, temp + xq.end(), stream);
 }
 
 }  // namespace gpuexp
