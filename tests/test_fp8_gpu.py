@@ -10,6 +10,7 @@ by less than 2^-13 of the largest, at most 2^-8 of the sum of magnitudes; over m
 have both signs, in norm they stay under 2^-13 (measured alone: 1.5e-5 < 2^-16)."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from kubernetes_gpu_exporter_amd.ops.fp8 import (dequantize_fp8, gemm_fp8, gemm_fp8_parts, gemm_fp8_variant,
                                                  linear_fp8, quantize_fp8, quantize_fp8_both, transpose_fp8)
@@ -466,6 +467,28 @@ def test_out_counts_as_changed():
     gemm_fp8(a, sa, a, sa, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         z.backward()
+
+
+def test_in_inference_mode_and_recomputed():
+    """Without autograd's records, and with a layer's forward pass run again for its backward pass."""
+    g = gen(5)
+    x, w = (torch.randn(s, device="cuda", generator=g).to(BF16).requires_grad_() for s in ((3, 40, 384), (200, 384)))
+    grad = torch.randn(3, 40, 200, device="cuda", generator=g).to(BF16)
+    y = linear_fp8(x, w)
+    want = torch.autograd.grad(y, (x, w), grad)
+    again = torch.utils.checkpoint.checkpoint(lambda a: torch.sin(linear_fp8(a, w)), x, use_reentrant=False)
+    got = torch.autograd.grad(again, (x, w), grad)
+    plain = torch.autograd.grad(torch.sin(linear_fp8(x, w)), (x, w), grad)
+    assert torch.equal(again, torch.sin(y)) and all(torch.equal(a, b) for a, b in zip(got, plain))
+    with torch.inference_mode():
+        pair_ = quantize_fp8(w, block_rows=128)
+        kept = quantize_fp8(x.reshape(120, 384))
+        out = torch.empty(120, 200, device="cuda", dtype=BF16)
+        assert gemm_fp8(*kept, *pair_, out=out) is not None and torch.equal(out.view(3, 40, 200), y)
+        assert torch.equal(linear_fp8(x, w), y) and torch.equal(linear_fp8(x, *pair_), y)
+    assert want[0].shape == x.shape and all(bool(t.isfinite().all()) for t in want)
+    with torch.enable_grad(), torch.autocast("cuda", dtype=BF16):
+        assert torch.equal(linear_fp8(x, w), y)
 
 
 def test_out_is_refused_where_it_cannot_be_written():
