@@ -13,6 +13,15 @@ enum Fp8Type { kE4M3 = 0, kE5M2 = 1 };               // also the matrix instruct
 enum WideType { kBF16 = 0, kF16 = 1, kF32 = 2 };     // types of 16 and 32 bits
 constexpr int kFp8Block = 128;
 
+// Bytes between the rows of a tensor of 8-bit values that this code lays out.  The kernels want multiples of
+// 16; where an eighth more memory is enough, rows start at lines of 128 bytes: a block of 128 values is then
+// one line, and no line is written by two blocks that share no cache (4112 x 4112 x 4112 112 -> 93 us,
+// 64 x 4000 x 5001 14.0 -> 12.2, the transpose of 4112 x 8208 27 -> 20).
+inline int64_t fp8_row_bytes(int64_t cols) {
+  const int64_t lines = (cols + 127) / 128 * 128;
+  return lines - cols <= cols / 8 ? lines : (cols + 15) / 16 * 16;
+}
+
 struct Fp8Out {  // a tensor in 8 bits to write; q == nullptr: not wanted
   uint8_t* q;
   uint8_t* scale;

@@ -116,9 +116,8 @@ Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType type) {
 
 Tensor bytes(int64_t n, const Tensor& like) { return empty({n}, like, at::kByte); }
 
-// [rows, cols] of 1-byte values whose rows start at multiples of `pad` bytes
-Tensor empty_rows(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int64_t pad) {
-  const int64_t ld = up(cols, pad);
+// [rows, cols] of 1-byte values whose rows start `ld` bytes apart
+Tensor empty_rows(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int64_t ld) {
   const Tensor t = empty({rows, ld}, like, type);
   return ld == cols ? t : t.narrow(1, 0, cols);
 }
@@ -128,10 +127,11 @@ struct Made {  // a tensor in 8 bits and where a kernel writes it
   Fp8Out out{};
   Made() = default;
   Made(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int block_rows)
-      : q(empty_rows(rows, cols, like, type, 16)),
-        scale(empty_rows((rows + block_rows - 1) / block_rows, blocks(cols), like, at::kFloat8_e8m0fnu, 4)),
-        out{static_cast<uint8_t*>(q.mutable_data_ptr()), static_cast<uint8_t*>(scale.mutable_data_ptr()), up(cols, 16),
-            up(blocks(cols), 4)} {}
+      : q(empty_rows(rows, cols, like, type, gpuexp::fp8_row_bytes(cols))),
+        scale(empty_rows((rows + block_rows - 1) / block_rows, blocks(cols), like, at::kFloat8_e8m0fnu,
+                         up(blocks(cols), 4))),
+        out{static_cast<uint8_t*>(q.mutable_data_ptr()), static_cast<uint8_t*>(scale.mutable_data_ptr()),
+            gpuexp::fp8_row_bytes(cols), up(blocks(cols), 4)} {}
 };
 
 std::pair<Made, Made> quantize(const Tensor& x, at::ScalarType dtype, int64_t block_rows, bool columns) {

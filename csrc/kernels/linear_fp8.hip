@@ -18,7 +18,7 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 struct Piece {
   int64_t rows, cols, at;
   int block_rows;
-  int64_t ld() const { return up(cols, 16); }
+  int64_t ld() const { return fp8_row_bytes(cols); }
   int64_t lds() const { return up(up(cols, kFp8Block) / kFp8Block, 4); }
   int64_t scales_at() const { return at + up(rows * ld(), 256); }
   int64_t end() const { return scales_at() + up(up(rows, block_rows) / block_rows * lds(), 256); }

@@ -7,7 +7,8 @@ columns and 1 row (activations, gradients: scale [rows, ceil(cols/128)]) or 128 
 scale [ceil(rows/128), ceil(cols/128)]).  q[i, j] stands for q * scale of its block.  A block's
 scale is the smallest 2^e, e >= -127, that brings its largest finite magnitude to at most the
 type's largest value (448 or 57344); each value is rounded once, to nearest even.  Rows of q start
-at multiples of 16 bytes and rows of scale at multiples of 4: the functions here make them so.
+at multiples of 16 bytes and rows of scale at multiples of 4: the functions here make them so, q's
+at multiples of 128 where that takes at most an eighth more memory (q is then a view of wider rows).
 
   quantize_fp8 / dequantize_fp8   an activation checkpoint in 8 bits, kept and given back
   transpose_fp8                   the same checkpoint by columns: the gradient of a weight reads it so
