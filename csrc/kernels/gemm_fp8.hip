@@ -814,8 +814,8 @@ namespace {
 // of K (`nk`) for each round of 256 blocks, whose slope grows with the part of the card that loads at
 // once.  In parts there is a second kernel and its bytes, and 1 us for a launch and a workspace more.
 // The numbers are those of 600 random sizes (1 to 8192 x 64 to 16384 x 128 to 16384, B in the caches and
-// from memory) with which the choice costs least: on 400 others 0.7 % (caches) and 1.2 % (memory) against
-// the fastest kernel in the mean.  Examples,
+// from memory) with which the choice costs least: on 520 others 0.6 % against the fastest kernel in the
+// mean, up to 16 rows 1.3 %.  Examples,
 // B from memory, us:                          128 x 128   two per CU   256 x 256   64 x 64
 //   256 x 4096 x 4096                          21.9        30.3         42.7        12.1
 //   1024 x 4096 x 4096                         23.1        31.4         42.4        33.6

@@ -179,6 +179,15 @@ def test_quantize_strided_and_unaligned_rows(offset, ld, xdtype):
     same(values(q, s), want)
 
 
+@pytest.mark.parametrize("cols,ld", [(1, 16), (16, 16), (100, 112), (120, 128), (128, 128), (900, 912), (1001, 1024),
+                                     (1024, 1024), (5000, 5120)])
+def test_rows_start_at_lines_where_that_is_cheap(cols, ld):
+    x = torch.randn(3, cols, device="cuda")
+    for q in (quantize_fp8(x)[0], quantize_fp8(x, block_rows=128)[0], quantize_fp8_both(x)[0][0],
+              quantize_fp8_both(x.T.contiguous())[1][0], transpose_fp8(*quantize_fp8(x.T.contiguous()))[0]):
+        assert tuple(q.shape) == (3, cols) and q.stride() == (ld, 1)
+
+
 def exact_product(a, sa, b, sb):
     return values(a, sa) @ values(b, sb).T
 
