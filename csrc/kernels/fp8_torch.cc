@@ -1,6 +1,8 @@
 // torch bindings of the 8-bit operators: checks of arguments, allocation, autograd.  In C++ because a
 // small call is bound by the host: the launches of a training step take 20 us, its Python took 100.
 // Tensors come in and go out as torch tensors, work goes to torch's current stream of their device.
+// The operators are torch.ops.gpuexp's, and Python calls them through torch's dispatcher: what records a
+// program (torch.jit.trace, make_fx) then records the operator, not the empty tensors that it fills.
 // The documentation is in ops/fp8.py.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -8,6 +10,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/library.h>
 
 #include <optional>
 #include <tuple>
@@ -23,6 +26,7 @@ using gpuexp::kFp8Block;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using Pair = std::tuple<Tensor, Tensor>;
+using Four = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
@@ -158,9 +162,9 @@ Pair quantize_fp8(const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
   return {std::move(out.q), std::move(out.scale)};
 }
 
-std::tuple<Pair, Pair> quantize_fp8_both(const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
+Four quantize_fp8_both(const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
   auto [out, out_t] = quantize(x, dtype, block_rows, true);
-  return {Pair{std::move(out.q), std::move(out.scale)}, Pair{std::move(out_t.q), std::move(out_t.scale)}};
+  return {std::move(out.q), std::move(out.scale), std::move(out_t.q), std::move(out_t.scale)};
 }
 
 Tensor dequantize_fp8(const Tensor& q, const Tensor& scale, at::ScalarType dtype) {
@@ -186,8 +190,8 @@ Pair transpose_fp8(const Tensor& q, const Tensor& scale) {
   return {std::move(out.q), std::move(out.scale)};
 }
 
-Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
-                const std::optional<Tensor>& given, at::ScalarType out_dtype, int64_t variant, int64_t parts) {
+Tensor product(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, const Tensor* given,
+               at::ScalarType out_dtype, int64_t variant, int64_t parts) {
   const Fp8In oa = operand("a", a, a_scale), ob = operand("b", b, b_scale);
   const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
   TORCH_CHECK_VALUE(b.size(1) == K, "shape mismatch ", a.sizes(), " x ", b.sizes(), "^T");
@@ -222,10 +226,32 @@ Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
   return out;
 }
 
+Tensor gemm_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
+                at::ScalarType out_dtype, int64_t variant, int64_t parts) {
+  return product(a, a_scale, b, b_scale, nullptr, out_dtype, variant, parts);
+}
+
+void gemm_fp8_out(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, const Tensor& out,
+                  int64_t variant, int64_t parts) {
+  product(a, a_scale, b, b_scale, &out, out.scalar_type(), variant, parts);
+}
+
 Tensor rows_of(const Tensor& x) { return row_major(x) ? x : x.contiguous(); }
 
+// what a layer's passes take: x [M, K] and w [N, K] as checked_linear passes them on
+void check_layer(const Tensor& x, at::ScalarType wtype) {
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+                   "linear_fp8 takes bfloat16 or float16 activations, got ", x.scalar_type());
+  TORCH_CHECK_TYPE(wtype == at::kBFloat16 || wtype == at::kHalf,
+                   "linear_fp8 takes bfloat16 or float16 weights, or 8-bit ones with weight_scale, got ", wtype);
+}
+
 // y = x w^T of x [M, K], w [N, K] and the workspace that the backward pass needs
-std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& w, bool want_dx, bool want_dw) {
+Pair linear_fp8_forward(const Tensor& x, const Tensor& w, bool want_dx, bool want_dw) {
+  check_layer(x, w.scalar_type());
+  check_gpu("linear_fp8", x, w);
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && row_major(x) && row_major(w),
+                    "linear_fp8_forward takes row-major x [M, K] and w [N, K], got ", x.sizes(), " and ", w.sizes());
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const On on(x);
   Tensor y = empty({M, N}, x, x.scalar_type()),
@@ -235,56 +261,33 @@ std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& w, bool want_dx
                           wide_stride(w), wide_type(x.scalar_type()), wide_type(w.scalar_type()),
                           static_cast<uint8_t*>(kept.mutable_data_ptr()), static_cast<uint8_t*>(temp.mutable_data_ptr())};
   check(gpuexp::launch_linear_fp8_forward(a, y.mutable_data_ptr(), on.stream), "linear_fp8");
-  return {y, kept};
+  return {std::move(y), std::move(kept)};
 }
 
-variable_list once(variable_list results) {
-  // Gradients of gradients are refused where they are asked for, not where the first ones are made; also for a
-  // constant dy, since dx depends on the weight and dw on x.
-  if (!at::GradMode::is_enabled()) return results;
-  for (Tensor& t : results) {  // DelayedError hangs its refusal only on tensors that take a gradient
-    if (t.defined()) t.set_requires_grad(true);
-  }
-  auto error = std::make_shared<torch::autograd::DelayedError>("linear_fp8 cannot be differentiated twice",
-                                                               int(results.size()));
-  return (*error)(std::move(results));
+// (dx, dw) of dy [M, N] and what the forward pass kept; one that is not wanted is undefined
+Pair linear_fp8_backward(const Tensor& given, const Tensor& kept, int64_t K, at::ScalarType wtype, bool want_dx,
+                         bool want_dw) {
+  const Tensor dy = rows_of(given);
+  check_layer(dy, wtype);
+  check_gpu("linear_fp8", dy, kept);
+  const int64_t M = dy.size(0), N = dy.size(1);
+  TORCH_CHECK_VALUE(dy.dim() == 2 && kept.scalar_type() == at::kByte && kept.is_contiguous() &&
+                        kept.numel() == gpuexp::linear_fp8_kept_bytes(M, N, K, want_dx, want_dw),
+                    "linear_fp8_backward: what was kept is not of these sizes");
+  const On on(dy);
+  Tensor dx, dw;
+  if (want_dx) dx = empty({M, K}, dy, dy.scalar_type());
+  if (want_dw) dw = empty({N, K}, dy, wtype);
+  const Tensor temp = bytes(gpuexp::linear_fp8_backward_bytes(M, N, K, want_dx, want_dw), dy);
+  gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, nullptr, 0, nullptr, 0, wide_type(dy.scalar_type()),
+                          wide_type(wtype), static_cast<uint8_t*>(kept.mutable_data_ptr()),
+                          static_cast<uint8_t*>(temp.mutable_data_ptr())};
+  check(gpuexp::launch_linear_fp8_backward(a, dy.const_data_ptr(), wide_stride(dy),
+                                           want_dx ? dx.mutable_data_ptr() : nullptr,
+                                           want_dw ? dw.mutable_data_ptr() : nullptr, on.stream),
+        "linear_fp8's backward pass");
+  return {std::move(dx), std::move(dw)};
 }
-
-struct LinearFp8 : torch::autograd::Function<LinearFp8> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
-    const bool want_dx = x.requires_grad(), want_dw = w.requires_grad();
-    auto [y, kept] = ::forward(x, w, want_dx, want_dw);
-    ctx->save_for_backward({kept});
-    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), w.size(0), x.size(1), want_dx, want_dw,
-                                                    int64_t(w.scalar_type())};
-    return y;
-  }
-
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor kept = ctx->get_saved_variables()[0];
-    const std::vector<int64_t> s = ctx->saved_data["sizes"].toIntVector();
-    const int64_t M = s[0], N = s[1], K = s[2];
-    const bool want_dx = s[3], want_dw = s[4];
-    const auto wtype = at::ScalarType(s[5]);
-    variable_list results(2);
-    {
-      at::AutoGradMode off(false);
-      const Tensor dy = rows_of(grads[0]);
-      const On on(dy);
-      if (want_dx) results[0] = empty({M, K}, dy, dy.scalar_type());
-      if (want_dw) results[1] = empty({N, K}, dy, wtype);
-      const Tensor temp = bytes(gpuexp::linear_fp8_backward_bytes(M, N, K, want_dx, want_dw), dy);
-      gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, nullptr, 0, nullptr, 0, wide_type(dy.scalar_type()),
-                              wide_type(wtype), static_cast<uint8_t*>(kept.mutable_data_ptr()),
-                              static_cast<uint8_t*>(temp.mutable_data_ptr())};
-      check(gpuexp::launch_linear_fp8_backward(a, dy.const_data_ptr(), wide_stride(dy),
-                                               want_dx ? results[0].mutable_data_ptr() : nullptr,
-                                               want_dw ? results[1].mutable_data_ptr() : nullptr, on.stream),
-            "linear_fp8's backward pass");
-    }
-    return once(std::move(results));
-  }
-};
 
 Tensor serve(const Tensor& x, const Tensor& w, const Tensor& scale) {
   const Fp8In in = operand("weight", w, scale);
@@ -301,59 +304,147 @@ Tensor serve(const Tensor& x, const Tensor& w, const Tensor& scale) {
   return y;
 }
 
+// the checks of a layer's arguments, and x's rows [M, K]
+Tensor checked_linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& scale, bool want_dx,
+                      bool want_dw) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1), "shape mismatch ", x.sizes(),
+                    " x ", weight.sizes(), "^T");
+  check_layer(x, scale ? x.scalar_type() : weight.scalar_type());
+  if (scale) {
+    TORCH_CHECK_VALUE(!weight.requires_grad(), "weights in 8 bits take no gradient");
+    operand("weight", weight, *scale);
+    check_gpu("linear_fp8", x, weight, *scale);
+  } else {
+    check_gpu("linear_fp8", x, weight);
+  }
+  const int64_t K = x.size(-1);
+  int64_t M = 1;
+  for (int64_t d = 0; d < x.dim() - 1; ++d) M *= x.size(d);
+  TORCH_CHECK_VALUE(K <= kLongest && (!want_dx || weight.size(0) <= kLongest) && (!want_dw || M <= kLongest),
+                    "linear_fp8: at most ", kLongest, " inputs, for x's gradient as many outputs and for the weight's as "
+                    "many rows of x, got ", K, ", ", weight.size(0), " and ", M);
+  return rows_of(x.dim() == 2 ? x : x.reshape({M, K}));
+}
+
+Tensor as_given(const Tensor& y, const Tensor& x) {
+  if (x.dim() == 2) return y;
+  std::vector<int64_t> size(x.sizes().begin(), x.sizes().end());
+  size.back() = y.size(1);
+  return y.reshape(size);
+}
+
+// without autograd
+Tensor linear_fp8(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& scale) {
+  const Tensor x2 = checked_linear(x, weight, scale, false, false);
+  return as_given(scale ? serve(x2, weight, *scale) : std::get<0>(linear_fp8_forward(x2, rows_of(weight), false, false)), x);
+}
+
+// ---- the operators through torch's dispatcher ----
+template <typename F>
+c10::TypedOperatorHandle<F> find(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+#define GPUEXP_CALL(op, ...)                            \
+  ([&] {                                                \
+    static const auto handle = find("gpuexp::" #op, op); \
+    return handle.call(__VA_ARGS__);                    \
+  }())
+
+variable_list once(variable_list results) {
+  // Gradients of gradients are refused where they are asked for, not where the first ones are made; also for a
+  // constant dy, since dx depends on the weight and dw on x.
+  if (!at::GradMode::is_enabled()) return results;
+  for (Tensor& t : results) {  // DelayedError hangs its refusal only on tensors that take a gradient
+    if (t.defined()) t.set_requires_grad(true);
+  }
+  auto error = std::make_shared<torch::autograd::DelayedError>("linear_fp8 cannot be differentiated twice",
+                                                               int(results.size()));
+  return (*error)(std::move(results));
+}
+
+struct LinearFp8 : torch::autograd::Function<LinearFp8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+    const bool want_dx = x.requires_grad(), want_dw = w.requires_grad();
+    auto [y, kept] = GPUEXP_CALL(linear_fp8_forward, x, w, want_dx, want_dw);
+    ctx->save_for_backward({kept});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(1), want_dx, want_dw, int64_t(w.scalar_type())};
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor kept = ctx->get_saved_variables()[0];
+    const std::vector<int64_t> s = ctx->saved_data["sizes"].toIntVector();
+    variable_list results(2);
+    {
+      at::AutoGradMode off(false);
+      std::tie(results[0], results[1]) =
+          GPUEXP_CALL(linear_fp8_backward, grads[0], kept, s[0], at::ScalarType(s[3]), s[1] != 0, s[2] != 0);
+    }
+    return once(std::move(results));
+  }
+};
+
 struct ServeFp8 : torch::autograd::Function<ServeFp8> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& scale) {
     ctx->save_for_backward({w, scale});
-    return serve(x, w, scale);
+    return GPUEXP_CALL(linear_fp8, x, w, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     variable_list results(3);
     {
       at::AutoGradMode off(false);
-      const auto [g, g_scale] = quantize_fp8(rows_of(grads[0]), at::kFloat8_e4m3fn, 1);
-      const auto [wt, wt_scale] = transpose_fp8(saved[0], saved[1]);
-      results[0] = gemm_fp8(g, g_scale, wt, wt_scale, std::nullopt, grads[0].scalar_type(), 0, 0);
+      const auto [g, g_scale] = GPUEXP_CALL(quantize_fp8, rows_of(grads[0]), at::kFloat8_e4m3fn, 1);
+      const auto [wt, wt_scale] = GPUEXP_CALL(transpose_fp8, saved[0], saved[1]);
+      results[0] = GPUEXP_CALL(gemm_fp8, g, g_scale, wt, wt_scale, grads[0].scalar_type(), 0, 0);
     }
     return once(std::move(results));
   }
 };
 
-Tensor linear_fp8(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& scale) {
-  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1), "shape mismatch ", x.sizes(),
-                    " x ", weight.sizes(), "^T");
-  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
-                   "linear_fp8 takes bfloat16 or float16 activations, got ", x.scalar_type());
-  if (scale) {
-    TORCH_CHECK_VALUE(!weight.requires_grad(), "weights in 8 bits take no gradient");
-    operand("weight", weight, *scale);
-    check_gpu("linear_fp8", x, weight, *scale);
-  } else {
-    TORCH_CHECK_TYPE(weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kHalf,
-                     "linear_fp8 takes bfloat16 or float16 weights, or 8-bit ones with weight_scale, got ",
-                     weight.scalar_type());
-    check_gpu("linear_fp8", x, weight);
-  }
-  const int64_t K = x.size(-1);
-  int64_t M = 1;
-  for (int64_t d = 0; d < x.dim() - 1; ++d) M *= x.size(d);
-  const Tensor x2 = rows_of(x.dim() == 2 ? x : x.reshape({M, K}));
-  const bool grad = at::GradMode::is_enabled(), want_dx = grad && x2.requires_grad(),
+Tensor linear_fp8_autograd(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& scale) {
+  const bool grad = at::GradMode::is_enabled(), want_dx = grad && x.requires_grad(),
              want_dw = grad && weight.requires_grad();
-  TORCH_CHECK_VALUE(K <= kLongest && (!want_dx || weight.size(0) <= kLongest) && (!want_dw || M <= kLongest),
-                    "linear_fp8: at most ", kLongest, " inputs, for x's gradient as many outputs and for the weight's as "
-                    "many rows of x, got ", K, ", ", weight.size(0), " and ", M);
-  Tensor y;
-  if (scale) {
-    y = want_dx ? ServeFp8::apply(x2, weight, *scale) : serve(x2, weight, *scale);
-  } else {
-    const Tensor w2 = rows_of(weight);
-    y = want_dx || want_dw ? LinearFp8::apply(x2, w2) : forward(x2, w2, false, false).first;
+  if (!want_dx && !want_dw) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return GPUEXP_CALL(linear_fp8, x, weight, scale);
   }
-  if (x.dim() == 2) return y;
-  std::vector<int64_t> size(x.sizes().begin(), x.sizes().end());
-  size.back() = weight.size(0);
-  return y.reshape(size);
+  const Tensor x2 = checked_linear(x, weight, scale, want_dx, want_dw);
+  return as_given(scale ? ServeFp8::apply(x2, weight, *scale) : LinearFp8::apply(x2, rows_of(weight)), x);
+}
+
+TORCH_LIBRARY(gpuexp, m) {
+  m.def("quantize_fp8(Tensor x, ScalarType dtype, int block_rows) -> (Tensor, Tensor)");
+  m.def("quantize_fp8_both(Tensor x, ScalarType dtype, int block_rows) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("dequantize_fp8(Tensor q, Tensor scale, ScalarType dtype) -> Tensor");
+  m.def("transpose_fp8(Tensor q, Tensor scale) -> (Tensor, Tensor)");
+  m.def("gemm_fp8(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, ScalarType out_dtype, int variant, int parts) "
+        "-> Tensor");
+  m.def("gemm_fp8_out(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, Tensor(a!) out, int variant, int parts) -> ()");
+  m.def("linear_fp8(Tensor x, Tensor weight, Tensor? weight_scale) -> Tensor");
+  m.def("linear_fp8_forward(Tensor x, Tensor weight, bool want_dx, bool want_dw) -> (Tensor, Tensor)");
+  m.def("linear_fp8_backward(Tensor dy, Tensor kept, int inputs, ScalarType weight_dtype, bool want_dx, bool want_dw) "
+        "-> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(gpuexp, CompositeExplicitAutograd, m) {
+  m.impl("quantize_fp8", quantize_fp8);
+  m.impl("quantize_fp8_both", quantize_fp8_both);
+  m.impl("dequantize_fp8", dequantize_fp8);
+  m.impl("transpose_fp8", transpose_fp8);
+  m.impl("gemm_fp8", gemm_fp8);
+  m.impl("gemm_fp8_out", gemm_fp8_out);
+  m.impl("linear_fp8", linear_fp8);
+  m.impl("linear_fp8_forward", linear_fp8_forward);
+  m.impl("linear_fp8_backward", linear_fp8_backward);
+}
+
+TORCH_LIBRARY_IMPL(gpuexp, Autograd, m) {
+  m.impl("linear_fp8", linear_fp8_autograd);
+  // the others take no part in autograd
+  for (const char* name : {"quantize_fp8", "quantize_fp8_both", "dequantize_fp8", "transpose_fp8", "gemm_fp8",
+                           "gemm_fp8_out", "linear_fp8_forward", "linear_fp8_backward"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 }  // namespace
@@ -361,12 +452,26 @@ Tensor linear_fp8(const Tensor& x, const Tensor& weight, const std::optional<Ten
 // Loaded after torch, whose HIP runtime it then shares (see ops/gemm.py).
 PYBIND11_MODULE(_gpuexp_fp8, m) {
   m.doc() = "8-bit floating point with block scales on torch tensors (ops/fp8.py)";
-  m.def("quantize_fp8", &quantize_fp8);
-  m.def("quantize_fp8_both", &quantize_fp8_both);
-  m.def("dequantize_fp8", &dequantize_fp8);
-  m.def("transpose_fp8", &transpose_fp8);
-  m.def("gemm_fp8", &gemm_fp8);
-  m.def("linear_fp8", &linear_fp8);
+  m.def("quantize_fp8", [](const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
+    return GPUEXP_CALL(quantize_fp8, x, dtype, block_rows);
+  });
+  m.def("quantize_fp8_both", [](const Tensor& x, at::ScalarType dtype, int64_t block_rows) {
+    auto [q, scale, q_t, scale_t] = GPUEXP_CALL(quantize_fp8_both, x, dtype, block_rows);
+    return std::make_tuple(Pair{std::move(q), std::move(scale)}, Pair{std::move(q_t), std::move(scale_t)});
+  });
+  m.def("dequantize_fp8", [](const Tensor& q, const Tensor& scale, at::ScalarType dtype) {
+    return GPUEXP_CALL(dequantize_fp8, q, scale, dtype);
+  });
+  m.def("transpose_fp8", [](const Tensor& q, const Tensor& scale) { return GPUEXP_CALL(transpose_fp8, q, scale); });
+  m.def("gemm_fp8", [](const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
+                       const std::optional<Tensor>& out, at::ScalarType out_dtype, int64_t variant, int64_t parts) {
+    if (!out) return GPUEXP_CALL(gemm_fp8, a, a_scale, b, b_scale, out_dtype, variant, parts);
+    GPUEXP_CALL(gemm_fp8_out, a, a_scale, b, b_scale, *out, variant, parts);
+    return *out;
+  });
+  m.def("linear_fp8", [](const Tensor& x, const Tensor& weight, const std::optional<Tensor>& weight_scale) {
+    return GPUEXP_CALL(linear_fp8, x, weight, weight_scale);
+  });
   m.def("gemm_fp8_plan", [](int64_t M, int64_t N, int64_t K, int variant, int parts) {
     const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, variant, parts);
     return std::make_pair(plan.variant, plan.parts);

@@ -22,7 +22,9 @@ Everything runs on torch's current stream of the tensors' device, or on `stream`
 in ops.gemm): then results are allocated on that stream, the inputs are kept from reuse until it
 is done with them, and ordering against other streams is the caller's.  All calls can be captured
 into a graph; linear_fp8's backward pass too, as any torch backward pass, only while no eager
-graph of the same leaves is alive.
+graph of the same leaves is alive.  To torch they are operators (torch.ops.gpuexp), so torch.jit.trace
+and make_fx record them as such; a traced linear_fp8 has its gradients.  torch.compile runs them between
+its graphs.
 """
 from __future__ import annotations
 

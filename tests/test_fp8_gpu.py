@@ -757,3 +757,57 @@ def test_fp8_trainer_pod_on_gpu(tmp_path):
     half = torch.finfo(BF16).eps / 2
     for got, want in zip(p.grads, (dx, dw)):
         assert float((got.double() - want).norm()) <= (half + 2.0 ** -13) * float(want.norm())
+
+
+PROGRAMS = {
+    "checkpoint": lambda x, w, wq, ws: dequantize_fp8(*transpose_fp8(*quantize_fp8(x))),
+    "both": lambda x, w, wq, ws: dequantize_fp8(*quantize_fp8_both(x)[1]),
+    "gemm": lambda x, w, wq, ws: gemm_fp8(*quantize_fp8(x), wq, ws),
+    "gemm_out": lambda x, w, wq, ws: gemm_fp8(*quantize_fp8(x), wq, ws, out=torch.empty(x.shape[0], wq.shape[0], dtype=BF16,
+                                                                                        device=x.device)),
+    "serve": lambda x, w, wq, ws: linear_fp8(x, wq, ws),
+    "layer": lambda x, w, wq, ws: linear_fp8(x, w),
+}
+
+
+@pytest.mark.parametrize("name", PROGRAMS)
+@pytest.mark.parametrize("tracer", ["jit", "fx"])
+def test_traced_programs_compute(name, tracer):
+    """A recorded program holds the operators themselves, not the memory that one recorded call wrote."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    g = gen(31)
+    w = torch.randn(96, 320, device="cuda", generator=g).to(BF16)
+    x, other = (torch.randn(40, 320, device="cuda", generator=g).to(BF16) for _ in range(2))
+    held = (w, *quantize_fp8(w, block_rows=128))
+    want = [PROGRAMS[name](t, *held) for t in (x, other)]
+    program = lambda t: PROGRAMS[name](t, *held)  # noqa: E731
+    traced = torch.jit.trace(program, (x,), check_trace=False) if tracer == "jit" else make_fx(program)(x)
+    for t, ref in ((x, want[0]), (other, want[1]), (x, want[0])):
+        assert torch.equal(traced(t), ref)
+
+
+def test_traced_training_steps_compute():
+    """The gradients of a traced layer, and a traced step with its backward pass."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    g = gen(32)
+    w = torch.randn(96, 320, device="cuda", generator=g).to(BF16)
+    x, other = (torch.randn(40, 320, device="cuda", generator=g).to(BF16) for _ in range(2))
+    grad = torch.randn(40, 96, device="cuda", generator=g).to(BF16)
+    wq, ws = quantize_fp8(w, block_rows=128)
+
+    def train(a, b, c):
+        return step(a.detach().requires_grad_(), b.detach().requires_grad_(), c)
+
+    def serve(a, c):
+        a = a.detach().requires_grad_()
+        y = linear_fp8(a, wq, ws)
+        return y.detach(), torch.autograd.grad(y, a, c)[0]
+    layer = torch.jit.trace(lambda a, b: linear_fp8(a, b), (x, w), check_trace=False)
+    train_fx, serve_fx = make_fx(train)(x, w, grad), make_fx(serve)(x, grad)
+    for t in (x, other):
+        want = train(t, w, grad)
+        a, b = t.detach().requires_grad_(), w.detach().requires_grad_()
+        y = layer(a, b)
+        for got in ((y.detach(), *torch.autograd.grad(y, (a, b), grad)), train_fx(t, w, grad)):
+            assert all(torch.equal(p, r) for p, r in zip(got, want))
+        assert all(torch.equal(p, r) for p, r in zip(serve_fx(t, grad), serve(t, grad)))
