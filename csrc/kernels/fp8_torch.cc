@@ -402,7 +402,15 @@ struct ServeFp8 : torch::autograd::Function<ServeFp8> {
   }
 };
 
+// (below autograd the tangent would be dropped without a word)
+void check_no_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
+                              "linear_fp8 has no forward-mode derivative");
+}
+
 Tensor linear_fp8_autograd(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& scale) {
+  check_no_tangent(x);
+  check_no_tangent(weight);
   const bool grad = at::GradMode::is_enabled(), want_dx = grad && x.requires_grad(),
              want_dw = grad && weight.requires_grad();
   if (!want_dx && !want_dw) {

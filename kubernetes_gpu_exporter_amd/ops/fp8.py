@@ -125,7 +125,7 @@ def linear_fp8(x, weight, weight_scale=None):
     Training: `weight` in bf16 or f16.  Both operands are quantised to e4m3 (x in blocks of 1 x 128,
     the weight 128 x 128).  For the backward pass x is kept as its 8-bit checkpoint, half the memory
     of the activation; dx = Q(dy) W with the kept 8-bit weight, dW = Q(dy^T) x with the checkpoint
-    transposed (as transpose_fp8 does).  A double backward is refused.  K is at most 2^22, and so is N
+    transposed (as transpose_fp8 does).  A double backward and forward-mode derivatives are refused.  K is at most 2^22, and so is N
     where x takes a gradient and the number of x's rows where the weight takes one.
 
     Serving: `weight` in 8 bits with its `weight_scale`, as quantize_fp8(w, block_rows=128) gives

@@ -147,3 +147,18 @@ def test_gemm_variant_resolution(M, N, K, variant, want):
     (64, 1024, 2048, 1), (64, 64, 0, 1), (0, 64, 8192, 1), (8192, 8192, 8192, 1)])
 def test_gemm_parts_of_k(M, N, K, parts):
     assert gemm_fp8_parts(M, N, K) == parts
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_forward_mode_is_refused(reverse):
+    """Also where no reverse-mode gradient is recorded, and under no_grad, which does not stop forward mode."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w = torch.zeros(4, 128).bfloat16(), torch.zeros(8, 128).bfloat16().requires_grad_(reverse)
+    wq, ws = q(256, 128, 128)
+    with forward_ad.dual_level():
+        for call in (lambda: linear_fp8(forward_ad.make_dual(x, x), w), lambda: linear_fp8(forward_ad.make_dual(x, x), wq, ws),
+                     lambda: linear_fp8(x, forward_ad.make_dual(w, torch.zeros_like(w)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -811,3 +811,15 @@ def test_traced_training_steps_compute():
         for got in ((y.detach(), *torch.autograd.grad(y, (a, b), grad)), train_fx(t, w, grad)):
             assert all(torch.equal(p, r) for p, r in zip(got, want))
         assert all(torch.equal(p, r) for p, r in zip(serve_fx(t, grad), serve(t, grad)))
+
+
+def test_forward_mode_is_refused_on_gpu():
+    import torch.autograd.forward_ad as forward_ad
+    x, w = (torch.randn(8, 128, device="cuda").to(BF16) for _ in range(2))
+    wq, ws = quantize_fp8(w, block_rows=128)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: linear_fp8(dual, w), lambda: linear_fp8(dual, wq, ws), lambda: linear_fp8(x, forward_ad.make_dual(w, x))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert torch.equal(linear_fp8(x, w), linear_fp8(x, w.clone()))
