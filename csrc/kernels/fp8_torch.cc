@@ -64,22 +64,29 @@ void check_gpu(const char* name, const Tensor& t) {
   TORCH_CHECK_VALUE(t.device().is_cuda(), name, ": tensors must be on the same GPU, got ", t.device());
 }
 
-// bytes between the rows of a 1-byte tensor [rows, cols] whose rows start at multiples of `pad`
-int64_t row_stride(const char* name, const char* of, const Tensor& t, int64_t rows, int64_t cols, int64_t pad) {
-  if (!rows || !cols) return up(cols, pad);
-  TORCH_CHECK_VALUE(cols == 1 || t.stride(1) == 1, of, name, " must have its columns next to each other, got strides ",
-                    t.strides());
-  const int64_t ld = rows == 1 ? up(cols, pad) : t.stride(0);
-  const int64_t off = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % pad;
-  TORCH_CHECK_VALUE(ld % pad == 0 && ld >= cols && off == 0, of, name, "'s rows must start at multiples of ", pad,
-                    " bytes and not overlap (row stride ", ld, ", address % ", pad, " = ", off,
-                    "); quantize_fp8 makes such tensors");
-  return ld;
+// A 1-byte tensor [rows, cols] whose rows start at multiples of `pad`: the bytes between them.
+struct Rows {
+  bool columns_ok, ok;
+  int64_t ld, off;
+  Rows(const Tensor& t, int64_t pad) : columns_ok(true), ok(true), ld(up(t.size(1), pad)), off(0) {
+    if (!t.numel()) return;  // (an empty view may have any address)
+    columns_ok = t.size(1) == 1 || t.stride(1) == 1;
+    if (t.size(0) > 1) ld = t.stride(0);
+    off = int64_t(reinterpret_cast<uintptr_t>(t.const_data_ptr()) % pad);
+    ok = columns_ok && ld % pad == 0 && ld >= t.size(1) && off == 0;
+  }
+};
+int64_t row_stride(const char* name, const char* of, const Tensor& t, int64_t pad) {
+  const Rows r(t, pad);
+  TORCH_CHECK_VALUE(r.columns_ok, of, name, " must have its columns next to each other, got strides ", t.strides());
+  TORCH_CHECK_VALUE(r.ok, of, name, "'s rows must start at multiples of ", pad, " bytes and not overlap (row stride ", r.ld,
+                    ", address % ", pad, " = ", r.off, "); quantize_fp8 makes such tensors, align_fp8 lays out copies");
+  return r.ld;
 }
 
-Fp8In operand(const char* name, const Tensor& q, const Tensor& scale) {
-  const int type = fp8_type(q.scalar_type());
-  TORCH_CHECK_TYPE(type >= 0, name, " must be float8_e4m3fn or float8_e5m2, got ", q.scalar_type());
+// the checks of types and sizes: whether (q, scale) has blocks of 1 x 128
+bool check_pair(const char* name, const Tensor& q, const Tensor& scale) {
+  TORCH_CHECK_TYPE(fp8_type(q.scalar_type()) >= 0, name, " must be float8_e4m3fn or float8_e5m2, got ", q.scalar_type());
   TORCH_CHECK_TYPE(scale.scalar_type() == at::kFloat8_e8m0fnu, "the scales of ", name, " must be float8_e8m0fnu, got ",
                    scale.scalar_type());
   TORCH_CHECK_VALUE(q.dim() == 2 && scale.dim() == 2, name, " and its scales must be 2-dimensional, got ", q.sizes(),
@@ -89,9 +96,14 @@ Fp8In operand(const char* name, const Tensor& q, const Tensor& scale) {
   TORCH_CHECK_VALUE(scale.size(1) == nb && (per_row || scale.size(0) == blocks(rows)), "the scales of ", name, " ",
                     q.sizes(), " must be [", rows, ", ", nb, "] (blocks of 1 x 128) or [", blocks(rows), ", ", nb,
                     "] (128 x 128), got ", scale.sizes());
-  Fp8In in{nullptr, nullptr, row_stride(name, "", q, rows, cols, 16),
-           row_stride(name, "the scales of ", scale, scale.size(0), nb, 4), per_row ? 1 : kFp8Block, type};
-  if (rows && cols) {  // (an empty view may have any address)
+  return per_row;
+}
+
+Fp8In operand(const char* name, const Tensor& q, const Tensor& scale) {
+  const bool per_row = check_pair(name, q, scale);
+  Fp8In in{nullptr, nullptr, row_stride(name, "", q, 16), row_stride(name, "the scales of ", scale, 4),
+           per_row ? 1 : kFp8Block, fp8_type(q.scalar_type())};
+  if (q.numel()) {
     in.q = static_cast<const uint8_t*>(q.const_data_ptr());
     in.scale = static_cast<const uint8_t*>(scale.const_data_ptr());
   }
@@ -137,6 +149,19 @@ struct Made {  // a tensor in 8 bits and where a kernel writes it
         out{static_cast<uint8_t*>(q.mutable_data_ptr()), static_cast<uint8_t*>(scale.mutable_data_ptr()),
             gpuexp::fp8_row_bytes(cols), up(blocks(cols), 4)} {}
 };
+
+// (q, scale) with rows that start where the kernels want them: what does already is given back as it is
+Pair align_fp8(const Tensor& q, const Tensor& scale) {
+  check_pair("q", q, scale);
+  const at::NoGradGuard none;
+  const auto aligned = [](const Tensor& t, int64_t pad, int64_t ld) {
+    if (Rows(t, pad).ok) return t;
+    const Tensor rows = empty_rows(t.size(0), t.size(1), t, t.scalar_type(), ld);
+    rows.copy_(t);
+    return rows;
+  };
+  return {aligned(q, 16, gpuexp::fp8_row_bytes(q.size(1))), aligned(scale, 4, up(scale.size(1), 4))};
+}
 
 std::pair<Made, Made> quantize(const Tensor& x, at::ScalarType dtype, int64_t block_rows, bool columns) {
   TORCH_CHECK_TYPE(fp8_type(dtype) >= 0, "quantize_fp8 makes float8_e4m3fn or float8_e5m2, not ", dtype);
@@ -470,6 +495,7 @@ PYBIND11_MODULE(_gpuexp_fp8, m) {
   m.def("dequantize_fp8", [](const Tensor& q, const Tensor& scale, at::ScalarType dtype) {
     return GPUEXP_CALL(dequantize_fp8, q, scale, dtype);
   });
+  m.def("align_fp8", align_fp8);
   m.def("transpose_fp8", [](const Tensor& q, const Tensor& scale) { return GPUEXP_CALL(transpose_fp8, q, scale); });
   m.def("gemm_fp8", [](const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
                        const std::optional<Tensor>& out, at::ScalarType out_dtype, int64_t variant, int64_t parts) {

@@ -9,8 +9,11 @@ scale is the smallest 2^e, e >= -127, that brings its largest finite magnitude t
 type's largest value (448 or 57344); each value is rounded once, to nearest even.  Rows of q start
 at multiples of 16 bytes and rows of scale at multiples of 4: the functions here make them so, q's
 at multiples of 128 where that takes at most an eighth more memory (q is then a view of wider rows).
+clone(), contiguous(), a copy on another device or load_state_dict() into a new buffer may lay rows out
+otherwise: align_fp8 puts such a copy right, once.
 
   quantize_fp8 / dequantize_fp8   an activation checkpoint in 8 bits, kept and given back
+  align_fp8                       rows of a copy put where the others want them
   transpose_fp8                   the same checkpoint by columns: the gradient of a weight reads it so
   quantize_fp8_both               a tensor by rows and by columns in one pass
   gemm_fp8                        C = A B^T of two such operands on the matrix cores
@@ -77,6 +80,16 @@ def dequantize_fp8(q, scale, dtype=torch.bfloat16, stream=None):
         with _elsewhere(stream, q, scale):
             return _native.dequantize_fp8(q, scale, dtype)
     return _native.dequantize_fp8(q, scale, dtype)
+
+
+def align_fp8(q, scale, stream=None):
+    """(q, scale) with rows where the functions here want them, for a pair that was cloned, made contiguous, moved
+    between devices or loaded from a file (serving weights: once, after loading).  Strides may be any; a tensor that
+    fits already is returned itself, not a copy.  On the CPU too."""
+    if stream is not None:
+        with _elsewhere(stream, q, scale):
+            return _native.align_fp8(q, scale)
+    return _native.align_fp8(q, scale)
 
 
 def transpose_fp8(q, scale, stream=None):

@@ -162,3 +162,37 @@ def test_forward_mode_is_refused(reverse):
                 call()
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("m,k,block_rows", [(1, 1, 1), (5, 300, 1), (130, 1101, 128), (4, 256, 1), (129, 0, 128), (0, 40, 1)])
+def test_copies_are_aligned_on_the_cpu(m, k, block_rows):
+    """Any strides in; rows at multiples of 16 and 4 bytes, the same codes and scales out; what fits stays itself."""
+    from kubernetes_gpu_exporter_amd.ops.fp8 import align_fp8
+    a, s = q(m, k, block_rows) if m and k else (torch.zeros(m, k).to(E4M3), torch.zeros(-(-m // block_rows), -(-k // 128)).to(E8M0))
+    again = align_fp8(a, s)
+    assert again[0] is a and again[1] is s
+    for copy in (lambda t: t.clone(), lambda t: t.contiguous(), lambda t: t.T.contiguous().T,
+                 lambda t: torch.cat([torch.zeros(1, dtype=torch.uint8), t.contiguous().view(torch.uint8).flatten()])[1:]
+                 .view(t.dtype).view(t.shape)):
+        b, t = align_fp8(copy(a), copy(s))
+        assert torch.equal(b.float(), a.float()) and torch.equal(t.view(torch.uint8), s.view(torch.uint8))
+        for got, pad in ((b, 16), (t, 4)):
+            if got.numel():
+                assert got.data_ptr() % pad == 0 and (got.shape[1] == 1 or got.stride(1) == 1)
+                assert got.shape[0] == 1 or (got.stride(0) % pad == 0 and got.stride(0) >= got.shape[1])
+
+
+def test_pairs_that_are_none_are_not_aligned():
+    from kubernetes_gpu_exporter_amd.ops.fp8 import align_fp8
+    a, s = q(4, 256)
+    with pytest.raises(TypeError, match="float8"):
+        align_fp8(a.float(), s)
+    with pytest.raises(TypeError, match="e8m0"):
+        align_fp8(a, s.view(torch.uint8))
+    with pytest.raises(ValueError, match="the scales of q"):
+        align_fp8(a, s[:, :1])
+    with pytest.raises(ValueError, match="2-dimensional"):
+        align_fp8(a[0], s)
+    with pytest.raises(ValueError, match="align_fp8"):  # the refusal of a copy says what to do
+        b, t = q(4, 250)
+        gemm_fp8(b.contiguous(), t, b, t)

@@ -823,3 +823,24 @@ def test_forward_mode_is_refused_on_gpu():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
         assert torch.equal(linear_fp8(x, w), linear_fp8(x, w.clone()))
+
+
+def test_copies_laid_out_again():
+    """A checkpoint and serving weights that went to the host, into a file's state or through clone(): align_fp8 lays them
+    out as the operators want them, and results are those of the originals."""
+    from kubernetes_gpu_exporter_amd.ops.fp8 import align_fp8
+    g = gen(33)
+    x = torch.randn(30, 1101, device="cuda", generator=g).to(BF16)
+    w = torch.randn(200, 1101, device="cuda", generator=g).to(BF16)
+    kept, weight = quantize_fp8(x), quantize_fp8(w, block_rows=128)
+    module = torch.nn.Module()
+    module.register_buffer("q", torch.empty(200, 1101, device="cuda", dtype=E4M3))
+    module.register_buffer("scale", torch.empty(2, 9, device="cuda", dtype=E8M0))
+    module.load_state_dict({"q": weight[0], "scale": weight[1]})
+    assert torch.equal(dequantize_fp8(*align_fp8(kept[0].cpu().cuda(), kept[1].cpu().cuda())), dequantize_fp8(*kept))
+    for copy in ((module.q, module.scale), tuple(t.contiguous() for t in weight), tuple(t.clone() for t in weight),
+                 (weight[0].T.contiguous().T, weight[1].cpu().cuda())):
+        again = align_fp8(*copy)
+        assert torch.equal(linear_fp8(x, *again), linear_fp8(x, *weight))
+        assert torch.equal(gemm_fp8(*kept, *again), gemm_fp8(*kept, *weight))
+        assert torch.equal(transpose_fp8(*again)[0].float(), transpose_fp8(*weight)[0].float())
