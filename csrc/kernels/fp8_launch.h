@@ -72,10 +72,11 @@ hipError_t launch_gemm_fp8_wide(const void* x, int type, int64_t ldx, Fp8In w, i
 
 // y[M][N] = x[M][K] . w[N][K]^T in 8 bits and its backward pass, several launches behind one call.
 // Two workspaces in device memory: `kept` holds between the passes what the backward pass reads (x in
-// 8 bits if dw is wanted, the transposed weight in 8 bits if dx is), `temp` only during a pass.
+// 8 bits for dw, the transposed weight in 8 bits for dx), `temp` only during a pass.
 struct LinearFp8Args {
   int64_t M, N, K;
-  bool want_dx, want_dw;
+  bool keep_dx, keep_dw;  // what `kept` is laid out for
+  bool want_dx, want_dw;  // what a backward pass computes, of these
   const void* x;  // [M][ldx], type
   int64_t ldx;
   const void* w;  // [N][ldw], wtype; not read by the backward pass
@@ -84,8 +85,8 @@ struct LinearFp8Args {
   uint8_t* kept;
   uint8_t* temp;
 };
-int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);
-int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);   // temp
+int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw);
+int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw);   // temp
 int64_t linear_fp8_backward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);  // temp
 hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream);
 hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,

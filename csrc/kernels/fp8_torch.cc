@@ -272,7 +272,7 @@ void check_layer(const Tensor& x, at::ScalarType wtype) {
 }
 
 // y = x w^T of x [M, K], w [N, K] and the workspace that the backward pass needs
-Pair linear_fp8_forward(const Tensor& x, const Tensor& w, bool want_dx, bool want_dw) {
+Pair linear_fp8_forward(const Tensor& x, const Tensor& w, bool keep_dx, bool keep_dw) {
   check_layer(x, w.scalar_type());
   check_gpu("linear_fp8", x, w);
   TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && row_major(x) && row_major(w),
@@ -280,33 +280,34 @@ Pair linear_fp8_forward(const Tensor& x, const Tensor& w, bool want_dx, bool wan
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const On on(x);
   Tensor y = empty({M, N}, x, x.scalar_type()),
-         kept = bytes(gpuexp::linear_fp8_kept_bytes(M, N, K, want_dx, want_dw), x),
-         temp = bytes(gpuexp::linear_fp8_forward_bytes(M, N, K, want_dx, want_dw), x);
-  gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, x.const_data_ptr(), wide_stride(x), w.const_data_ptr(),
+         kept = bytes(gpuexp::linear_fp8_kept_bytes(M, N, K, keep_dx, keep_dw), x),
+         temp = bytes(gpuexp::linear_fp8_forward_bytes(M, N, K, keep_dx, keep_dw), x);
+  gpuexp::LinearFp8Args a{M, N, K, keep_dx, keep_dw, false, false, x.const_data_ptr(), wide_stride(x), w.const_data_ptr(),
                           wide_stride(w), wide_type(x.scalar_type()), wide_type(w.scalar_type()),
                           static_cast<uint8_t*>(kept.mutable_data_ptr()), static_cast<uint8_t*>(temp.mutable_data_ptr())};
   check(gpuexp::launch_linear_fp8_forward(a, y.mutable_data_ptr(), on.stream), "linear_fp8");
   return {std::move(y), std::move(kept)};
 }
 
-// (dx, dw) of dy [M, N] and what the forward pass kept; one that is not wanted is undefined
-Pair linear_fp8_backward(const Tensor& given, const Tensor& kept, int64_t K, at::ScalarType wtype, bool want_dx,
-                         bool want_dw) {
+// (dx, dw) of dy [M, N] and what the forward pass kept for them; one that is not wanted is undefined
+Pair linear_fp8_backward(const Tensor& given, const Tensor& kept, int64_t K, at::ScalarType wtype, bool kept_dx,
+                         bool kept_dw, bool want_dx, bool want_dw) {
   const Tensor dy = rows_of(given);
   check_layer(dy, wtype);
   check_gpu("linear_fp8", dy, kept);
   const int64_t M = dy.size(0), N = dy.size(1);
   TORCH_CHECK_VALUE(dy.dim() == 2 && kept.scalar_type() == at::kByte && kept.is_contiguous() &&
-                        kept.numel() == gpuexp::linear_fp8_kept_bytes(M, N, K, want_dx, want_dw),
-                    "linear_fp8_backward: what was kept is not of these sizes");
+                        kept.numel() == gpuexp::linear_fp8_kept_bytes(M, N, K, kept_dx, kept_dw) &&
+                        (kept_dx || !want_dx) && (kept_dw || !want_dw),
+                    "linear_fp8_backward: what was kept is not of these sizes, or not for these gradients");
   const On on(dy);
   Tensor dx, dw;
   if (want_dx) dx = empty({M, K}, dy, dy.scalar_type());
   if (want_dw) dw = empty({N, K}, dy, wtype);
   const Tensor temp = bytes(gpuexp::linear_fp8_backward_bytes(M, N, K, want_dx, want_dw), dy);
-  gpuexp::LinearFp8Args a{M, N, K, want_dx, want_dw, nullptr, 0, nullptr, 0, wide_type(dy.scalar_type()),
-                          wide_type(wtype), static_cast<uint8_t*>(kept.mutable_data_ptr()),
-                          static_cast<uint8_t*>(temp.mutable_data_ptr())};
+  gpuexp::LinearFp8Args a{M, N, K, kept_dx, kept_dw, want_dx, want_dw, nullptr, 0, nullptr, 0,
+                          wide_type(dy.scalar_type()), wide_type(wtype),
+                          static_cast<uint8_t*>(kept.mutable_data_ptr()), static_cast<uint8_t*>(temp.mutable_data_ptr())};
   check(gpuexp::launch_linear_fp8_backward(a, dy.const_data_ptr(), wide_stride(dy),
                                            want_dx ? dx.mutable_data_ptr() : nullptr,
                                            want_dw ? dw.mutable_data_ptr() : nullptr, on.stream),
@@ -389,21 +390,24 @@ variable_list once(variable_list results) {
 
 struct LinearFp8 : torch::autograd::Function<LinearFp8> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
-    const bool want_dx = x.requires_grad(), want_dw = w.requires_grad();
-    auto [y, kept] = GPUEXP_CALL(linear_fp8_forward, x, w, want_dx, want_dw);
+    const bool keep_dx = x.requires_grad(), keep_dw = w.requires_grad();
+    auto [y, kept] = GPUEXP_CALL(linear_fp8_forward, x, w, keep_dx, keep_dw);
     ctx->save_for_backward({kept});
-    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(1), want_dx, want_dw, int64_t(w.scalar_type())};
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(1), keep_dx, keep_dw, int64_t(w.scalar_type())};
     return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor kept = ctx->get_saved_variables()[0];
     const std::vector<int64_t> s = ctx->saved_data["sizes"].toIntVector();
+    const bool kept_dx = s[1] != 0, kept_dw = s[2] != 0;
+    // a call may ask for one gradient alone (torch.autograd.grad(y, x), backward(inputs=[w]))
+    const bool want_dx = kept_dx && ctx->needs_input_grad(0), want_dw = kept_dw && ctx->needs_input_grad(1);
     variable_list results(2);
     {
       at::AutoGradMode off(false);
-      std::tie(results[0], results[1]) =
-          GPUEXP_CALL(linear_fp8_backward, grads[0], kept, s[0], at::ScalarType(s[3]), s[1] != 0, s[2] != 0);
+      std::tie(results[0], results[1]) = GPUEXP_CALL(linear_fp8_backward, grads[0], kept, s[0], at::ScalarType(s[3]),
+                                                     kept_dx, kept_dw, want_dx, want_dw);
     }
     return once(std::move(results));
   }
@@ -455,9 +459,9 @@ TORCH_LIBRARY(gpuexp, m) {
         "-> Tensor");
   m.def("gemm_fp8_out(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, Tensor(a!) out, int variant, int parts) -> ()");
   m.def("linear_fp8(Tensor x, Tensor weight, Tensor? weight_scale) -> Tensor");
-  m.def("linear_fp8_forward(Tensor x, Tensor weight, bool want_dx, bool want_dw) -> (Tensor, Tensor)");
-  m.def("linear_fp8_backward(Tensor dy, Tensor kept, int inputs, ScalarType weight_dtype, bool want_dx, bool want_dw) "
-        "-> (Tensor, Tensor)");
+  m.def("linear_fp8_forward(Tensor x, Tensor weight, bool keep_dx, bool keep_dw) -> (Tensor, Tensor)");
+  m.def("linear_fp8_backward(Tensor dy, Tensor kept, int inputs, ScalarType weight_dtype, bool kept_dx, bool kept_dw, "
+        "bool want_dx, bool want_dw) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(gpuexp, CompositeExplicitAutograd, m) {

@@ -2,7 +2,7 @@
 //   forward    x -> Q(x) (kept if the weight takes a gradient), w -> Q(w) and its transpose (kept if x
 //              takes one), y = Q(x) Q(w)^T
 //   backward   dy -> Q(dy) and Q(dy^T) in one pass over dy, dx = Q(dy) Q(w), dw = Q(dy^T) T(Q(x))^T
-//              with T the kept x transposed and requantised along the tokens
+//              with T the kept x transposed and requantised along the tokens; of these what is asked for
 // Host code only; one call from Python per pass, since a small step is bound by the host.
 #include <algorithm>
 
@@ -37,26 +37,29 @@ struct Product {
   }
 };
 
-struct Plan {
-  Piece xq, wq, wt;      // forward: x, w; w transposed
-  Piece gq, gt, xt;      // backward: dy, dy transposed, x transposed
-  struct {
-    int64_t kept, forward_temp, backward_temp;
-  } bytes;  // without the products' sums, which follow in a pass's workspace
-  Plan(int64_t M, int64_t N, int64_t K, bool dx, bool dw) : bytes{0, 0, 0} {
-    auto take = [](Piece& p, int64_t& at, int64_t rows, int64_t cols, int block_rows) {
-      p = {rows, cols, at, block_rows};
-      at = p.end();
-    };
-    take(xq, dw ? bytes.kept : bytes.forward_temp, M, K, 1);
-    take(wq, bytes.forward_temp, N, K, kFp8Block);
-    if (dx) {
-      take(wt, bytes.kept, K, N, kFp8Block);
-      take(gq, bytes.backward_temp, M, N, 1);
-    }
-    if (dw) {
-      take(gt, bytes.backward_temp, N, M, 1);
-      take(xt, bytes.backward_temp, K, M, 1);
+void take(Piece& p, int64_t& at, int64_t rows, int64_t cols, int block_rows) {
+  p = {rows, cols, at, block_rows};
+  at = p.end();
+}
+
+// Bytes are without the products' sums, which follow in a pass's workspace.
+struct Forward {
+  Piece xq, wq, wt;  // x, w; w transposed
+  int64_t kept = 0, temp = 0;
+  Forward(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw) {
+    take(xq, keep_dw ? kept : temp, M, K, 1);
+    take(wq, temp, N, K, kFp8Block);
+    if (keep_dx) take(wt, kept, K, N, kFp8Block);
+  }
+};
+struct Backward {
+  Piece gq, gt, xt;  // dy, dy transposed, x transposed
+  int64_t temp = 0;
+  Backward(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
+    if (want_dx) take(gq, temp, M, N, 1);
+    if (want_dw) {
+      take(gt, temp, N, M, 1);
+      take(xt, temp, K, M, 1);
     }
   }
 };
@@ -67,40 +70,43 @@ struct Plan {
 
 }  // namespace
 
-int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
-  return Plan(M, N, K, want_dx, want_dw).bytes.kept;
+int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw) {
+  return Forward(M, N, K, keep_dx, keep_dw).kept;
 }
 
-int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
-  return Plan(M, N, K, want_dx, want_dw).bytes.forward_temp + Product(M, N, K).bytes();
+int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw) {
+  return Forward(M, N, K, keep_dx, keep_dw).temp + Product(M, N, K).bytes();
 }
 
 // the two products take turns at the same place
 int64_t linear_fp8_backward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw) {
-  return Plan(M, N, K, want_dx, want_dw).bytes.backward_temp +
+  return Backward(M, N, K, want_dx, want_dw).temp +
          std::max(want_dx ? Product(M, K, N).bytes() : 0, want_dw ? Product(N, K, M).bytes() : 0);
 }
 
 hipError_t launch_linear_fp8_forward(const LinearFp8Args& a, void* y, hipStream_t stream) {
-  const Plan p(a.M, a.N, a.K, a.want_dx, a.want_dw);
-  uint8_t* x_at = a.want_dw ? a.kept : a.temp;
+  const Forward p(a.M, a.N, a.K, a.keep_dx, a.keep_dw);
+  uint8_t* x_at = a.keep_dw ? a.kept : a.temp;
   GPUEXP_RETURN_IF(launch_quantize_fp8(a.x, a.type, a.ldx, a.M, a.K, kE4M3, 1, p.xq.out(x_at), {}, stream));
   GPUEXP_RETURN_IF(launch_quantize_fp8(a.w, a.wtype, a.ldw, a.N, a.K, kE4M3, kFp8Block, p.wq.out(a.temp),
-                                       a.want_dx ? p.wt.out(a.kept) : Fp8Out{}, stream));
-  return Product(a.M, a.N, a.K).run(p.xq.in(x_at), p.wq.in(a.temp), y, a.type, a.temp + p.bytes.forward_temp, stream);
+                                       a.keep_dx ? p.wt.out(a.kept) : Fp8Out{}, stream));
+  return Product(a.M, a.N, a.K).run(p.xq.in(x_at), p.wq.in(a.temp), y, a.type, a.temp + p.temp, stream);
 }
 
 hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, int64_t lddy, void* dx, void* dw,
                                       hipStream_t stream) {
-  const Plan p(a.M, a.N, a.K, a.want_dx, a.want_dw);
-  uint8_t* sums = a.temp + p.bytes.backward_temp;
+  if ((a.want_dx && !a.keep_dx) || (a.want_dw && !a.keep_dw)) return hipErrorInvalidValue;
+  if (!a.want_dx && !a.want_dw) return hipSuccess;
+  const Forward f(a.M, a.N, a.K, a.keep_dx, a.keep_dw);
+  const Backward p(a.M, a.N, a.K, a.want_dx, a.want_dw);
+  uint8_t* sums = a.temp + p.temp;
   GPUEXP_RETURN_IF(launch_quantize_fp8(dy, a.type, lddy, a.M, a.N, kE4M3, 1,
                                        a.want_dx ? p.gq.out(a.temp) : Fp8Out{},
                                        a.want_dw ? p.gt.out(a.temp) : Fp8Out{}, stream));
   if (a.want_dx)
-    GPUEXP_RETURN_IF(Product(a.M, a.K, a.N).run(p.gq.in(a.temp), p.wt.in(a.kept), dx, a.type, sums, stream));
+    GPUEXP_RETURN_IF(Product(a.M, a.K, a.N).run(p.gq.in(a.temp), f.wt.in(a.kept), dx, a.type, sums, stream));
   if (a.want_dw) {
-    GPUEXP_RETURN_IF(launch_transpose_fp8(p.xq.in(a.kept), a.M, a.K, p.xt.out(a.temp), stream));
+    GPUEXP_RETURN_IF(launch_transpose_fp8(f.xq.in(a.kept), a.M, a.K, p.xt.out(a.temp), stream));
     GPUEXP_RETURN_IF(Product(a.N, a.K, a.M).run(p.gt.in(a.temp), p.xt.in(a.temp), dw, a.wtype, sums, stream));
   }
   return hipSuccess;

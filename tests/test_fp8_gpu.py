@@ -844,3 +844,38 @@ def test_copies_laid_out_again():
         assert torch.equal(linear_fp8(x, *again), linear_fp8(x, *weight))
         assert torch.equal(gemm_fp8(*kept, *again), gemm_fp8(*kept, *weight))
         assert torch.equal(transpose_fp8(*again)[0].float(), transpose_fp8(*weight)[0].float())
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 520, 4096), (300, 256, 640), (8200, 260, 500)])
+def test_only_the_gradient_asked_for_is_computed(m, n, k):
+    g = gen(34)
+    x = torch.randn(m, k, device="cuda", generator=g).to(BF16).requires_grad_()
+    w = torch.randn(n, k, device="cuda", generator=g).to(BF16).requires_grad_()
+    grad = torch.randn(m, n, device="cuda", generator=g).to(BF16)
+    y = linear_fp8(x, w)
+
+    def asked(*leaves):
+        before = torch.cuda.memory_stats()["requested_bytes.all.allocated"]
+        got = torch.autograd.grad(y, leaves, grad, retain_graph=True)
+        return got, torch.cuda.memory_stats()["requested_bytes.all.allocated"] - before
+    (dx, dw), both = asked(x, w)
+    (only_x,), of_x = asked(x)
+    (only_w,), of_w = asked(w)
+    assert torch.equal(only_x, dx) and torch.equal(only_w, dw)
+    assert of_x <= both - 2 * dw.numel() and of_w <= both - 2 * dx.numel()
+    y.backward(grad, inputs=[w])
+    assert x.grad is None and torch.equal(w.grad, dw)
+
+
+def test_traced_step_of_one_gradient_computes():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    g = gen(36)
+    w = torch.randn(96, 320, device="cuda", generator=g).to(BF16)
+    x, other = (torch.randn(40, 320, device="cuda", generator=g).to(BF16) for _ in range(2))
+
+    def of_weight(a, b):
+        b = b.detach().requires_grad_()
+        return torch.autograd.grad(linear_fp8(a.detach().requires_grad_(), b).float().square().sum(), b)[0]
+    traced = make_fx(of_weight)(x, w)
+    for t in (x, other):
+        assert torch.equal(traced(t, w), of_weight(t, w))
