@@ -36,7 +36,7 @@ constexpr int64_t kLongest = int64_t(1) << 22;
 
 void check(hipError_t e, const char* what) {
   TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": larger than the kernels index (fewer than 2^31 rows, rows at most "
-                    "4 MiB apart in 8 bits, fewer than 2^35 values to quantise, fewer than 2^23 tiles of a product)");
+                    "4 MiB apart in 8 bits, fewer than 2^35 values to quantise, fewer than 2^32 threads of a product)");
   TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
 }
 
@@ -228,7 +228,7 @@ Tensor product(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Te
                       ", strides ", given->strides());
   const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, int(variant), int(parts));
   TORCH_CHECK_VALUE(plan.variant >= 0, "variant ", variant, " with ", parts, " parts does not take these sizes (", M, ", ",
-                    N, ", ", K, ")");
+                    N, ", ", K, ")", variant == 0 && parts == 0 ? ": more blocks than a launch has" : "");
   check_gpu("gemm_fp8", a, a_scale, b, b_scale, given ? *given : a);
   TORCH_CHECK_VALUE(K <= kLongest, "gemm_fp8: rows of at most ", kLongest, " values, got ", K);
   const On on(a);

@@ -843,14 +843,34 @@ double estimate_us(int variant, int64_t M, int64_t blocks, double nk) {
 
 }  // namespace
 
+// waves of a few-rows block: each takes at least a unit of 512 bytes of K
+static int rows_waves(int64_t K) {
+  const int64_t quads = ((K & ~int64_t(15)) + 4 * kBK - 1) / (4 * kBK);
+  int waves = 1;
+  while (waves < 16 && waves < quads) waves *= 2;
+  return waves;
+}
+
+// whether a launch has less than 2^32 threads
+static bool grid_ok(int variant, int parts, int64_t M, int64_t N, int64_t K) {
+  const auto blocks = [](int64_t n, int64_t edge) { return (n + edge - 1) / edge; };
+  constexpr int64_t kThreads = int64_t(1) << 32;
+  if (variant == 3 || variant == 6) return blocks(N, variant == 3 ? 16 : 32) * rows_waves(K) * 64 < kThreads;
+  if (variant == 2) return blocks(M, 256) * blocks(N, 256) * 512 < kThreads;
+  const int64_t edge = variant == 4 ? 64 : 128;
+  return blocks(M, edge) * blocks(N, edge) * (parts > 1 ? 16 : 1) * 256 < kThreads;  // (16: join_parts_kernel's)
+}
+
 // variant 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows (M <= 16), 4 = 64 x 64
 // tile, 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU), 6 = few rows, 32 of B per wave;
 // parts 0 = by the sizes, with a variant 1
 GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts) {
-  const auto takes = [&](int v) { return v == 2 ? K >= kBK + 16 : v == 3 || v == 6 ? M <= 16 : v >= 1 && v <= 5; };
+  const auto takes = [&](int v, int p) {
+    return (v == 2 ? K >= kBK + 16 : v == 3 || v == 6 ? M <= 16 : v >= 1 && v <= 5) && grid_ok(v, p, M, N, K);
+  };
   const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
   if (variant != 0) {
-    const bool ok = takes(variant) && parts >= 0 &&
+    const bool ok = takes(variant, parts) && parts >= 0 &&
                     (parts <= 1 || ((variant == 1 || variant == 4) && parts <= 16 && parts <= quads));
     return {ok ? variant : -1, parts > 1 ? parts : 1};
   }
@@ -858,15 +878,16 @@ GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int part
   const double nk = double(K) * (1.0 / kBK);
   const auto tiles = [&](int edge) { return ((M + edge - 1) / edge) * ((N + edge - 1) / edge); };
   const int64_t of_64 = tiles(64), of_128 = tiles(128);
-  GemmFp8Plan plan{4, 1};
-  double best = estimate_us(4, M, of_64, nk);
+  GemmFp8Plan plan{-1, 1};
+  double best = 0;
   const auto consider = [&](int v, int p, double us) {
-    if (us < best) best = us, plan = {v, p};
+    if ((plan.variant < 0 || us < best) && takes(v, p)) best = us, plan = {v, p};
   };
+  consider(4, 1, estimate_us(4, M, of_64, nk));
   consider(1, 1, estimate_us(1, M, of_128, nk));
   consider(5, 1, estimate_us(5, M, of_128, nk));
-  if (takes(2)) consider(2, 1, estimate_us(2, M, tiles(256), nk));
-  if (takes(3)) {
+  consider(2, 1, estimate_us(2, M, tiles(256), nk));
+  if (M <= 16) {
     consider(3, 1, estimate_us(3, M, (N + 15) / 16, nk));
     consider(6, 1, estimate_us(6, M, (N + 31) / 32, nk));
   }
@@ -890,11 +911,8 @@ namespace {
 
 template <int a, int b, int kR, int kWide = -1>
 void launch_rows(const GemmFp8Args& g, Operand oa, Operand ob, hipStream_t stream) {
-  const int64_t quads = ((g.K & ~int64_t(15)) + kQuad - 1) / kQuad;
-  int waves = 1;
-  while (waves < 16 && waves < quads) waves *= 2;
   hipLaunchKernelGGL((gemm_fp8_rows_kernel<a, b, kR, kWide>), dim3(uint32_t((g.N + 16 * kR - 1) / (16 * kR))),
-                     dim3(waves * 64), 0, stream, oa, ob, static_cast<uint16_t*>(g.c), g.ldc, int(g.K),
+                     dim3(rows_waves(g.K) * 64), 0, stream, oa, ob, static_cast<uint16_t*>(g.c), g.ldc, int(g.K),
                      g.ctype == kF16);
 }
 
@@ -907,9 +925,7 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   const int variant = plan.variant, parts = plan.parts;
   if (variant < 0 || (parts > 1 && !g.temp)) return hipErrorInvalidValue;
   const int64_t edge = variant == 2 ? 256 : variant == 4 ? 64 : 128;
-  const int64_t tiles = variant == 3 || variant == 6 ? (g.N + 15) / 16 : ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
-  const int64_t threads = variant == 3 || variant == 6 ? 1024 : variant == 2 ? 512 : 256;
-  if (tiles * (parts > 1 && parts < 16 ? 16 : parts) * threads >= (int64_t(1) << 32)) return hipErrorInvalidValue;
+  const int64_t tiles = ((g.M + edge - 1) / edge) * ((g.N + edge - 1) / edge);
   by_types(g.a.type, g.b.type, g.ctype, [&](auto ta, auto tb, auto tc) {
     constexpr int a = decltype(ta)::value, b = decltype(tb)::value;
     const Operand oa = operand(g.a, g.M), ob = operand(g.b, g.N);
@@ -955,7 +971,7 @@ bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64
 
 hipError_t launch_gemm_fp8_wide(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K,
                                 void* y, hipStream_t stream) {
-  if (!gemm_fp8_takes_wide(x, ldx, M, N, K) || !side_ok(w, N, K) || (N + 15) / 16 >= (int64_t(1) << 22))
+  if (!gemm_fp8_takes_wide(x, ldx, M, N, K) || !side_ok(w, N, K) || !grid_ok(3, 1, M, N, K))
     return hipErrorInvalidValue;
   if (N == 0) return hipSuccess;
   GemmFp8Args g{};

@@ -196,3 +196,19 @@ def test_pairs_that_are_none_are_not_aligned():
     with pytest.raises(ValueError, match="align_fp8"):  # the refusal of a copy says what to do
         b, t = q(4, 250)
         gemm_fp8(b.contiguous(), t, b, t)
+
+
+@pytest.mark.parametrize("M,N,K,variant,want", [
+    (1, 1 << 26, 16, 3, 3), (1, 1 << 26, 16, 6, 6), (1, 1 << 26, 8192, 3, -1), (1, 1 << 26, 8192, 6, 6),
+    (1, 1 << 27, 8192, 6, -1), (16, 1 << 30, 16, 6, 6), (16, 1 << 30, 16, 3, -1),
+    (1 << 21, 1 << 16, 64, 4, -1), (1 << 21, 1 << 16, 64, 1, 1), (1 << 24, 1 << 24, 256, 2, -1), (1 << 24, 1 << 24, 256, 0, -1)])
+def test_kernels_whose_launch_is_too_large_are_not_chosen(M, N, K, variant, want):
+    """A launch has less than 2^32 threads: 64 for each 512 of K (at most 1024) and 16 or 32 columns of C, 256 or 512 a tile."""
+    assert gemm_fp8_variant(M, N, K, variant) == want
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1 << 26, 16), (16, 1 << 28, 64), (1, 1 << 26, 8192), (1 << 21, 1 << 16, 64),
+                                   (1 << 23, 1 << 14, 16)])
+def test_the_choice_passes_over_them(M, N, K):
+    chosen = gemm_fp8_variant(M, N, K)
+    assert chosen > 0 and gemm_fp8_variant(M, N, K, chosen) == chosen

@@ -879,3 +879,16 @@ def test_traced_step_of_one_gradient_computes():
     traced = make_fx(of_weight)(x, w)
     for t in (x, other):
         assert torch.equal(traced(t, w), of_weight(t, w))
+
+
+def test_many_outputs_for_few_rows():
+    """2^26 columns of C: more blocks of 1024 threads than a launch takes, fewer of those that this K needs."""
+    n = 1 << 26
+    b = torch.zeros(n, 16, device="cuda", dtype=E4M3)
+    digits = torch.arange(n, device="cuda", dtype=torch.int32).remainder_(9).sub_(4).to(BF16)
+    b[:, 0] = digits.to(E4M3)
+    sb = torch.full((n // 128, 4), 127, device="cuda", dtype=torch.uint8).view(E8M0)[:, :1]
+    a, sa = quantize_fp8(torch.full((1, 16), 2.0, device="cuda"))
+    for variant in (0, 3, 4, 6):
+        assert torch.equal(gemm_fp8(a, sa, b, sb, variant=variant)[0], 2 * digits)
+    assert torch.equal(linear_fp8(torch.full((1, 16), 2.0, device="cuda", dtype=BF16), b, sb)[0], 2 * digits)
