@@ -38,6 +38,12 @@ struct Fp8In {
   int type;        // Fp8Type
 };
 
+// what the kernels index: of a tensor to quantise, give back or transpose its blocks of 128 along rows
+inline bool fp8_blocks_ok(int64_t rows, int64_t cols) {  // (16 lanes for each, and a launch has less than 2^32 threads)
+  return rows >= 0 && cols >= 0 && rows < (int64_t(1) << 28) && cols < (int64_t(1) << 31) - 128 &&
+         rows * ((cols + 127) / 128) < (int64_t(1) << 28) - 16;
+}
+
 // out = x[rows][cols] in 8 bits; outT = its transpose [cols][rows].  block_rows 1: blocks of
 // 1 x 128 along each output's own rows; 128: blocks of 128 x 128, the transpose the same values.
 hipError_t launch_quantize_fp8(const void* x, int xtype, int64_t ldx, int64_t rows, int64_t cols, int type,
@@ -63,6 +69,7 @@ struct GemmFp8Plan {
   int variant, parts;
 };
 GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts);
+bool gemm_fp8_ok(int64_t M, int64_t N, int64_t K);  // whether a product of these sizes has a kernel
 int64_t gemm_fp8_temp_bytes(int64_t M, int64_t N, const GemmFp8Plan& plan);
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream);
 // the same for x[M][ldx] in bf16 or f16, quantised on its way (blocks of 1 x 128, e4m3), where it takes x
@@ -85,6 +92,8 @@ struct LinearFp8Args {
   uint8_t* kept;
   uint8_t* temp;
 };
+// whether every launch of the passes takes these sizes, so that none is refused behind others
+bool linear_fp8_ok(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw);
 int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw);
 int64_t linear_fp8_forward_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw);   // temp
 int64_t linear_fp8_backward_bytes(int64_t M, int64_t N, int64_t K, bool want_dx, bool want_dw);  // temp
@@ -93,6 +102,7 @@ hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, in
                                       hipStream_t stream);
 // the same with a weight that is in 8 bits already; temp: x in 8 bits, where the product
 // does not make it, and the product's own
+bool serve_fp8_ok(int64_t M, int64_t N, int64_t K, bool want_dx);
 int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K);
 hipError_t launch_serve_fp8(const void* x, int type, int64_t ldx, Fp8In w, int64_t M, int64_t N, int64_t K, void* y,
                             uint8_t* temp, hipStream_t stream);

@@ -525,17 +525,11 @@ void by_types(int xtype, int type, F f) {
   else t(std::integral_constant<int, kF32>{});
 }
 
-// 16 lanes for each block of 128 values, and a launch has less than 2^32 threads
-bool count_ok(int64_t rows, int64_t cols) {
-  return rows >= 0 && cols >= 0 && rows < (int64_t(1) << 28) && cols < (int64_t(1) << 31) - 128 &&
-         rows * ((cols + 127) / 128) < (int64_t(1) << 28) - 16;
-}
-
 }  // namespace
 
 hipError_t launch_quantize_fp8(const void* x, int xtype, int64_t ldx, int64_t rows, int64_t cols, int type,
                                int block_rows, Fp8Out out, Fp8Out outT, hipStream_t stream) {
-  if (!count_ok(rows, cols)) return hipErrorInvalidValue;
+  if (!fp8_blocks_ok(rows, cols)) return hipErrorInvalidValue;
   if (rows == 0 || cols == 0) return hipSuccess;
   const uint32_t nb = uint32_t((cols + 127) / 128);
   by_types(xtype, type, [&](auto kx, auto kt) {
@@ -556,7 +550,7 @@ hipError_t launch_quantize_fp8(const void* x, int xtype, int64_t ldx, int64_t ro
 
 hipError_t launch_dequantize_fp8(Fp8In in, int64_t rows, int64_t cols, void* x, int xtype, int64_t ldx,
                                  hipStream_t stream) {
-  if (!count_ok(rows, cols)) return hipErrorInvalidValue;
+  if (!fp8_blocks_ok(rows, cols)) return hipErrorInvalidValue;
   if (rows == 0 || cols == 0) return hipSuccess;
   const uint32_t nb = uint32_t((cols + 127) / 128), units = uint32_t(rows) * nb;
   by_types(xtype, in.type, [&](auto kx, auto kt) {
@@ -569,7 +563,7 @@ hipError_t launch_dequantize_fp8(Fp8In in, int64_t rows, int64_t cols, void* x, 
 }
 
 hipError_t launch_transpose_fp8(Fp8In in, int64_t rows, int64_t cols, Fp8Out outT, hipStream_t stream) {
-  if (!count_ok(rows, cols)) return hipErrorInvalidValue;
+  if (!fp8_blocks_ok(rows, cols)) return hipErrorInvalidValue;
   if (rows == 0 || cols == 0) return hipSuccess;
   const uint32_t nb = uint32_t((cols + 127) / 128), tiles = uint32_t((rows + 127) / 128) * nb;
   auto k = in.type == kE4M3 ? (in.block_rows == 1 ? transpose_kernel<kE4M3, false> : transpose_kernel<kE4M3, true>)

@@ -34,9 +34,13 @@ int64_t blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 // the longest row of a product's operand: a tile of 256 of them has to fit in a buffer's 31 bits
 constexpr int64_t kLongest = int64_t(1) << 22;
 
+constexpr const char* kLimits =
+    "larger than the kernels index: of a tensor to quantise, give back or transpose fewer than 2^28 rows and 2^28 - 16 blocks "
+    "of 128 values along them, of a product's operand fewer than 2^31 - 256 rows at most 4 MiB apart, and fewer than 2^32 "
+    "threads in a launch";
+
 void check(hipError_t e, const char* what) {
-  TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": larger than the kernels index (fewer than 2^31 rows, rows at most "
-                    "4 MiB apart in 8 bits, fewer than 2^35 values to quantise, fewer than 2^32 threads of a product)");
+  TORCH_CHECK_VALUE(e != hipErrorInvalidValue, what, ": ", kLimits);
   TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
 }
 
@@ -339,16 +343,18 @@ Tensor checked_linear(const Tensor& x, const Tensor& weight, const std::optional
   if (scale) {
     TORCH_CHECK_VALUE(!weight.requires_grad(), "weights in 8 bits take no gradient");
     operand("weight", weight, *scale);
-    check_gpu("linear_fp8", x, weight, *scale);
-  } else {
-    check_gpu("linear_fp8", x, weight);
   }
-  const int64_t K = x.size(-1);
+  const int64_t N = weight.size(0), K = x.size(-1);
   int64_t M = 1;
   for (int64_t d = 0; d < x.dim() - 1; ++d) M *= x.size(d);
-  TORCH_CHECK_VALUE(K <= kLongest && (!want_dx || weight.size(0) <= kLongest) && (!want_dw || M <= kLongest),
+  TORCH_CHECK_VALUE(K <= kLongest && (!want_dx || N <= kLongest) && (!want_dw || M <= kLongest),
                     "linear_fp8: at most ", kLongest, " inputs, for x's gradient as many outputs and for the weight's as "
-                    "many rows of x, got ", K, ", ", weight.size(0), " and ", M);
+                    "many rows of x, got ", K, ", ", N, " and ", M);
+  // (here, so that no backward pass is refused after its forward pass has run)
+  TORCH_CHECK_VALUE(scale ? gpuexp::serve_fp8_ok(M, N, K, want_dx) : gpuexp::linear_fp8_ok(M, N, K, want_dx, want_dw),
+                    "linear_fp8: ", M, " rows of ", K, " inputs and ", N, " outputs are ", kLimits);
+  if (scale) check_gpu("linear_fp8", x, weight, *scale);
+  else check_gpu("linear_fp8", x, weight);
   return rows_of(x.dim() == 2 ? x : x.reshape({M, K}));
 }
 

@@ -799,9 +799,11 @@ void by_types(int a, int b, int c, F f) {
   else t(std::integral_constant<int, kE5M2>{});
 }
 
+// a tile of 256 rows has to fit in a buffer's 31 bits
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 256, kMaxLd = int64_t(1) << 22;
+
 bool side_ok(const Fp8In& in, int64_t rows, int64_t K) {
-  // a tile of 256 rows has to fit in a buffer's 31 bits
-  return rows < (int64_t(1) << 31) - 256 && in.ld >= K && in.ld % 16 == 0 && in.ld <= (int64_t(1) << 22) &&
+  return rows < kMaxRows && in.ld >= K && in.ld % 16 == 0 && in.ld <= kMaxLd &&
          in.lds % 4 == 0 && in.lds * 128 >= K && reinterpret_cast<uintptr_t>(in.q) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(in.scale) % 4 == 0;
 }
@@ -900,6 +902,12 @@ GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int part
     }
   }
   return plan;
+}
+
+bool gemm_fp8_ok(int64_t M, int64_t N, int64_t K) {
+  return M < kMaxRows && N < kMaxRows && fp8_row_bytes(K) <= kMaxLd &&
+         (grid_ok(4, 1, M, N, K) || grid_ok(1, 1, M, N, K) || (K >= kBK + 16 && grid_ok(2, 1, M, N, K)) ||
+          (M <= 16 && grid_ok(6, 1, M, N, K)));
 }
 
 int64_t gemm_fp8_temp_bytes(int64_t M, int64_t N, const GemmFp8Plan& plan) {

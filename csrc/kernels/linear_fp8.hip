@@ -70,6 +70,12 @@ struct Backward {
 
 }  // namespace
 
+bool linear_fp8_ok(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw) {
+  return fp8_blocks_ok(M, K) && fp8_blocks_ok(N, K) && gemm_fp8_ok(M, N, K) &&
+         (!(keep_dx || keep_dw) || fp8_blocks_ok(M, N)) && (!keep_dx || gemm_fp8_ok(M, K, N)) &&
+         (!keep_dw || gemm_fp8_ok(N, K, M));
+}
+
 int64_t linear_fp8_kept_bytes(int64_t M, int64_t N, int64_t K, bool keep_dx, bool keep_dw) {
   return Forward(M, N, K, keep_dx, keep_dw).kept;
 }
@@ -110,6 +116,11 @@ hipError_t launch_linear_fp8_backward(const LinearFp8Args& a, const void* dy, in
     GPUEXP_RETURN_IF(Product(a.N, a.K, a.M).run(p.gt.in(a.temp), p.xt.in(a.temp), dw, a.wtype, sums, stream));
   }
   return hipSuccess;
+}
+
+bool serve_fp8_ok(int64_t M, int64_t N, int64_t K, bool want_dx) {
+  return fp8_blocks_ok(M, K) && gemm_fp8_ok(M, N, K) &&
+         (!want_dx || (fp8_blocks_ok(M, N) && fp8_blocks_ok(N, K) && gemm_fp8_ok(M, K, N)));
 }
 
 int64_t serve_fp8_bytes(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {

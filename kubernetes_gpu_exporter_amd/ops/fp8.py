@@ -139,7 +139,9 @@ def linear_fp8(x, weight, weight_scale=None):
     the weight 128 x 128).  For the backward pass x is kept as its 8-bit checkpoint, half the memory
     of the activation; dx = Q(dy) W with the kept 8-bit weight, dW = Q(dy^T) x with the checkpoint
     transposed (as transpose_fp8 does).  A double backward and forward-mode derivatives are refused.  K is at most 2^22, and so is N
-    where x takes a gradient and the number of x's rows where the weight takes one.
+    where x takes a gradient and the number of x's rows where the weight takes one; each tensor that is quantised, the
+    result's gradient among them, has fewer than 2^28 blocks of 128 along its rows.  Sizes that only the backward pass
+    would not take are refused before the forward pass.
 
     Serving: `weight` in 8 bits with its `weight_scale`, as quantize_fp8(w, block_rows=128) gives
     them; x may take a gradient, the weight takes none."""

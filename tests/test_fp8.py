@@ -212,3 +212,20 @@ def test_kernels_whose_launch_is_too_large_are_not_chosen(M, N, K, variant, want
 def test_the_choice_passes_over_them(M, N, K):
     chosen = gemm_fp8_variant(M, N, K)
     assert chosen > 0 and gemm_fp8_variant(M, N, K, chosen) == chosen
+
+
+@pytest.mark.parametrize("M,N,K,dx,dw,taken", [
+    (1 << 22, 8192, 16, True, False, False), ((1 << 22) - 1, 8192, 16, True, False, True),  # 2^28 blocks of dy, just fewer
+    (1 << 22, 8192, 16, False, False, True), (1 << 22, 8192, 16, False, True, False),
+    (1 << 27, 129, 8, True, False, False), (1 << 27, 128, 8, True, False, True),
+    (1 << 28, 8, 4, False, False, False)])  # x itself
+def test_sizes_that_the_backward_pass_would_refuse(M, N, K, dx, dw, taken):
+    """Refused before anything runs, the forward pass too; what is taken goes on to the next check."""
+    x = torch.empty(M, K, dtype=torch.bfloat16).requires_grad_(dx)  # (never touched: no memory)
+    w = torch.empty(N, K, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="same GPU" if taken else "larger than the kernels index"):
+        linear_fp8(x, w.clone().requires_grad_(dw))
+    if not dw:
+        wq, ws = torch.zeros(N, 16, dtype=torch.uint8)[:, :K].view(E4M3), torch.zeros(-(-N // 128), 4, dtype=torch.uint8)
+        with pytest.raises(ValueError, match="same GPU" if taken else "larger than the kernels index"):
+            linear_fp8(x, wq, ws.view(E8M0)[:, :1])
