@@ -68,7 +68,7 @@ struct GemmFp8Args {
 struct GemmFp8Plan {
   int variant, parts;
 };
-GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts);
+GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int64_t variant, int64_t parts);
 bool gemm_fp8_ok(int64_t M, int64_t N, int64_t K);  // whether a product of these sizes has a kernel
 int64_t gemm_fp8_temp_bytes(int64_t M, int64_t N, const GemmFp8Plan& plan);
 hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream);

@@ -230,7 +230,7 @@ Tensor product(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Te
     TORCH_CHECK_VALUE(given->dim() == 2 && given->size(0) == M && given->size(1) == N && row_major(*given),
                       "out must be [", M, ", ", N, "] with its columns next to each other, got ", given->sizes(),
                       ", strides ", given->strides());
-  const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, int(variant), int(parts));
+  const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, variant, parts);
   TORCH_CHECK_VALUE(plan.variant >= 0, "variant ", variant, " with ", parts, " parts does not take these sizes (", M, ", ",
                     N, ", ", K, ")", variant == 0 && parts == 0 ? ": more blocks than a launch has" : "");
   check_gpu("gemm_fp8", a, a_scale, b, b_scale, given ? *given : a);
@@ -516,7 +516,7 @@ PYBIND11_MODULE(_gpuexp_fp8, m) {
   m.def("linear_fp8", [](const Tensor& x, const Tensor& weight, const std::optional<Tensor>& weight_scale) {
     return GPUEXP_CALL(linear_fp8, x, weight, weight_scale);
   });
-  m.def("gemm_fp8_plan", [](int64_t M, int64_t N, int64_t K, int variant, int parts) {
+  m.def("gemm_fp8_plan", [](int64_t M, int64_t N, int64_t K, int64_t variant, int64_t parts) {
     const gpuexp::GemmFp8Plan plan = gpuexp::plan_gemm_fp8(M, N, K, variant, parts);
     return std::make_pair(plan.variant, plan.parts);
   }, py::arg("M"), py::arg("N"), py::arg("K"), py::arg("variant") = 0, py::arg("parts") = 0,

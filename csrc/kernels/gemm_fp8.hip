@@ -854,7 +854,7 @@ static int rows_waves(int64_t K) {
 }
 
 // whether a launch has less than 2^32 threads
-static bool grid_ok(int variant, int parts, int64_t M, int64_t N, int64_t K) {
+static bool grid_ok(int64_t variant, int64_t parts, int64_t M, int64_t N, int64_t K) {
   const auto blocks = [](int64_t n, int64_t edge) { return (n + edge - 1) / edge; };
   constexpr int64_t kThreads = int64_t(1) << 32;
   if (variant == 3 || variant == 6) return blocks(N, variant == 3 ? 16 : 32) * rows_waves(K) * 64 < kThreads;
@@ -866,15 +866,15 @@ static bool grid_ok(int variant, int parts, int64_t M, int64_t N, int64_t K) {
 // variant 0 = by the sizes, 1 = 128 x 128 tile, 2 = 256 x 256 tile, 3 = few rows (M <= 16), 4 = 64 x 64
 // tile, 5 = 128 x 128 tile with two K tiles in LDS (two blocks per CU), 6 = few rows, 32 of B per wave;
 // parts 0 = by the sizes, with a variant 1
-GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int variant, int parts) {
-  const auto takes = [&](int v, int p) {
+GemmFp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t K, int64_t variant, int64_t parts) {
+  const auto takes = [&](int64_t v, int64_t p) {
     return (v == 2 ? K >= kBK + 16 : v == 3 || v == 6 ? M <= 16 : v >= 1 && v <= 5) && grid_ok(v, p, M, N, K);
   };
   const int64_t quads = (K + 4 * kBK - 1) / (4 * kBK);
   if (variant != 0) {
     const bool ok = takes(variant, parts) && parts >= 0 &&
                     (parts <= 1 || ((variant == 1 || variant == 4) && parts <= 16 && parts <= quads));
-    return {ok ? variant : -1, parts > 1 ? parts : 1};
+    return {ok ? int(variant) : -1, ok && parts > 1 ? int(parts) : 1};
   }
   if (parts < 0 || parts > 1) return {-1, 1};
   const double nk = double(K) * (1.0 / kBK);

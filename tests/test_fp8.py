@@ -229,3 +229,13 @@ def test_sizes_that_the_backward_pass_would_refuse(M, N, K, dx, dw, taken):
         wq, ws = torch.zeros(N, 16, dtype=torch.uint8)[:, :K].view(E4M3), torch.zeros(-(-N // 128), 4, dtype=torch.uint8)
         with pytest.raises(ValueError, match="same GPU" if taken else "larger than the kernels index"):
             linear_fp8(x, wq, ws.view(E8M0)[:, :1])
+
+
+@pytest.mark.parametrize("far", [1 << 32, (1 << 32) + 1, -(1 << 32)])
+def test_variants_and_parts_past_32_bits_are_refused(far):
+    a, s = q(4, 1024)
+    with pytest.raises(ValueError, match="variant"):
+        gemm_fp8(a, s, a, s, variant=far)
+    with pytest.raises(ValueError, match="parts"):
+        gemm_fp8(a, s, a, s, variant=1, parts=far)
+    assert gemm_fp8_variant(4, 4, 1024, far) == -1
