@@ -56,7 +56,9 @@ def quantize_fp8(x, dtype=torch.float8_e4m3fn, block_rows: int = 1, stream=None)
     """x [rows, cols] (bf16, f16 or f32, columns next to each other, any row stride) in 8 bits:
     (q, scale).  block_rows 1: a scale for each 128 values of a row (activations, gradients);
     128: for each 128 x 128 block (weights).  Infinities and NaN do not count for a scale; they
-    become the type's NaN (e4m3) or stay as they are (e5m2)."""
+    become the type's NaN (e4m3) or stay as they are (e5m2).  A value within half an 8-bit step of 2^16 (f16:
+    from 63488 on in e4m3, 61440 in e5m2) or 2^128 (bf16, f32) is rounded up to that power, which its wide type
+    does not hold: dequantize_fp8 into that type gives infinity."""
     if stream is not None:
         with _elsewhere(stream, x):
             return _native.quantize_fp8(x, dtype, block_rows)
@@ -75,7 +77,7 @@ def quantize_fp8_both(x, dtype=torch.float8_e4m3fn, block_rows: int = 1, stream=
 
 def dequantize_fp8(q, scale, dtype=torch.bfloat16, stream=None):
     """The values that (q, scale) stands for, [rows, cols] contiguous, in bf16, f16 or f32.  Exact
-    wherever `dtype` has the exponent's range."""
+    wherever `dtype` has the exponent's range; a value past its largest number is infinite."""
     if stream is not None:
         with _elsewhere(stream, q, scale):
             return _native.dequantize_fp8(q, scale, dtype)

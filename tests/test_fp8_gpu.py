@@ -892,3 +892,37 @@ def test_many_outputs_for_few_rows():
     for variant in (0, 3, 4, 6):
         assert torch.equal(gemm_fp8(a, sa, b, sb, variant=variant)[0], 2 * digits)
     assert torch.equal(linear_fp8(torch.full((1, 16), 2.0, device="cuda", dtype=BF16), b, sb)[0], 2 * digits)
+
+
+@pytest.mark.parametrize("dtype,xdtype,far", [(E4M3, F16, 63488.0), (E5M2, F16, 61440.0), (E4M3, BF16, 1.9375 * 2.0 ** 127),
+                                              (E4M3, F32, 1.9375 * 2.0 ** 127), (E5M2, F32, 1.875 * 2.0 ** 127)])
+def test_values_next_to_the_types_largest_come_back_infinite(dtype, xdtype, far):
+    """From `far` on, the middle between the largest 8-bit number below 2^16 (f16) or 2^128 and that power itself, a value
+    is rounded up to the power, which the wide type does not hold; below `far` it comes back finite."""
+    top = torch.finfo(xdtype).max
+    x = torch.zeros(3, 128, device="cuda", dtype=xdtype)
+    x[0, 0], x[1, 0], x[2, 0] = top, -top, far * (1 - 2.0 ** -7)
+    q, s = quantize_fp8(x, dtype)
+    back = dequantize_fp8(q, s, xdtype)
+    assert back[:2, 0].tolist() == [float("inf"), float("-inf")]
+    assert torch.isfinite(back[2, 0]) and not bool(back[:, 1:].any())
+    same(back, quantized(x, dtype)[0].float().to(xdtype))
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
+def test_gemm_with_extreme_scales(variant):
+    """Products of scales next to 2^-127 and 2^127: what leaves bf16's range is infinite or zero, a NaN scale gives NaN."""
+    g = gen(35)
+    m = 16 if variant in (3, 6) else 40
+    a, sa = pair(m, 256, g, block_rows=1)
+    b, sb = pair(48, 256, g, block_rows=1)
+    ta = torch.tensor([0, 254, 255, 127, 100, 7, 200, 64], dtype=torch.uint8, device="cuda").repeat(5)[:m]
+    tb = torch.tensor([254, 0, 127, 255, 150, 247], dtype=torch.uint8, device="cuda").repeat(8)
+    sa.view(torch.uint8)[:], sb.view(torch.uint8)[:] = ta[:, None], tb[:, None]
+    want = exact_product(a, sa, b, sb)
+    got = gemm_fp8(a, sa, b, sb, variant=variant)
+    e = (ta.int()[:, None] + tb.int()[None, :] - 254).double()
+    for keep in ((ta == 255)[:, None] | (tb == 255)[None, :], e.abs() <= 110):
+        same(got[keep], want.float().to(BF16)[keep])
+    assert not bool(got[(e < -160) & ~want.isnan()].any())
+    assert not bool(got[(e >= 128) & (want != 0)].isfinite().any())  # (a sum of infinities of both signs: NaN)
