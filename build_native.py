@@ -3,7 +3,7 @@
 
 Outputs (all inside kubernetes_gpu_exporter_amd/, so they travel with the repo):
   _gpuexp<EXT_SUFFIX>        pybind11 module: C++ telemetry core + HIP sentinel + MFMA GEMM
-  _gpuexp_fp8<EXT_SUFFIX>    8-bit operators on torch tensors (HIP kernels + torch bindings; where torch is)
+  _gpuexp_fp8<EXT_SUFFIX>    8-bit operators on torch tensors (HIP kernels + torch bindings; where a ROCm torch is)
   _gpuexp_aqlpmc.so          device PMC plugin: aqlprofile PM4 on an owned HSA queue (default)
   _gpuexp_rocprof.so         rocprofiler-sdk device-counting plugin (alternative counter backend)
   libgpuexp_rccl_tracer.so   rocprofiler-sdk RCCL API-tracing tool (ROCP_TOOL_LIBRARIES)
@@ -48,7 +48,7 @@ SENTINEL_HSACO = "gpuexp/sentinel_hsaco.hip"  # device-only code object for raw 
 CALIB_HSACO = "kernels/calib_hsaco.hip"       # PMC calibration workloads, dispatched on the PMC queue
 KERNELS_HIP = ["kernels/gemm_bf16.hip", "kernels/probe_kernels.hip", "kernels/kernels_bindings.hip"]
 FP8_HIP = ["kernels/fp8_quant.hip", "kernels/gemm_fp8.hip", "kernels/linear_fp8.hip"]
-FP8_CC = ["kernels/fp8_torch.cc"]  # against torch's headers: built where torch is installed
+FP8_CC = ["kernels/fp8_torch.cc"]  # against torch's headers: built where a ROCm build of torch is installed
 ROCPROF_CC = ["gpuexp/rocprof_plugin.cc"]
 AQLPMC_CC = ["gpuexp/aql_pmc.cc"]
 TRACER_CC = ["gpuexp/rccl_tracer.cc"]
@@ -92,6 +92,12 @@ def torch_dir() -> Path | None:
     return Path(spec.origin).parent if spec and spec.origin else None
 
 
+def rocm_torch_dir() -> Path | None:
+    """torch_dir() where that torch is built for ROCm (a CPU or CUDA one has not the libraries to link against)."""
+    where = torch_dir()
+    return where if where and (where / "lib" / "libc10_hip.so").exists() else None
+
+
 def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | None) -> Path:
     src = CSRC / src_rel
     obj = BUILD / (src_rel.replace("/", "__") + ".o")
@@ -106,7 +112,7 @@ def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | Non
     else:
         cmd = ["g++"]
         if src_rel in FP8_CC:  # torch's headers (its pybind11 among them) before ours
-            inc = torch_dir() / "include"
+            inc = rocm_torch_dir() / "include"
             cmd += [f"-I{inc}", f"-I{inc / 'torch' / 'csrc' / 'api' / 'include'}", "-DUSE_ROCM"]
         cmd += _common_flags(sanitize)
     cmd += ["-c", str(src), "-o", str(obj)]
@@ -163,8 +169,8 @@ def build(force: bool = False, jobs: int = 8, sanitize: str | None = None, verbo
     hdr = _hdr_mtime()
     BUILD.mkdir(parents=True, exist_ok=True)
     srcs = CORE_CC + SENTINEL_HIP + KERNELS_HIP
-    torch_lib = torch_dir() / "lib" if torch_dir() else None
-    if torch_lib:
+    torch = rocm_torch_dir()
+    if torch:
         srcs = srcs + FP8_HIP + FP8_CC
     extra = [s for s in ROCPROF_CC + AQLPMC_CC + TRACER_CC if (CSRC / s).exists()]
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
@@ -176,9 +182,9 @@ def build(force: bool = False, jobs: int = 8, sanitize: str | None = None, verbo
                                  ["-lamdhip64", "-lhsa-runtime64"])),
         "kernels": str(link_hip([objs[s] for s in KERNELS_HIP], _ext("_gpuexp_kernels"), ["-lamdhip64"])),
     }
-    if torch_lib:
+    if torch:
         outputs["fp8"] = str(link_hip([objs[s] for s in FP8_HIP + FP8_CC], _ext("_gpuexp_fp8"),
-                                      [f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+                                      [f"-L{torch / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
                                        "-lamdhip64"]))
     if (CSRC / ROCPROF_CC[0]).exists():
         outputs["rocprof_plugin"] = str(link_plain([objs[ROCPROF_CC[0]]], PKG / "_gpuexp_rocprof.so",
@@ -196,6 +202,8 @@ def build(force: bool = False, jobs: int = 8, sanitize: str | None = None, verbo
     if verbose:
         for k, v in outputs.items():
             print(f"[build_native] {k}: {v}")
+        if not torch:
+            print("[build_native] fp8: not built (no ROCm build of torch here)")
     return outputs
 
 

@@ -36,8 +36,8 @@ import torch  # (first: the native module shares torch's HIP runtime)
 try:
     from .. import _gpuexp_fp8 as _native
 except ImportError as e:
-    raise ImportError(f"native module _gpuexp_fp8 is not built; run `python build_native.py` where torch is "
-                      f"installed: {e}") from e
+    raise ImportError(f"native module _gpuexp_fp8 is not built; run `python build_native.py` where a ROCm "
+                      f"build of torch is installed: {e}") from e
 
 
 def _elsewhere(stream, *tensors):
