@@ -63,11 +63,26 @@ def _hdr_mtime() -> float:
     return max((p.stat().st_mtime for p in CSRC.rglob("*.h")), default=0.0)
 
 
-def _needs(obj: Path, src: Path, hdr_mtime: float, force: bool) -> bool:
+def _key_of(obj: Path) -> Path:
+    return BUILD / (obj.name + ".cmd")
+
+
+def _needs(obj: Path, src: Path, hdr_mtime: float, force: bool, key: str) -> bool:
+    """Whether `obj` is older than its sources, or was built by another command (`key`)."""
     if force or not obj.exists():
         return True
     m = obj.stat().st_mtime
-    return m < src.stat().st_mtime or m < hdr_mtime
+    recorded = _key_of(obj)
+    return (m < src.stat().st_mtime or m < hdr_mtime or not recorded.exists() or recorded.read_text() != key)
+
+
+def _compile(cmd: list[str], obj: Path, src: Path, hdr_mtime: float, force: bool, also: str = "") -> None:
+    """Runs `cmd`, which writes `obj`, if need be.  What else the object depends on is in `also`."""
+    key = "\n".join(cmd) + "\n" + also
+    if _needs(obj, src, hdr_mtime, force, key):
+        _key_of(obj).unlink(missing_ok=True)
+        _run(cmd)
+        _key_of(obj).write_text(key)
 
 
 def _run(cmd: list[str]) -> None:
@@ -101,9 +116,8 @@ def rocm_torch_dir() -> Path | None:
 def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | None) -> Path:
     src = CSRC / src_rel
     obj = BUILD / (src_rel.replace("/", "__") + ".o")
-    if not _needs(obj, src, hdr_mtime, force):
-        return obj
     obj.parent.mkdir(parents=True, exist_ok=True)
+    also = ""
     if src.suffix == ".hip":
         cmd = [str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "-x", "hip"] + HIP_FLAGS + _common_flags(None)
         if sanitize:
@@ -114,9 +128,11 @@ def compile_one(src_rel: str, hdr_mtime: float, force: bool, sanitize: str | Non
         if src_rel in FP8_CC:  # torch's headers (its pybind11 among them) before ours
             inc = rocm_torch_dir() / "include"
             cmd += [f"-I{inc}", f"-I{inc / 'torch' / 'csrc' / 'api' / 'include'}", "-DUSE_ROCM"]
+            version = rocm_torch_dir() / "version.py"  # (an object goes with one version of torch)
+            also = version.read_text() if version.exists() else ""
         cmd += _common_flags(sanitize)
     cmd += ["-c", str(src), "-o", str(obj)]
-    _run(cmd)
+    _compile(cmd, obj, src, hdr_mtime, force, also)
     return obj
 
 
@@ -148,11 +164,11 @@ def link_hip(objs: list[Path], out: Path, libs: list[str]) -> Path:
 def build_hsaco(src: str, out: Path, hdr_mtime: float, force: bool) -> Path:
     """A plain gfx950 code object (no host code, no offload bundle) for hsa_executable loading."""
     s = CSRC / src
-    if not _needs(out, s, hdr_mtime, force):
-        return out
+    obj = BUILD / out.name
+    _compile([str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "--cuda-device-only", "--no-gpu-bundle-output",
+              *HIP_FLAGS, "-O3", "-std=c++17", f"-I{CSRC}", "-o", str(obj), str(s)], obj, s, hdr_mtime, force)
     tmp = out.with_suffix(".tmp.hsaco")
-    _run([str(ROCM / "bin" / "hipcc"), f"--offload-arch={ARCH}", "--cuda-device-only", "--no-gpu-bundle-output",
-          *HIP_FLAGS, "-O3", "-std=c++17", f"-I{CSRC}", "-o", str(tmp), str(s)])
+    shutil.copyfile(obj, tmp)
     os.replace(tmp, out)
     return out
 
