@@ -926,3 +926,20 @@ def test_gemm_with_extreme_scales(variant):
         same(got[keep], want.float().to(BF16)[keep])
     assert not bool(got[(e < -160) & ~want.isnan()].any())
     assert not bool(got[(e >= 128) & (want != 0)].isfinite().any())  # (a sum of infinities of both signs: NaN)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 16, 8192), (8, 64, 8192), (8, 256, 8192), (16, 64, 4096), (5, 33, 8192)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_serving_few_weights_on_long_inputs(m, n, k, dtype):
+    """Quantised inside the product where the two-call way would cut K into parts and add in another order: against 64
+    bits, and on whole numbers, whose sums are exact in any order, the same bits as in two calls."""
+    g = gen(m + n)
+    wq, ws = quantize_fp8(torch.randn(n, k, device="cuda", generator=g) * 0.1, block_rows=128)
+    x = torch.randn(m, k, device="cuda", generator=g).to(dtype)
+    xq, w = quantized(x)[0], values(wq, ws)
+    want, size = xq @ w.T, xq.abs() @ w.abs().T
+    half, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert bool(((linear_fp8(x, wq, ws).double() - want).abs() <= half * want.abs() + 2.0 ** -8 * size + tiny).all())
+    whole, wide = pair(n, k, g, block_rows=128), small_whole(m, k, g).to(dtype)
+    wide[:, ::128] = 4.0  # (each block's largest: the scale is the same everywhere, and every value exact)
+    assert torch.equal(linear_fp8(wide, *whole), gemm_fp8(*quantize_fp8(wide), *whole, out_dtype=dtype))
