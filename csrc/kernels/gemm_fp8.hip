@@ -203,8 +203,8 @@ __device__ __forceinline__ void store4(uint16_t* dst, const f32x4& v, int column
 // on out of range, so the count holds.  The K loop is unrolled by 4, so with 2 or 4 stages every LDS
 // address is a constant.  The scales come as in the 256 x 256 kernel; a quad's words are read with its
 // first K tile, and the next quad's loaded then, which the count covers.
-// From memory a CU gets 22 bytes a clock this way, 0.31 us for a K tile of 64 x 64, and 8 stages get no
-// more.  So where there are fewer tiles than CUs, K is cut into parts at multiples of 512 (a row's four
+// From memory a CU gets 56 GB/s this way, 0.30 us for a K tile of 64 x 64 (64 blocks; from the caches
+// 0.18), and 8 stages get no more.  So where there are fewer tiles than CUs, K is cut into parts at multiples of 512 (a row's four
 // scales are one word), blockIdx.y of them: TC = float stores the sums of a part in 32 bits as the lanes
 // hold them, and join_parts_kernel adds them.
 template <int kA, int kB, typename TC, int kBM, int kBN, int kStages>
@@ -382,8 +382,7 @@ gemm_fp8_tile_kernel(Operand A, Operand B, uint16_t* __restrict__ C, int64_t ldc
 
 // C from the parts' sums, added in the parts' order, so results do not depend on timing.  A thread has 4
 // columns of a row, as they lie in the matrix instruction's result, and its loads are in flight together.
-// Bound by the launch and its bytes: with the stores that it waits for 4.7 us for 4 parts of 64 x 4096, 11
-// for 16.  (Joining in the last block to arrive would want counters that someone has cleared: a launch too.)
+// Bound by the launch and its bytes: 3.3 to 4.2 us for 4 parts of 64 x 4096.  (Joining in the last block to arrive would want counters that someone has cleared: a launch too.)
 template <typename TC, int kBM, int kBN>
 __global__ void __launch_bounds__(256)
 join_parts_kernel(const f32x4* __restrict__ sums, uint16_t* __restrict__ C, int64_t ldc, int M, int N, int parts) {
@@ -817,7 +816,7 @@ namespace {
 // once.  In parts there is a second kernel and its bytes, and 1 us for a launch and a workspace more.
 // The numbers are those of 600 random sizes (1 to 8192 x 64 to 16384 x 128 to 16384, B in the caches and
 // from memory) with which the choice costs least: on 520 others 0.6 % against the fastest kernel in the
-// mean, up to 16 rows 1.3 %.  Examples,
+// mean, up to 16 rows 1.3 %, on 160 more 0.7 and 0.6 %.  Examples,
 // B from memory, us:                          128 x 128   two per CU   256 x 256   64 x 64
 //   256 x 4096 x 4096                          21.9        30.3         42.7        12.1
 //   1024 x 4096 x 4096                         23.1        31.4         42.4        33.6
@@ -966,11 +965,14 @@ hipError_t launch_gemm_fp8(const GemmFp8Args& g, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Every block quantises the rows of x that it needs, which up to 2^24 weights, and 2^25 for up to 8 tokens,
-// costs no more than a launch of its own (1 and 16 tokens, us, this way / two launches: 512 x 512 2.9 / 4.6
-// and 3.0 / 5.1, 4096 x 4096 7.6 / 8.4 and 9.2 / 9.0, 16384 x 2048 10.5 / 11.2 and 14.5 / 12.2) and beyond
-// more (8 x 8192 x 8192 23.2 / 17.3); likewise up to 2^16 values of x (16 x 1024 x 8192 13.2 / 11.1).  The vector loads of x want its rows at multiples of 16
-// bytes and no row to end inside 16 values.
+// Every block quantises the rows of x that it needs, which takes the place of a launch (1, 4, 8 and 16 tokens, weights
+// from memory, us, this way: 512 x 512 3.0 3.1 3.1 3.1, by two launches 5.1 5.2 5.4 5.5; 4096 x 2048 4.8 5.0 5.1 5.3 and
+// 7.1 7.2 7.3 7.4) until every block's repetition costs as much.  That is near 2^24 weights (4096 x 4096 7.7 7.9 8.1 9.2
+// and 8.3 8.5 8.6 9.0), up to 8 tokens near 2^25 (16384 x 2048 10.1 10.7 11.4 and 11.1 11.4 11.7; 8192 x 4096 11.5 11.9
+// 12.6 and 11.9 12.2 12.4; from the caches 8 tokens 11.2 and 10.3), and beyond it is more (8 x 8192 x 8192 23.2 and 17.3);
+// likewise up to 2^16 values of x (16 x 1024 x 8192 13.2 and 11.1).  The limits cost up to 5 % from memory and 10 % from
+// the caches where they are reached.  The vector loads of x want its rows at multiples of 16 bytes and no row to end
+// inside 16 values.
 bool gemm_fp8_takes_wide(const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K) {
   return M >= 1 && M <= 16 && K >= 1 && K % 16 == 0 && K <= 8192 && M * K <= 65536 &&
          N * K <= (int64_t(1) << (M <= 8 ? 25 : 24)) &&

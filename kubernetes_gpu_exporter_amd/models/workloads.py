@@ -7,7 +7,8 @@ per pod"), so each workload class here reproduces one pod type's GPU signature:
   GemmPod       bf16 MFMA GEMM bursts (our gfx950 kernel, csrc/kernels/gemm_bf16.hip)
                 -> gfx/MFMA busy, power, HBM traffic, VRAM held by one process
                 dtype "fp8": the same product in 8 bits with block scales (ops/fp8.py)
-                -> matrix FLOP/s of operand type fp8, at twice bf16's rate
+                -> matrix FLOP/s of operand type fp8 (the counter reads 2 size^3 a product exactly), at
+                up to twice bf16's rate
   TrainerPod    a GemmPod's compute + one parallelism strategy's collectives per step
                 (parallel/collectives.py: dp tp pp sp ep cp ulysses) -> xGMI per-link
                 traffic + RCCL per-op calls/bytes attributable to the pod

@@ -96,7 +96,7 @@ def align_fp8(q, scale, stream=None):
 
 def transpose_fp8(q, scale, stream=None):
     """The transpose [cols, rows] of a tensor in 8 bits, itself in 8 bits: (q_t, scale_t).  Blocks
-    of 128 x 128 stay what they are.  Blocks of 1 x 128 become blocks of 1 x 128 along the
+    of 128 x 128 stay what they are (a single row's are 1 x 128: its scales have the same shape).  Blocks of 1 x 128 become blocks of 1 x 128 along the
     transpose's own rows: the values are quantised anew from what they stand for, which, both
     scales being powers of two, changes only values below the type's normal range in their new
     block (2^-14 of its largest for e4m3, 2^-29 for e5m2, and less)."""
@@ -138,13 +138,18 @@ def linear_fp8(x, weight, weight_scale=None):
     """y[..., N] = x[..., K] @ weight[N, K]^T in 8 bits, in x's type (bf16 or f16).
 
     Training: `weight` in bf16 or f16.  Both operands are quantised to e4m3 (x in blocks of 1 x 128,
-    the weight 128 x 128).  For the backward pass x is kept as its 8-bit checkpoint, half the memory
-    of the activation; dx = Q(dy) W with the kept 8-bit weight, dW = Q(dy^T) x with the checkpoint
-    transposed (as transpose_fp8 does).  A double backward and forward-mode derivatives are refused.  K is at most 2^22, and so is N
+    the weight 128 x 128).  What the backward pass reads is kept in 8 bits: x's checkpoint where the
+    weight takes a gradient (half the memory of the activation) and the transposed weight where x takes
+    one (in every call: with fewer tokens than outputs the two are more than x in 16 bits);
+    dx = Q(dy) W with the kept 8-bit weight, dW = Q(dy^T) x with the checkpoint
+    transposed (as transpose_fp8 does).  A backward pass computes the gradients asked for.  A double backward and forward-mode derivatives are refused.  K is at most 2^22, and so is N
     where x takes a gradient and the number of x's rows where the weight takes one; each tensor that is quantised, the
     result's gradient among them, has fewer than 2^28 blocks of 128 along its rows.  Sizes that only the backward pass
     would not take are refused before the forward pass.
 
     Serving: `weight` in 8 bits with its `weight_scale`, as quantize_fp8(w, block_rows=128) gives
-    them; x may take a gradient, the weight takes none."""
+    them; x may take a gradient, the weight takes none (its backward pass transposes the weight each time).
+
+    All three products are gemm_fp8's: sums in 32 bits, the matrix instruction drops products 2^-14 and more below
+    the largest of the 32 it adds at once.  Sums may be added in another order than in separate calls."""
     return _native.linear_fp8(x, weight, weight_scale)
