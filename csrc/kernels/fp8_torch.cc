@@ -429,9 +429,10 @@ struct ServeFp8 : torch::autograd::Function<ServeFp8> {
     variable_list results(3);
     {
       at::AutoGradMode off(false);
-      const auto [g, g_scale] = GPUEXP_CALL(quantize_fp8, rows_of(grads[0]), at::kFloat8_e4m3fn, 1);
-      const auto [wt, wt_scale] = GPUEXP_CALL(transpose_fp8, saved[0], saved[1]);
-      results[0] = GPUEXP_CALL(gemm_fp8, g, g_scale, wt, wt_scale, grads[0].scalar_type(), 0, 0);
+      const Pair g = GPUEXP_CALL(quantize_fp8, rows_of(grads[0]), at::kFloat8_e4m3fn, 1);
+      const Pair wt = GPUEXP_CALL(transpose_fp8, saved[0], saved[1]);
+      results[0] = GPUEXP_CALL(gemm_fp8, std::get<0>(g), std::get<1>(g), std::get<0>(wt), std::get<1>(wt),
+                               grads[0].scalar_type(), 0, 0);
     }
     return once(std::move(results));
   }
